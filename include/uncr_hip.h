@@ -566,6 +566,30 @@ int uncr_adam_max_tensors(void);
 int uncr_adam_step(const long long* desc, const long long* grads_host, int n_tensors, const int* chunks, int n_chunks, float lr,
                    const float* lr_dev, double beta1, double beta2, float eps, float weight_decay, hipStream_t stream);
 
+/* ---- packed token sequences (date, row, column tokens of an image time series): rotation, norms of queries and keys, attention ----
+ * Tensors here are token-major rows [tokens][heads][D], D contiguous, with strides in ELEMENTS between tokens (`_ts`) and heads (`_hs`), so
+ * the queries, keys and values of one fused projection are read in place.  act: UNCR_F32 / UNCR_BF16 storage; arithmetic in fp32.
+ *
+ * Rotary positions: pos [N][n_axes] (pos_dt 0 fp32, 1 fp64, 2 int32, 3 int64), n_axes <= 4; axis a owns the next sec_a (even) elements of
+ * the head vector, elements behind the last section pass through.  turns [D / 2] fp64 (device): full turns per unit of position of every
+ * pair in order.  Pairs are (i, i + sec / 2) inside a section, or (2i, 2i + 1) with neighbours != 0.  inverse != 0 rotates back: the
+ * gradient.  Even D <= 256.  y may be x. */
+int uncr_rotary_axes(const void* x, long long x_ts, long long x_hs, void* y, long long y_ts, long long y_hs, const void* pos, int pos_dt,
+                     int n_axes, int sec0, int sec1, int sec2, int sec3, const double* turns, int neighbours, int inverse, int N, int H,
+                     int D, int act, hipStream_t stream);
+/* y = rotate(w * x / sqrt(mean(x^2) + eps)) for queries and keys in one launch; wq, wk [D] fp32; qo [N][Hq][D], ko [N][Hk][D] contiguous */
+int uncr_headnorm_rotary_fwd(const void* q, long long q_ts, long long q_hs, const void* k, long long k_ts, long long k_hs, const float* wq,
+                             const float* wk, float eps, void* qo, void* ko, const void* pos, int pos_dt, int n_axes, int sec0, int sec1,
+                             int sec2, int sec3, const double* turns, int neighbours, int N, int Hq, int Hk, int D, int act,
+                             hipStream_t stream);
+/* gradients dq, dk (contiguous) from gq, gk and the forward's inputs; dwq, dwk [D]; part: float [uncr_headnorm_slots(N)][2][D] workspace */
+int uncr_headnorm_slots(int N);
+int uncr_headnorm_rotary_bwd(const void* q, long long q_ts, long long q_hs, const void* k, long long k_ts, long long k_hs, const float* wq,
+                             const float* wk, float eps, const void* gq, long long gq_ts, long long gq_hs, const void* gk, long long gk_ts,
+                             long long gk_hs, void* dq, void* dk, float* part, float* dwq, float* dwk, const void* pos, int pos_dt,
+                             int n_axes, int sec0, int sec1, int sec2, int sec3, const double* turns, int neighbours, int N, int Hq, int Hk,
+                             int D, int act, hipStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -12,6 +12,7 @@ into per-(frame,channel) coefficients and the consuming kernel applies them in i
 """
 from __future__ import annotations
 
+import contextlib
 import threading
 import weakref
 
@@ -2144,6 +2145,101 @@ def sdpa_rows_backward(dattn: Optional[Tensor], dout: Optional[Tensor], dcomp: O
     else:
         dq = dq_rows
     return dq, dkk, dvv
+
+
+# ------------------------------------------------------------------------------------------------
+# Packed token sequences: rotation, norms of queries and keys, attention (csrc/rotary.hip, csrc/packed_attn*.hip)
+# ------------------------------------------------------------------------------------------------
+
+_POS_DT = {torch.float32: 0, torch.float64: 1, torch.int32: 2, torch.int64: 3}
+
+
+def _on(dev):
+    """The device the tensors live on becomes the current one for a launch (and its stream the launch's stream)."""
+    return contextlib.nullcontext() if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
+
+
+def check_tokens(**tensors):
+    """Token rows [tokens, heads, d]: storage type, common type and device.  Raises before anything is launched."""
+    first = None
+    for name, t in tensors.items():
+        if t.dtype not in (torch.float32, torch.bfloat16):
+            raise RuntimeError(f"{name}: unsupported dtype {t.dtype} (float32 or bfloat16)")
+        first = first if first is not None else (name, t)
+        if t.dtype != first[1].dtype:
+            raise RuntimeError(f"{name} is {t.dtype} but {first[0]} is {first[1].dtype}")
+    check_device(**tensors)
+
+
+def check_device(**tensors):
+    dev = None
+    for name, t in tensors.items():
+        if t is None:
+            continue
+        if not t.is_cuda:
+            raise RuntimeError(f"{name}: uncrtaints_amd kernels need tensors on the GPU (cuda device); there is no CPU path")
+        dev = dev if dev is not None else t.device
+        if t.device != dev:
+            raise RuntimeError(f"{name} is on {t.device}, the other tensors on {dev}")
+
+
+def _token_rows(x: Tensor) -> Tensor:
+    """[tokens, heads, d] with d contiguous; token and head strides stay as they are (a slice of a fused projection is read in place)."""
+    return x if x.stride(-1) == 1 or x.shape[-1] == 1 else x.contiguous()
+
+
+@dataclass
+class RotaryPlan:
+    """What the rotation kernels need beside the tensor: positions [N, axes] and the axes' sections with their turns per unit."""
+    positions: Optional[Tensor] = None
+    sections: Tuple[int, ...] = ()
+    turns: Optional[Tensor] = None
+    neighbours: bool = False
+
+    def args(self):
+        s = tuple(self.sections) + (0,) * (4 - len(self.sections))
+        p = self.positions
+        if p is None:
+            return (None, 0, 0, 0, 0, 0, 0, None, 0)
+        return (p.data_ptr(), _POS_DT[p.dtype], len(self.sections), *s, self.turns.data_ptr(), int(self.neighbours))
+
+
+def rotary_axes(x: Tensor, plan: RotaryPlan, inverse: bool = False) -> Tensor:
+    """x [N, H, D] rotated (back, with `inverse`) by the plan's positions -> contiguous [N, H, D]"""
+    x = _token_rows(x)
+    N, H, D = x.shape
+    with _on(x.device):
+        y = torch.empty((N, H, D), device=x.device, dtype=x.dtype)
+        hb.call("uncr_rotary_axes", x.data_ptr(), x.stride(0), x.stride(1), y.data_ptr(), H * D, D, *plan.args(), int(inverse), N, H, D,
+                _dt(x), _stream())
+    return y
+
+
+def headnorm_rotary_forward(q: Tensor, k: Tensor, wq: Tensor, wk: Tensor, eps: float, plan: RotaryPlan):
+    """q [N, Hq, D], k [N, Hk, D] -> contiguous normalised, rotated (q, k)"""
+    q, k = _token_rows(q), _token_rows(k)
+    N, Hq, D = q.shape
+    Hk = k.shape[1]
+    with _on(q.device):
+        qo, ko = torch.empty((N, Hq, D), device=q.device, dtype=q.dtype), torch.empty((N, Hk, D), device=q.device, dtype=q.dtype)
+        hb.call("uncr_headnorm_rotary_fwd", q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1), wq, wk,
+                float(eps), qo.data_ptr(), ko.data_ptr(), *plan.args(), N, Hq, Hk, D, _dt(q), _stream())
+    return qo, ko
+
+
+def headnorm_rotary_backward(gq: Tensor, gk: Tensor, q: Tensor, k: Tensor, wq: Tensor, wk: Tensor, eps: float, plan: RotaryPlan):
+    """-> dq [N, Hq, D], dk [N, Hk, D] in the storage type, dwq [D], dwk [D] in fp32"""
+    q, k, gq, gk = _token_rows(q), _token_rows(k), _token_rows(gq), _token_rows(gk)
+    N, Hq, D = q.shape
+    Hk = k.shape[1]
+    with _on(q.device):
+        dq, dk = torch.empty((N, Hq, D), device=q.device, dtype=q.dtype), torch.empty((N, Hk, D), device=q.device, dtype=q.dtype)
+        dwq, dwk = _f32((D,), q.device), _f32((D,), q.device)
+        part = _f32((hb.query("uncr_headnorm_slots", N), 2, D), q.device)
+        hb.call("uncr_headnorm_rotary_bwd", q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1), wq, wk,
+                float(eps), gq.data_ptr(), gq.stride(0), gq.stride(1), gk.data_ptr(), gk.stride(0), gk.stride(1), dq.data_ptr(),
+                dk.data_ptr(), part, dwq, dwk, *plan.args(), N, Hq, Hk, D, _dt(q), _stream())
+    return dq, dk, dwq, dwk
 
 
 # ------------------------------------------------------------------------------------------------
