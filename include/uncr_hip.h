@@ -590,6 +590,24 @@ int uncr_headnorm_rotary_bwd(const void* q, long long q_ts, long long q_hs, cons
                              int n_axes, int sec0, int sec1, int sec2, int sec3, const double* turns, int neighbours, int N, int Hq, int Hk,
                              int D, int act, hipStream_t stream);
 
+/* Attention over packed sequences: q [Nq][Hq][D], k / v [Nk][Hk][D], Hq a multiple of Hk (query head i reads key head i / (Hq / Hk)), D <= 128.
+ * Sequence b owns query rows off_q[b] .. off_q[b+1]-1 and key rows off_k[b] .. off_k[b+1]-1, of which k_len[b] (null: all) are used: the rest
+ * is room in a cache.  off_q, off_k [B+1], k_len [B]: int32, device.  causal: row i of Lq sees keys j <= i + Lk - Lq.
+ *   out = softmax(q k^T / temperature) v;  a row that sees nothing: 0.  lse [Nq][Hq] (nullable): log of the row's sum, -inf where it sees
+ *   nothing.  Query rows of no sequence: zeros (lse -inf) with fill != 0, left as they are without.
+ * Offsets are clamped into the tensors on the device.  Rows of no sequence and keys behind k_len are never multiplied. */
+int uncr_packed_attn_fwd(const void* q, long long q_ts, long long q_hs, const void* k, long long k_ts, long long k_hs, const void* v,
+                         long long v_ts, long long v_hs, void* out, long long o_ts, long long o_hs, float* lse, const int* off_q,
+                         const int* off_k, const int* k_len, float temperature, int causal, int fill, int B, int Nq, int Nk, int Hq, int Hk,
+                         int D, int act, hipStream_t stream);
+/* gradients dq, dk, dv (contiguous; zeros for rows of no sequence and keys behind k_len) from dout, the forward's inputs, out and lse;
+ * delta: float [Nq][Hq] workspace */
+int uncr_packed_attn_bwd(const void* q, long long q_ts, long long q_hs, const void* k, long long k_ts, long long k_hs, const void* v,
+                         long long v_ts, long long v_hs, const void* out, long long o_ts, long long o_hs, const void* dout, long long do_ts,
+                         long long do_hs, const float* lse, void* dq, void* dk, void* dv, float* delta, const int* off_q, const int* off_k,
+                         const int* k_len, float temperature, int causal, int B, int Nq, int Nk, int Hq, int Hk, int D, int act,
+                         hipStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,454 @@
+"""Attention over packed sequences (packed_attention.PackedAttention) against softmax(q k^T / temperature) v in 64 bits, sequence by sequence.
+
+Tolerances, fixed before the first run; u = 2^-24 (fp32 half step), h = finfo(storage).eps / 2 (a rounding to the storage type), r = h for bf16
+storage and 0 for fp32 (there the probabilities are rounded to bf16 before they are multiplied), n = number of keys (rows) summed:
+  score      a dot product of d terms in fp32, the scale, the exponent's argument:  e = (d + 8) u max_j sum|q k_j| / temperature
+  p          relative: e_p = 2 e + (n + 32) u + 2 u |lse|       (its own score, the reference's, the sum of n terms, exp2 and log2)
+  out        (e_p + r + n u) sum p |v| + h |out|
+  lse        e + (n + 32) u + 2 u |lse|
+  dS         p (e_p |dP - delta| + (d + 8) u sum|dO v| + e_delta) + r |dS|,   e_delta = sum |dO| (error of out) + (d + 8) u sum |dO out|
+  dQ, dK     the sum over dS' error times |k| (|q|), n u of the absolute sum, + h |result|;   dV = p^T dO alike with p (e_p + r + n u)
+  underflow  a probability, and a dS, below the smallest normal number 2^-126 may be flushed to 0: an absolute error of at most 2^-126 in each
+             p and of 2^-126 (|dP - delta| + 1) in each dS, through the same sums.  (Scores of several hundred leave such probabilities, and
+             their exact gradients of 1e-37 are in range: seen with test_large_scores_and_a_temperature.)"""
+import math
+
+import pytest
+import torch
+
+U = 2.0 ** -24
+DEV = "cuda"
+gpu = pytest.mark.gpu
+
+
+def _gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+def reference(q, k, v, do, causal, temperature, dtype):
+    """One sequence and one group: q [G, Lq, D], k / v [Lk, D] in fp64 -> dict of (value, bound)"""
+    G, lq, d = q.shape
+    lk = k.shape[0]
+    h = torch.finfo(dtype).eps / 2
+    r = h if dtype == torch.bfloat16 else 0.0
+    if lk == 0 or lq == 0:
+        z, zk = torch.zeros_like(q), torch.zeros_like(k)
+        return dict(out=(z, z), lse=(torch.full((G, lq), -math.inf, dtype=torch.float64), z[..., 0]), dq=(z, z), dk=(zk, zk), dv=(zk, zk))
+    s = q @ k.T / temperature
+    see = torch.ones(lq, lk, dtype=torch.bool)
+    if causal:
+        see = torch.arange(lk)[None] <= torch.arange(lq)[:, None] + (lk - lq)
+    none = ~see.any(1)
+    lse = torch.logsumexp(s.masked_fill(~see, -math.inf), -1)
+    p = torch.exp(s - lse.masked_fill(none, 0.0)[..., None]).masked_fill(~see, 0.0)
+    out = p @ v
+    e = (d + 8) * U * ((q.abs() @ k.abs().T / temperature).masked_fill(~see, 0.0)).amax(-1)
+    base = lse.masked_fill(none, 0.0).abs()
+    ep = 2 * e + (lk + 32) * U + 2 * U * base
+    flush = 2.0 ** -126 * see.double()
+    b_out = (ep + r + lk * U)[..., None] * (p @ v.abs()) + h * out.abs() + flush @ v.abs()
+    res = dict(out=(out, b_out), lse=(lse, e + (lk + 32) * U + 2 * U * base))
+    dp = do @ v.T
+    delta = (do * out).sum(-1, keepdim=True)
+    ds = p * (dp - delta)
+    e_delta = (do.abs() * b_out).sum(-1, keepdim=True) + (d + 8) * U * (do * out).abs().sum(-1, keepdim=True)
+    e_ds = p * (ep[..., None] * (dp - delta).abs() + (d + 8) * U * (do.abs() @ v.abs().T) + e_delta) + r * ds.abs() + flush * ((dp - delta).abs() + 1)
+    dq = ds @ k / temperature
+    res["dq"] = (dq, (e_ds @ k.abs() + lk * U * (ds.abs() @ k.abs())) / temperature + (h + 2 * U) * dq.abs())
+    n = G * lq
+    dk = (ds.transpose(1, 2) @ q).sum(0) / temperature
+    res["dk"] = (dk, ((e_ds.transpose(1, 2) @ q.abs()).sum(0) + n * U * (ds.abs().transpose(1, 2) @ q.abs()).sum(0)) / temperature
+                 + (h + 2 * U) * dk.abs())
+    dv = (p.transpose(1, 2) @ do).sum(0)
+    res["dv"] = (dv, ((p * (ep + r + n * U)[..., None] + flush).transpose(1, 2) @ do.abs()).sum(0) + (h + 2 * U) * dv.abs())
+    return res
+
+
+def _check(name, got, ref, bound):
+    got, tiny = got.detach().cpu().double(), 2.0 ** -126
+    bad = ~((got - ref).abs() <= bound + tiny) & ~((got == ref) & torch.isinf(ref))
+    assert not bad.any(), (name, int(bad.sum()), bad.numel(), bad.nonzero()[0].tolist(), float(got[bad][0]), float(ref[bad][0]), float(bound[bad][0]))
+
+
+def _offsets(lengths, front=0):
+    return torch.tensor([front] + [front + sum(lengths[:i + 1]) for i in range(len(lengths))], dtype=torch.int32)
+
+
+def _run(lq, lk, hq, hk, d, causal, dtype, room=None, front=0, behind=0, temperature=None, train=True, scale=1.0, layout="plain", seed=0, hints=True):
+    """lq, lk: lengths; room: rows each key sequence owns (>= lk, or None); front / behind: rows of no sequence.  Everything outside is NaN."""
+    from uncrtaints_amd.src.backbones.packed_attention import PackedAttention
+    own = room if room is not None else lk
+    off_q, off_k = _offsets(lq, front), _offsets(own, front)
+    nq, nk = int(off_q[-1]) + behind, int(off_k[-1]) + behind
+    g = _gen(seed)
+    q, k, v, do = (torch.randn(n, heads, d, generator=g) for n, heads in ((nq, hq), (nk, hk), (nk, hk), (nq, hq)))
+    q *= scale
+    used_q, used_k = torch.zeros(nq, dtype=torch.bool), torch.zeros(nk, dtype=torch.bool)
+    for b in range(len(lq)):
+        used_q[off_q[b]:off_q[b] + lq[b]] = True
+        used_k[off_k[b]:off_k[b] + lk[b]] = True
+    q[~used_q], do[~used_q], k[~used_k], v[~used_k] = math.nan, math.nan, math.nan, math.nan
+    q, k, v, do = (t.to(dtype) for t in (q, k, v, do))
+
+    def place(t):
+        if layout == "heads_first":
+            return t.to(DEV).transpose(0, 1).contiguous().transpose(0, 1)
+        if layout == "odd_start":
+            z = torch.empty(t.shape[0], t.shape[1] * d + 3, dtype=dtype, device=DEV)
+            z[:, 1:1 + t.shape[1] * d] = t.to(DEV).flatten(1)
+            return z[:, 1:1 + t.shape[1] * d].unflatten(1, (t.shape[1], d))
+        if layout == "fused":
+            z = torch.full((t.shape[0], t.shape[1] + 2, d), math.nan, dtype=dtype, device=DEV)
+            z[:, 1:-1] = t.to(DEV)
+            return z[:, 1:-1]
+        if layout == "last_strided":
+            z = torch.empty(t.shape[0], t.shape[1], 2 * d, dtype=dtype, device=DEV)
+            z[..., ::2] = t.to(DEV)
+            return z[..., ::2]
+        return t.to(DEV)
+
+    m = PackedAttention(causal=causal, temperature=temperature)
+    temp = temperature if temperature is not None else math.sqrt(d)
+    qd, kd, vd = (place(t).detach().requires_grad_(train) for t in (q, k, v))
+    k_len = torch.tensor(lk, dtype=torch.int32, device=DEV) if room is not None else None
+    hint = dict(max_q=max(lq), max_k=max(lk)) if hints else {}
+    out, lse = m(qd, kd, vd, off_q.to(DEV), off_k.to(DEV), k_len=k_len, return_lse=True, **hint)
+    grads = torch.autograd.grad(out, (qd, kd, vd), place(do)) if train else ()
+    want = {n: (torch.zeros(*sh, dtype=torch.float64), torch.zeros(*sh, dtype=torch.float64))
+            for n, sh in dict(out=q.shape, dq=q.shape, dk=k.shape, dv=k.shape, lse=(nq, hq)).items()}
+    want["lse"][0].fill_(-math.inf)
+    G = hq // hk
+    for b in range(len(lq)):
+        rq, rk = slice(int(off_q[b]), int(off_q[b]) + lq[b]), slice(int(off_k[b]), int(off_k[b]) + lk[b])
+        for c in range(hk):
+            hs = slice(c * G, (c + 1) * G)
+            ref = reference(q[rq, hs].double().transpose(0, 1), k[rk, c].double(), v[rk, c].double(), do[rq, hs].double().transpose(0, 1), causal,
+                            temp, dtype)
+            for i in (0, 1):
+                want["out"][i][rq, hs], want["dq"][i][rq, hs] = ref["out"][i].transpose(0, 1), ref["dq"][i].transpose(0, 1)
+                want["lse"][i][rq, hs] = ref["lse"][i].T
+                want["dk"][i][rk, c], want["dv"][i][rk, c] = ref["dk"][i], ref["dv"][i]
+    assert out.dtype == dtype and lse.dtype == torch.float32 and not lse.requires_grad
+    _check("lse", lse, *want["lse"])
+    _check("out", out, *want["out"])
+    for name, t in zip(("dq", "dk", "dv"), grads):
+        assert t.dtype == dtype
+        _check(name, t, *want[name])
+    return out
+
+
+BOTH = pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+MASK = pytest.mark.parametrize("causal", [False, True])
+
+
+@gpu
+@MASK
+@BOTH
+@pytest.mark.parametrize("n", [1, 2, 31, 32, 33, 63, 64, 65, 127, 128, 129, 255, 257])
+def test_one_sequence_lengths(n, dtype, causal):
+    _run([n], [n], 2, 1, 32, causal, dtype)
+
+
+@gpu
+@MASK
+@BOTH
+@pytest.mark.parametrize("d", [1, 3, 4, 8, 16, 20, 33, 40, 64, 72, 96, 100, 128])
+def test_head_sizes(d, dtype, causal):
+    _run([70, 3, 131], [70, 3, 131], 4, 2, d, causal, dtype, seed=d)
+
+
+@gpu
+@MASK
+@BOTH
+@pytest.mark.parametrize("hq,hk", [(1, 1), (3, 1), (6, 2), (8, 8), (16, 2), (35, 5), (40, 1)])
+def test_head_groups(hq, hk, dtype, causal):
+    _run([45, 0, 7, 100], [45, 0, 7, 100], hq, hk, 64, causal, dtype, seed=hq)
+
+
+@gpu
+@MASK
+@BOTH
+def test_lengths_that_differ_between_queries_and_keys(dtype, causal):
+    """More keys than queries (a cache), fewer (the first rows see nothing under the causal mask), none on either side."""
+    _run([5, 40, 33, 0, 9, 70], [200, 10, 33, 8, 0, 65], 6, 3, 64, causal, dtype)
+
+
+@gpu
+@MASK
+@BOTH
+@pytest.mark.parametrize("d", [16, 128])
+def test_rows_of_no_sequence_and_room_in_the_cache_are_never_read(d, dtype, causal):
+    """NaN in front of, behind and between the sequences' used rows leaves no trace, in the gradients either."""
+    _run([12, 1, 90], [50, 0, 77], 4, 2, d, causal, dtype, room=[64, 5, 80], front=3, behind=37)
+
+
+@gpu
+@BOTH
+@pytest.mark.parametrize("layout", ["fused", "heads_first", "odd_start", "last_strided"])
+@pytest.mark.parametrize("d", [32, 128])
+def test_layouts(layout, d, dtype):
+    _run([33, 80], [33, 80], 4, 2, d, True, dtype, layout=layout)
+
+
+@gpu
+@MASK
+@BOTH
+@pytest.mark.parametrize("batch", [64, 65, 700, 5000])
+def test_many_short_sequences(batch, dtype, causal):
+    lengths = torch.randint(0, 5, (batch,), generator=_gen(batch)).tolist()
+    _run(lengths, lengths, 2, 1, 16, causal, dtype)
+
+
+@gpu
+@MASK
+@BOTH
+@pytest.mark.parametrize("d", [32, 64, 128])
+def test_longer_sequences(d, dtype, causal):
+    _run([1030, 517], [1030, 517], 4, 2, d, causal, dtype)
+
+
+@gpu
+@BOTH
+def test_large_scores_and_a_temperature(dtype):
+    """Scores of +-several hundred: the running maximum is passed by many powers of two from tile to tile."""
+    _run([300], [300], 2, 2, 64, True, dtype, scale=40.0, temperature=2.0)
+
+
+@gpu
+@BOTH
+@pytest.mark.parametrize("hq,hk,d", [(1, 1, 64), (8, 2, 128), (16, 1, 64), (40, 1, 32), (6, 2, 20), (12, 4, 4)])
+@pytest.mark.parametrize("lens", [[1], [1000], [5, 1, 300, 64, 2000], [0, 129]])
+def test_single_tokens_over_a_cache(lens, hq, hk, d, dtype):
+    _run([1] * len(lens), lens, hq, hk, d, True, dtype, room=[n + 9 for n in lens], train=False)
+
+
+@gpu
+@BOTH
+@pytest.mark.parametrize("lq", [[2, 3, 1], [1, 0, 9], [40, 1, 1]])
+@pytest.mark.parametrize("hints", [True, False])
+def test_a_few_tokens_over_a_cache(lq, hints, dtype):
+    _run(lq, [700, 40, 1025], 8, 2, 64, True, dtype, room=[704, 41, 1030], train=False, front=2, behind=3, hints=hints)
+
+
+@gpu
+@BOTH
+def test_hints_that_are_too_small_change_nothing(dtype):
+    from uncrtaints_amd.src.backbones.packed_attention import PackedAttention, pack_offsets
+    q, k, v = (torch.randn(300, n, 64, generator=_gen(n)).to(dtype).to(DEV) for n in (4, 2, 3))
+    v = v[:, :2]
+    off = pack_offsets([200, 100], DEV)
+    m = PackedAttention(causal=True)
+    a, b = m(q, k, v, off), m(q, k, v, off, max_q=1, max_k=1)
+    assert float((a.float() - b.float()).abs().max()) <= 4 * torch.finfo(dtype).eps * float(v.float().abs().max())
+
+
+@gpu
+def test_gradients_against_differences():
+    """fp32: (f(x + t w) - f(x - t w)) / 2t along random directions, t = 1e-2, f summed in fp64.  The third-order term t^2 / 6 and the forward's
+    noise 1e-6 / t = 1e-4 per value, both random over 97 x 4 x 32 values, stay far below 1e-2 of the slope's scale sqrt(values)."""
+    from uncrtaints_amd.src.backbones.packed_attention import PackedAttention, pack_offsets
+    off = pack_offsets([60, 37], DEV)
+    x = [torch.randn(97, n, 32, generator=_gen(50 + n)).to(DEV) for n in (4, 2, 2)]
+    w = [torch.randn(97, n, 32, generator=_gen(60 + n)).to(DEV) for n in (4, 2, 2)]
+    g = torch.randn(97, 4, 32, generator=_gen(70)).to(DEV)
+    for causal in (False, True):
+        m = PackedAttention(causal=causal)
+        f = lambda z: (m(*z, off).double() * g.double()).sum()
+        leaves = [t.clone().requires_grad_() for t in x]
+        grads = torch.autograd.grad(m(*leaves, off), leaves, g)
+        for i in range(3):
+            t = 1e-2
+            up, dn = list(x), list(x)
+            up[i], dn[i] = x[i] + t * w[i], x[i] - t * w[i]
+            slope = float((grads[i].double() * w[i].double()).sum())
+            assert abs(slope - float(f(up) - f(dn)) / (2 * t)) < 1e-2 * math.sqrt(97 * 4 * 32), (causal, i)
+
+
+@gpu
+@BOTH
+def test_given_out_keeps_rows_of_no_sequence(dtype):
+    from uncrtaints_amd.src.backbones.packed_attention import PackedAttention
+    q = torch.randn(20, 4, 16, generator=_gen(1)).to(dtype).to(DEV)
+    off = torch.tensor([3, 8, 15], dtype=torch.int32, device=DEV)
+    m = PackedAttention()
+    out = torch.full_like(q, 7.0)
+    res = m(q, q, q, off, out=out)
+    new = m(q, q, q, off)
+    assert res.data_ptr() == out.data_ptr() and torch.equal(out[3:15], new[3:15])
+    assert (out[:3] == 7).all() and (out[15:] == 7).all() and (new[:3] == 0).all() and (new[15:] == 0).all()
+
+
+@gpu
+@BOTH
+def test_offsets_outside_the_tensors_are_clamped(dtype):
+    from uncrtaints_amd.src.backbones.packed_attention import PackedAttention
+    q = torch.randn(20, 2, 16, generator=_gen(1)).to(dtype).to(DEV)
+    m = PackedAttention(causal=True)
+    good = m(q, q, q, torch.tensor([0, 9, 20], dtype=torch.int32, device=DEV))
+    bad = m(q, q, q, torch.tensor([-5, 9, 2 ** 31 - 1], dtype=torch.int32, device=DEV), k_len=torch.tensor([9, 2 ** 31 - 1], dtype=torch.int32, device=DEV))
+    assert torch.equal(good, bad)
+    x = q.clone().requires_grad_()
+    for off in ([0, 15, 4], [30, 40, 50], [-9, -3, -1]):       # wrong rows at worst, nothing outside
+        off = torch.tensor(off, dtype=torch.int32, device=DEV)
+        y = m(x, x, x, off, k_len=torch.tensor([-4, 100], dtype=torch.int32, device=DEV))
+        torch.autograd.grad(y, x, torch.ones_like(y))
+    torch.cuda.synchronize()
+
+
+@gpu
+@BOTH
+def test_results_do_not_depend_on_the_run(dtype):
+    from uncrtaints_amd.src.backbones.packed_attention import PackedAttention, pack_offsets
+    off = pack_offsets([500, 0, 900, 20], DEV)
+    x = [torch.randn(1420, n, 64, generator=_gen(n)).to(dtype).to(DEV).requires_grad_() for n in (8, 2, 2)]
+    g = torch.randn(1420, 8, 64, generator=_gen(9)).to(dtype).to(DEV)
+    runs = []
+    for _ in range(3):
+        y = PackedAttention(causal=True)(*x, off)
+        runs.append((y.detach(),) + torch.autograd.grad(y, x, g))
+    assert all(torch.equal(a, b) for r in runs[1:] for a, b in zip(runs[0], r))
+
+
+@gpu
+@BOTH
+def test_whole_path_trains_serves_and_replays(dtype):
+    """Projection -> norms and rotation -> attention, as a token stage uses them: the whole series at once, its last token over the cache, and
+    both from a captured graph with other lengths and values put into the same buffers."""
+    from uncrtaints_amd.src.backbones.packed_attention import HeadNormRotary, PackedAttention, pack_offsets
+    from uncrtaints_amd.src.backbones.positional_encoding import RotaryAxes
+    heads, kv, d, lengths, room = 8, 2, 32, [37, 64, 5], 70
+    norms = HeadNormRotary(d, rotary=RotaryAxes(d, sections=(8, 12, 12), T=(10000.0, 100.0, 100.0))).to(DEV)
+    attend = PackedAttention(causal=True)
+    n = sum(lengths)
+    qkv = torch.randn(n, heads + 2 * kv, d, generator=_gen(3)).to(dtype).to(DEV).requires_grad_()
+    pos = torch.stack([torch.arange(n) // 8, torch.arange(n) % 8, torch.arange(n) % 5], 1).to(torch.int32).to(DEV)
+    off = pack_offsets(lengths, DEV)
+    g = torch.randn(n, heads, d, generator=_gen(4)).to(dtype).to(DEV)
+
+    def step():
+        q, k = norms(qkv[:, :heads], qkv[:, heads:heads + kv], pos)
+        y = attend(q, k, qkv[:, heads + kv:], off, max_q=64)
+        # detached: a captured graph's outputs do not keep an autograd graph of these leaves alive
+        return (y.detach(), k.detach()) + torch.autograd.grad(y, (qkv, norms.q_weight, norms.k_weight), g)
+
+    eager = [t.detach().clone() for t in step()]
+    assert all(torch.isfinite(t).all() for t in eager)
+    # serving: the last token of every series over a cache that holds the others
+    cache_k = torch.full((3, room, kv, d), math.nan, dtype=dtype, device=DEV)
+    cache_v = torch.full_like(cache_k, math.nan)
+    for b, ln in enumerate(lengths):
+        at = int(off[b])
+        cache_k[b, :ln], cache_v[b, :ln] = eager[1][at:at + ln], qkv.detach()[at:at + ln, heads + kv:]
+    last = off[1:].long() - 1
+    one = torch.arange(4, device=DEV, dtype=torch.int32)
+    with torch.no_grad():
+        q1, _ = norms(qkv[last, :heads], qkv[last, heads:heads + kv], pos[last])
+    k_len = torch.tensor(lengths, dtype=torch.int32, device=DEV)
+
+    def serve():
+        return attend(q1, cache_k.view(3 * room, kv, d), cache_v.view(3 * room, kv, d), one, one * room, k_len=k_len, max_q=1, max_k=64)
+
+    served = serve()
+    assert float((served.float() - eager[0][last].float()).abs().max()) < (0.05 if dtype == torch.bfloat16 else 1e-5)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = step() + (serve(),)
+    for i in range(4):
+        with torch.no_grad():
+            if i == 2:
+                qkv.mul_(-1.0)
+                off.copy_(pack_offsets([1, 80, 25], DEV))
+                k_len.copy_(torch.tensor([5, 9, 5], dtype=torch.int32, device=DEV))
+        want = [t.detach().clone() for t in step()] + [serve().clone()]
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(want, held):
+            assert torch.equal(a, b), i
+        if i < 2:
+            assert all(torch.equal(a, b) for a, b in zip(eager, want))
+
+
+@gpu
+def test_two_streams_at_once():
+    from uncrtaints_amd.src.backbones.packed_attention import PackedAttention, pack_offsets
+    m = PackedAttention(causal=True)
+    off = [pack_offsets([1] * 4, DEV), pack_offsets([3000, 2000, 10, 400], DEV)]
+    x = [torch.randn(5410, n, 64, generator=_gen(n)).to(torch.bfloat16).to(DEV) for n in (8, 2, 2)]
+    qs = [torch.randn(4, 8, 64, generator=_gen(20 + i)).to(torch.bfloat16).to(DEV) for i in range(2)]
+    want = [m(q, x[1], x[2], off[0], off[1], max_q=1) for q in qs]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [[], []]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    for _ in range(5):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(m(qs[i], x[1], x[2], off[0], off[1], max_q=1))
+    torch.cuda.synchronize()
+    assert all(torch.equal(g, want[i]) for i in range(2) for g in got[i])
+
+
+def test_packed_attention_refuses():
+    from uncrtaints_amd.src.backbones.packed_attention import PackedAttention, pack_offsets
+    for t in (0.0, -1.0, math.nan, math.inf):
+        with pytest.raises(ValueError):
+            PackedAttention(temperature=t)
+    with pytest.raises(ValueError):
+        pack_offsets([3, -1], "cpu")
+    m = PackedAttention()
+    q, k, off = torch.zeros(6, 4, 8), torch.zeros(6, 2, 8), pack_offsets([2, 4], "cpu")
+    assert off.tolist() == [0, 2, 6] and off.dtype == torch.int32
+    for args, kw in (((q[0], k, k, off), {}), ((q, k, k[:5], off), {}), ((q, k, k[..., :4], off), {}), ((q[..., :4], k, k, off), {}),
+                     ((torch.zeros(6, 4, 129), torch.zeros(6, 2, 129), torch.zeros(6, 2, 129), off), {}),
+                     ((q[:, :3], k, k, off), {}), ((q, k[:, :0], k[:, :0], off), {}), ((q[:4], k, k, off), {}),
+                     ((q, k, k, off.long()), {}), ((q, k, k, off.view(1, 3)), {}), ((q, k, k, off[::2]), {}), ((q, k, k, off, off[:2]), {}),
+                     ((q, k, k, off[:1]), {}), ((q, k, k, off), dict(k_len=off)), ((q, k, k, off), dict(k_len=off[:2].float())),
+                     ((q, k, k, off), dict(max_q=-1))):
+        with pytest.raises(ValueError):
+            m(*args, **kw)
+    with pytest.raises(RuntimeError, match="unsupported dtype"):
+        m(q.half(), k.half(), k.half(), off)
+    with pytest.raises(RuntimeError, match="but q is"):
+        m(q, k.bfloat16(), k, off)
+    with pytest.raises(RuntimeError, match="cuda device"):
+        m(q, k, k, off)
+
+
+@gpu
+def test_packed_attention_refuses_on_the_gpu():
+    from uncrtaints_amd.src.backbones.packed_attention import PackedAttention, pack_offsets
+    m = PackedAttention()
+    q, off = torch.zeros(6, 4, 8, device=DEV), pack_offsets([2, 4], DEV)
+    with pytest.raises(RuntimeError, match="offsets_q"):
+        m(q, q, q, off.cpu())
+    with pytest.raises(ValueError, match="without gradients"):
+        m(q.clone().requires_grad_(), q, q, off, out=torch.empty_like(q))
+    with pytest.raises(ValueError, match="contiguous"):
+        m(q, q, q, off, out=torch.empty(6, 4, 16, device=DEV)[..., :8])
+    with pytest.raises(RuntimeError, match="but q is"):
+        m(q, q, q, off, out=torch.empty_like(q, dtype=torch.bfloat16))
+
+
+def test_entry_points_refuse_bad_sizes():
+    """The C entries' own checks: no GPU is needed, nothing is enqueued."""
+    from uncrtaints_amd import hip_backend as hb
+    fwd = hb.lib().fn["uncr_packed_attn_fwd"]
+    names = [n for _, n in hb.parse_header()["uncr_packed_attn_fwd"]]
+    ok = dict.fromkeys(names, 0)
+    ok.update(q=16, k=16, v=16, out=16, off_q=16, off_k=16, lse=None, k_len=None, temperature=1.0, B=1, Nq=0, Nk=4, Hq=4, Hk=2, D=8, stream=None)
+    if "work" in ok:
+        ok["work"] = None
+    call = lambda **kw: fwd(*{**ok, **kw}.values())
+    assert call() == 0
+    for kw in (dict(B=0), dict(Nq=-1), dict(Nk=-1), dict(Hq=3), dict(Hk=0), dict(D=0), dict(D=129), dict(act=2), dict(temperature=0.0), dict(temperature=math.nan),
+               dict(off_q=None), dict(off_k=None), dict(Nq=1 << 30, Hq=8), dict(Nq=2, q=None), dict(Nq=2, out=None), dict(Nq=2, k=None),
+               dict(Nq=2, out=18)):
+        assert call(**kw) < 0, kw
+    bwd = hb.lib().fn["uncr_packed_attn_bwd"]
+    names = [n for _, n in hb.parse_header()["uncr_packed_attn_bwd"]]
+    ok2 = dict.fromkeys(names, 0)
+    ok2.update(q=16, k=16, v=16, out=16, dout=16, lse=16, dq=16, dk=16, dv=16, delta=16, off_q=16, off_k=16, k_len=None, temperature=1.0, B=1, Nq=2, Nk=2, Hq=4,
+               Hk=2, D=8, stream=None)
+    for kw in (dict(Hq=5), dict(D=200), dict(lse=None), dict(delta=None), dict(dq=None), dict(dk=None), dict(v=None), dict(dk=24 - 4), dict(act=-1)):
+        assert bwd(*{**ok2, **kw}.values()) < 0, kw

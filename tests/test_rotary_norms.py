@@ -233,7 +233,7 @@ def test_rotary_and_norms_replay_from_a_graph_and_run_on_a_side_stream():
 
     def step():
         a, b = m(qr[:, :4], qr[:, 4:], pos)
-        return (a, b) + torch.autograd.grad((a, b), (qr, m.q_weight, m.k_weight), (g[:, :4], g[:, 4:]))
+        return (a.detach(), b.detach()) + torch.autograd.grad((a, b), (qr, m.q_weight, m.k_weight), (g[:, :4], g[:, 4:]))
 
     eager = [t.detach().clone() for t in step()]
     side = torch.cuda.Stream()

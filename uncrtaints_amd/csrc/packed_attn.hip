@@ -1,0 +1,183 @@
+// Forward of the attention over packed token sequences (see packed_attn.h for the layout of a product):
+//   S = Q K^T / temperature over the keys a row may see (its own sequence; causal: key j <= i + Lk - Lq),  out = softmax(S) V
+// One pass over the keys with the running maximum m and sum l of each row, in fp32 and in powers of two.  m is only a reference for the
+// exponents: it is moved -- and out, l rescaled -- when a tile's maximum passes it by more than 8, so the accumulators are rarely touched
+// and exponentials stay below 2^8.  Rows that see nothing: out = 0, lse = -inf.
+#include "packed_attn.h"
+
+namespace {
+
+template <typename T, int DP, int NW, int TK, bool VEC>
+__global__ __launch_bounds__(NW * 64) void packed_attn_fwd_kernel(const AttnGeom g, const AttnTensor q, const AttnTensor k, const AttnTensor v,
+                                                                  T* __restrict__ out, long long o_ts, long long o_hs,
+                                                                  float* __restrict__ lse, int slots) {
+    typedef AttnTile<T, DP> L;
+    constexpr int NT = NW * 64, BM = NW * 32, SHIFT = NW == 8 ? 8 : NW == 4 ? 7 : NW == 2 ? 6 : 5;
+    __shared__ alignas(16) char lds_k[2][TK * L::RB], lds_v[2][TK * L::RB];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5, col = lane & 31;
+    if (g.fill) attn_fill_outside<T>(g.off_q, g.B, g.Nq, out, o_ts, o_hs, g.Hq, g.D, lse, blockIdx.x, gridDim.x);
+    const int hk = blockIdx.x % g.Hk;
+    int b, tile;
+    // the last tiles of a causal sequence are the longest: they start first
+    if (!attn_find(g.off_q, g.B, g.Nq, g.G, SHIFT, slots - 1 - (int)(blockIdx.x / g.Hk), b, tile)) return;
+    const AttnSeq s = attn_seq(g, b);
+    const int rows = s.lq * g.G;
+    if (tile * BM >= rows) return;
+    const int row0 = tile * BM + wave * 32;
+    const int row = min(row0 + col, rows - 1), tok = row / g.G, head = hk * g.G + row - tok * g.G;
+    // keys [0, limit) are visible to this lane's row
+    const int shift = s.lk - s.lq;
+    auto limit_of = [&](int r) { return g.causal ? min(max(min(r, rows - 1) / g.G + shift + 1, 0), s.lk) : s.lk; };
+    const int limit = limit_of(row);
+    const int wave_lo = limit_of(row0), wave_hi = row0 < rows ? limit_of(row0 + 31) : 0, block_hi = limit_of(tile * BM + BM - 1);
+
+    typename L::Frag qf[L::KS];
+    {
+        const T* qr = (const T*)q.p + (size_t)(s.q0 + tok) * q.ts + (size_t)head * q.hs;
+#pragma unroll
+        for (int i = 0; i < L::KS; ++i) qf[i] = L::template fetch<VEC>(qr, 2 * i + h, g.D);
+    }
+    f32x16 acc[L::DB];
+#pragma unroll
+    for (int db = 0; db < L::DB; ++db) acc[db] = (f32x16)(0.f);
+    float m = -INFINITY, l = 0.f;
+
+    const T* kb = (const T*)k.p + (size_t)s.k0 * k.ts + (size_t)hk * k.hs;
+    const T* vb = (const T*)v.p + (size_t)s.k0 * v.ts + (size_t)hk * v.hs;
+    const int tiles = (block_hi + TK - 1) / TK;
+    AttnStage<T, DP, TK, NT, VEC> ks, vs;
+    if (tiles) {
+        ks.fetch(kb, k.ts, 0, s.lk - 1, g.D);
+        vs.fetch(vb, v.ts, 0, s.lk - 1, g.D);
+        ks.store(lds_k[0]);
+        vs.store(lds_v[0]);
+    }
+    __syncthreads();
+    for (int it = 0; it < tiles; ++it) {
+        const int j0 = it * TK;
+        if (it + 1 < tiles) {
+            ks.fetch(kb, k.ts, j0 + TK, s.lk - 1, g.D);
+            vs.fetch(vb, v.ts, j0 + TK, s.lk - 1, g.D);
+        }
+        if (j0 < wave_hi) {
+            const char* tk = lds_k[it & 1];
+            const char* tv = lds_v[it & 1];
+            f32x16 sc[TK / 32];
+#pragma unroll
+            for (int t = 0; t < TK / 32; ++t) {
+                sc[t] = (f32x16)(0.f);
+#pragma unroll
+                for (int i = 0; i < L::KS; ++i) attn_mma(sc[t], L::frag(tk, t * 32 + col, i, h), qf[i]);
+            }
+            if (j0 + TK > wave_lo) {
+#pragma unroll
+                for (int t = 0; t < TK / 32; ++t)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        if (j0 + t * 32 + 8 * (i / 4) + 4 * h + i % 4 >= limit) sc[t][i] = -INFINITY;
+            }
+            float mx = sc[0][0];
+#pragma unroll
+            for (int t = 0; t < TK / 32; ++t)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) mx = fmaxf(mx, sc[t][i]);
+            mx = fmaxf(mx, attn_other_half(mx)) * g.c;
+            if (__any(mx > m + 8.f)) {
+                const float mn = fmaxf(m, mx), f = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+                m = mn;
+                l *= f;
+#pragma unroll
+                for (int db = 0; db < L::DB; ++db)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) acc[db][i] *= f;
+            }
+            const float ref = m == -INFINITY ? 0.f : m;
+#pragma unroll
+            for (int t = 0; t < TK / 32; ++t) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    sc[t][i] = __builtin_amdgcn_exp2f(fmaf(sc[t][i], g.c, -ref));
+                    l += sc[t][i];
+                }
+                AttnProb<T> p;
+                p.set(sc[t]);
+#pragma unroll
+                for (int db = 0; db < L::DB; ++db) attn_mma_t<DP>(acc[db], tv, t * 32, db, lane, p);
+            }
+        }
+        if (it + 1 < tiles) {
+            ks.store(lds_k[(it + 1) & 1]);
+            vs.store(lds_v[(it + 1) & 1]);
+        }
+        __syncthreads();
+    }
+    l += attn_other_half(l);
+    if (row0 + col >= rows) return;
+    const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
+    attn_store_row<T, L::DB>(out + (size_t)(s.q0 + tok) * o_ts + (size_t)head * o_hs, acc, inv, h, g.D);
+    if (lse && h == 0) lse[(size_t)(s.q0 + tok) * g.Hq + head] = l > 0.f || l != l ? (m + __builtin_amdgcn_logf(l)) * 0.69314718055994531f : -INFINITY;
+}
+
+template <typename T, int DP, int NW, int TK>
+void launch(const AttnGeom& g, const AttnTensor& q, const AttnTensor& k, const AttnTensor& v, void* out, long long o_ts, long long o_hs, float* lse,
+            bool vec, hipStream_t stream) {
+    constexpr int SHIFT = NW == 8 ? 8 : 7;
+    const int slots = attn_slots((long long)g.Nq * g.G, g.B, SHIFT);
+    if (vec) hipLaunchKernelGGL((packed_attn_fwd_kernel<T, DP, NW, TK, true>), dim3(slots * g.Hk), dim3(NW * 64), 0, stream, g, q, k, v, (T*)out, o_ts, o_hs, lse, slots);
+    else hipLaunchKernelGGL((packed_attn_fwd_kernel<T, DP, NW, TK, false>), dim3(slots * g.Hk), dim3(NW * 64), 0, stream, g, q, k, v, (T*)out, o_ts, o_hs, lse, slots);
+}
+
+}  // namespace
+
+int attn_geom(AttnGeom& g, const int* off_q, const int* off_k, const int* k_len, float temperature, int causal, int B, int Nq, int Nk, int Hq,
+              int Hk, int D, int act) {
+    if (B <= 0 || Nq < 0 || Nk < 0 || Hq <= 0 || Hk <= 0 || Hq % Hk || D <= 0 || D > 128) return UNCR_ESHAPE;
+    if ((long long)Nq * (Hq / Hk) > 0x40000000ll || Nk > 0x40000000) return UNCR_ESHAPE;      // rows and keys are counted in 32 bits
+    if ((act != 0 && act != 1) || !off_q || !off_k || !(temperature > 0.f)) return UNCR_EINVAL;
+    // blocks of a launch: at least 32 rows each
+    if (((((long long)Nq * (Hq / Hk)) >> 5) + B) * Hk > 0x7fffffffll || (((long long)Nk >> 5) + B) * Hk > 0x7fffffffll) return UNCR_ESHAPE;
+    g.off_q = off_q; g.off_k = off_k; g.k_len = k_len;
+    g.B = B; g.Nq = Nq; g.Nk = Nk; g.Hq = Hq; g.Hk = Hk; g.G = Hq / Hk; g.D = D;
+    g.causal = causal ? 1 : 0;
+    g.fill = 0;
+    g.scale = 1.f / temperature;
+    g.c = (float)(1.4426950408889634 / (double)temperature);
+    return UNCR_OK;
+}
+
+bool attn_aligned(const AttnTensor* t, int n, int D, int act) {
+    const int size = act ? 2 : 4;
+    bool ok = (D * size) % 16 == 0;
+    for (int i = 0; i < n; ++i) ok = ok && (uintptr_t)t[i].p % 16 == 0 && (t[i].ts * size) % 16 == 0 && (t[i].hs * size) % 16 == 0;
+    return ok;
+}
+
+extern "C" int uncr_packed_attn_fwd(const void* q, long long q_ts, long long q_hs, const void* k, long long k_ts, long long k_hs, const void* v,
+                                    long long v_ts, long long v_hs, void* out, long long o_ts, long long o_hs, float* lse, const int* off_q,
+                                    const int* off_k, const int* k_len, float temperature, int causal, int fill, int B, int Nq, int Nk, int Hq,
+                                    int Hk, int D, int act, hipStream_t stream) {
+    AttnGeom g;
+    const int rc = attn_geom(g, off_q, off_k, k_len, temperature, causal, B, Nq, Nk, Hq, Hk, D, act);
+    if (rc != UNCR_OK) return rc;
+    if (Nq == 0) return UNCR_OK;
+    if (!q || !out || (Nk && (!k || !v))) return UNCR_EINVAL;
+    g.fill = fill ? 1 : 0;
+    const AttnTensor tq = {q, q_ts, q_hs}, tk = {k, k_ts, k_hs}, tv = {v, v_ts, v_hs};
+    const AttnTensor all[] = {tq, tk, tv};
+    const bool vec = attn_aligned(all, 3, D, act);
+    if ((D & 3) == 0) {         // the epilogue's 4-element stores
+        const int size = (act ? 2 : 4) * 4;
+        if ((uintptr_t)out % size || (o_ts * size / 4) % size || (o_hs * size / 4) % size) return UNCR_EINVAL;
+    }
+    if (act) {
+        if (D <= 32) launch<__bf16, 32, 4, 64>(g, tq, tk, tv, out, o_ts, o_hs, lse, vec, stream);
+        else if (D <= 64) launch<__bf16, 64, 4, 64>(g, tq, tk, tv, out, o_ts, o_hs, lse, vec, stream);
+        else launch<__bf16, 128, 8, 64>(g, tq, tk, tv, out, o_ts, o_hs, lse, vec, stream);
+    } else {
+        if (D <= 32) launch<float, 32, 4, 64>(g, tq, tk, tv, out, o_ts, o_hs, lse, vec, stream);
+        else if (D <= 64) launch<float, 64, 4, 64>(g, tq, tk, tv, out, o_ts, o_hs, lse, vec, stream);
+        else launch<float, 128, 4, 32>(g, tq, tk, tv, out, o_ts, o_hs, lse, vec, stream);
+    }
+    UNCR_LAUNCH_CHECK();
+    return UNCR_OK;
+}

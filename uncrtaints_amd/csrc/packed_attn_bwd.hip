@@ -1,0 +1,303 @@
+// Backward of the attention over packed token sequences (see packed_attn.h for the layout of a product):
+//   P = exp(S - lse),  delta = sum(dOut * Out),  dP = dOut V^T,  dS = P (dP - delta) / temperature
+//   dQ = dS K,   dV = P^T dOut,   dK = dS^T Q,   dK and dV summed over the query heads of a group
+// Two kernels, each recomputing S and dP from the stored lse: one owns rows of queries (dQ, and delta on its way), one owns keys (dK, dV).
+// That is 7 products instead of the 5 of a single kernel that would add its share of dQ to memory from every key tile -- but no atomics: the
+// result does not depend on the order blocks run in, and no fp32 copy of dQ is written, read back and rounded.  The group's heads are
+// consecutive rows of one problem, so dK and dV are sums inside a block as well.
+#include "packed_attn.h"
+
+namespace {
+
+template <typename T, int DP, int NW, int TK, bool VEC>
+__global__ __launch_bounds__(NW * 64) void packed_attn_dq_kernel(const AttnGeom g, const AttnTensor q, const AttnTensor k, const AttnTensor v,
+                                                                 const AttnTensor o, const AttnTensor go, const float* __restrict__ lse,
+                                                                 T* __restrict__ dq, float* __restrict__ delta, int slots) {
+    typedef AttnTile<T, DP> L;
+    constexpr int NT = NW * 64, BM = NW * 32, SHIFT = NW == 8 ? 8 : 7;
+    __shared__ alignas(16) char lds_k[2][TK * L::RB], lds_v[2][TK * L::RB];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5, col = lane & 31;
+    attn_fill_outside<T>(g.off_q, g.B, g.Nq, dq, (long long)g.Hq * g.D, g.D, g.Hq, g.D, nullptr, blockIdx.x, gridDim.x);
+    const int hk = blockIdx.x % g.Hk;
+    int b, tile;
+    if (!attn_find(g.off_q, g.B, g.Nq, g.G, SHIFT, slots - 1 - (int)(blockIdx.x / g.Hk), b, tile)) return;
+    const AttnSeq s = attn_seq(g, b);
+    const int rows = s.lq * g.G;
+    if (tile * BM >= rows) return;
+    const int row0 = tile * BM + wave * 32;
+    const int row = min(row0 + col, rows - 1), tok = row / g.G, head = hk * g.G + row - tok * g.G;
+    const int shift = s.lk - s.lq;
+    auto limit_of = [&](int r) { return g.causal ? min(max(min(r, rows - 1) / g.G + shift + 1, 0), s.lk) : s.lk; };
+    const int limit = limit_of(row);
+    const int wave_lo = limit_of(row0), wave_hi = row0 < rows ? limit_of(row0 + 31) : 0, block_hi = limit_of(tile * BM + BM - 1);
+
+    typename L::Frag qf[L::KS], gf[L::KS];
+    float dl = 0.f;
+    {
+        const T* qr = (const T*)q.p + (size_t)(s.q0 + tok) * q.ts + (size_t)head * q.hs;
+        const T* gr = (const T*)go.p + (size_t)(s.q0 + tok) * go.ts + (size_t)head * go.hs;
+        const T* orow = (const T*)o.p + (size_t)(s.q0 + tok) * o.ts + (size_t)head * o.hs;
+#pragma unroll
+        for (int i = 0; i < L::KS; ++i) {
+            qf[i] = L::template fetch<VEC>(qr, 2 * i + h, g.D);
+            gf[i] = L::template fetch<VEC>(gr, 2 * i + h, g.D);
+            const typename L::Frag of = L::template fetch<VEC>(orow, 2 * i + h, g.D);
+#pragma unroll
+            for (int e = 0; e < L::EPC; ++e) dl = fmaf((float)gf[i][e], (float)of[e], dl);
+        }
+    }
+    dl += attn_other_half(dl);
+    const size_t at = (size_t)(s.q0 + tok) * g.Hq + head;
+    if (h == 0 && row0 + col < rows) delta[at] = dl;
+    // a row that saw nothing has lse = -inf: +inf makes its probabilities 0
+    float ls = lse[at] * 1.4426950408889634f;
+    if (ls == -INFINITY) ls = INFINITY;
+
+    f32x16 acc[L::DB];
+#pragma unroll
+    for (int db = 0; db < L::DB; ++db) acc[db] = (f32x16)(0.f);
+    const T* kb = (const T*)k.p + (size_t)s.k0 * k.ts + (size_t)hk * k.hs;
+    const T* vb = (const T*)v.p + (size_t)s.k0 * v.ts + (size_t)hk * v.hs;
+    const int tiles = (block_hi + TK - 1) / TK;
+    AttnStage<T, DP, TK, NT, VEC> ks, vs;
+    if (tiles) {
+        ks.fetch(kb, k.ts, 0, s.lk - 1, g.D);
+        vs.fetch(vb, v.ts, 0, s.lk - 1, g.D);
+        ks.store(lds_k[0]);
+        vs.store(lds_v[0]);
+    }
+    __syncthreads();
+    for (int it = 0; it < tiles; ++it) {
+        const int j0 = it * TK;
+        if (it + 1 < tiles) {
+            ks.fetch(kb, k.ts, j0 + TK, s.lk - 1, g.D);
+            vs.fetch(vb, v.ts, j0 + TK, s.lk - 1, g.D);
+        }
+        if (j0 < wave_hi) {
+            const char* tk = lds_k[it & 1];
+            const char* tv = lds_v[it & 1];
+            const bool edge = j0 + TK > wave_lo;
+#pragma unroll
+            for (int t = 0; t < TK / 32; ++t) {
+                f32x16 sc = (f32x16)(0.f), dp = (f32x16)(0.f);
+#pragma unroll
+                for (int i = 0; i < L::KS; ++i) {
+                    attn_mma(sc, L::frag(tk, t * 32 + col, i, h), qf[i]);
+                    attn_mma(dp, L::frag(tv, t * 32 + col, i, h), gf[i]);
+                }
+#pragma unroll
+                for (int i = 0; i < 16; ++i) sc[i] = __builtin_amdgcn_exp2f(fmaf(sc[i], g.c, -ls)) * (dp[i] - dl);
+                if (edge) {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        if (j0 + t * 32 + 8 * (i / 4) + 4 * h + i % 4 >= limit) sc[i] = 0.f;
+                }
+                AttnProb<T> p;
+                p.set(sc);
+#pragma unroll
+                for (int db = 0; db < L::DB; ++db) attn_mma_t<DP>(acc[db], tk, t * 32, db, lane, p);
+            }
+        }
+        if (it + 1 < tiles) {
+            ks.store(lds_k[(it + 1) & 1]);
+            vs.store(lds_v[(it + 1) & 1]);
+        }
+        __syncthreads();
+    }
+    if (row0 + col < rows) attn_store_row<T, L::DB>(dq + at * g.D, acc, g.scale, h, g.D);
+}
+
+template <typename T, int DP, int NW, int TQ, bool VEC>
+__global__ __launch_bounds__(NW * 64) void packed_attn_dkv_kernel(const AttnGeom g, const AttnTensor q, const AttnTensor k, const AttnTensor v,
+                                                                  const AttnTensor go, const float* __restrict__ lse,
+                                                                  const float* __restrict__ delta, T* __restrict__ dk, T* __restrict__ dv,
+                                                                  int slots) {
+    typedef AttnTile<T, DP> L;
+    constexpr int NT = NW * 64, BN = NW * 32, SHIFT = NW == 8 ? 8 : 7;
+    __shared__ alignas(16) char lds_q[2][TQ * L::RB], lds_g[2][TQ * L::RB];
+    __shared__ alignas(16) float lds_l[2][TQ], lds_d[2][TQ];
+    __shared__ alignas(16) int lds_lim[2][TQ];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5, col = lane & 31;
+    attn_fill_outside<T>(g.off_k, g.B, g.Nk, dk, (long long)g.Hk * g.D, g.D, g.Hk, g.D, nullptr, blockIdx.x, gridDim.x);
+    attn_fill_outside<T>(g.off_k, g.B, g.Nk, dv, (long long)g.Hk * g.D, g.D, g.Hk, g.D, nullptr, blockIdx.x, gridDim.x);
+    const int hk = blockIdx.x % g.Hk;
+    int b, tile;
+    // the first keys of a causal sequence are seen by the most rows: they start first
+    if (!attn_find(g.off_k, g.B, g.Nk, 1, SHIFT, (int)(blockIdx.x / g.Hk), b, tile)) return;
+    const AttnSeq s = attn_seq(g, b);
+    if (tile * BN >= s.room) return;
+    const int key0 = tile * BN + wave * 32, key = key0 + col;
+    const int rows = s.lq * g.G, shift = s.lk - s.lq;
+    f32x16 ak[L::DB], av[L::DB];
+#pragma unroll
+    for (int db = 0; db < L::DB; ++db) ak[db] = av[db] = (f32x16)(0.f);
+
+    // rows [start, rows) see a key of this block; keys behind lk are room in a cache that nothing sees
+    int start = g.causal ? min(max(tile * BN - shift, 0), s.lq) * g.G : 0;
+    if (tile * BN >= s.lk) start = rows;
+    const int tiles = (rows - start + TQ - 1) / TQ;
+    if (tiles > 0) {
+        typename L::Frag kf[L::KS], vf[L::KS];
+        {
+            const size_t at = (size_t)(s.k0 + min(key, s.lk - 1));
+            const T* kr = (const T*)k.p + at * k.ts + (size_t)hk * k.hs;
+            const T* vr = (const T*)v.p + at * v.ts + (size_t)hk * v.hs;
+#pragma unroll
+            for (int i = 0; i < L::KS; ++i) {
+                kf[i] = L::template fetch<VEC>(kr, 2 * i + h, g.D);
+                vf[i] = L::template fetch<VEC>(vr, 2 * i + h, g.D);
+            }
+        }
+        const T* qb = (const T*)q.p + (size_t)s.q0 * q.ts + (size_t)hk * g.G * q.hs;
+        const T* gb = (const T*)go.p + (size_t)s.q0 * go.ts + (size_t)hk * g.G * go.hs;
+        const float* lb = lse + (size_t)s.q0 * g.Hq + hk * g.G;
+        const float* db_ = delta + (size_t)s.q0 * g.Hq + hk * g.G;
+        AttnStage<T, DP, TQ, NT, VEC> qs, gs;
+        float fl = INFINITY, fd = 0.f;
+        int flim = 0;
+        // a row's lse in powers of two, its delta, and how many keys it sees; rows behind the last and rows that see nothing: lse = +inf
+        auto fetch_row = [&](int r0) {
+            if (threadIdx.x < TQ) {
+                const unsigned r = r0 + threadIdx.x;
+                const unsigned rr = min((int)r, rows - 1), t = rr / (unsigned)g.G;
+                const size_t at = (size_t)t * g.Hq + (rr - t * g.G);
+                fl = lb[at] * 1.4426950408889634f;
+                if (fl == -INFINITY || (int)r >= rows) fl = INFINITY;
+                fd = (int)r >= rows ? 0.f : db_[at];
+                flim = g.causal ? (int)t + shift + 1 : s.lk;
+            }
+        };
+        auto store_row = [&](int buf) {
+            if (threadIdx.x < TQ) {
+                lds_l[buf][threadIdx.x] = fl;
+                lds_d[buf][threadIdx.x] = fd;
+                lds_lim[buf][threadIdx.x] = flim;
+            }
+        };
+        qs.fetch_packed(qb, q.ts, q.hs, start, rows - 1, g.G, g.D);
+        gs.fetch_packed(gb, go.ts, go.hs, start, rows - 1, g.G, g.D);
+        fetch_row(start);
+        qs.store(lds_q[0]);
+        gs.store(lds_g[0]);
+        store_row(0);
+        __syncthreads();
+        for (int it = 0; it < tiles; ++it) {
+            const int r0 = start + it * TQ, cur = it & 1;
+            if (it + 1 < tiles) {
+                qs.fetch_packed(qb, q.ts, q.hs, r0 + TQ, rows - 1, g.G, g.D);
+                gs.fetch_packed(gb, go.ts, go.hs, r0 + TQ, rows - 1, g.G, g.D);
+                fetch_row(r0 + TQ);
+            }
+            // the tile's last row sees keys below `see`: a wave whose keys all lie behind has nothing to do
+            const int see = g.causal ? min(r0 + TQ, rows) - 1 : 0, first = g.causal ? lds_lim[cur][0] : s.lk;
+            if (key0 < s.lk && (!g.causal || key0 < see / g.G + shift + 1)) {
+                const bool edge = g.causal && first < key0 + 32;
+#pragma unroll
+                for (int t = 0; t < TQ / 32; ++t) {
+                    f32x16 sc = (f32x16)(0.f), dp = (f32x16)(0.f);
+#pragma unroll
+                    for (int i = 0; i < L::KS; ++i) {
+                        attn_mma(sc, L::frag(lds_q[cur], t * 32 + col, i, h), kf[i]);
+                        attn_mma(dp, L::frag(lds_g[cur], t * 32 + col, i, h), vf[i]);
+                    }
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const f32x4 ls = *reinterpret_cast<const f32x4*>(&lds_l[cur][t * 32 + 8 * e + 4 * h]);
+                        const f32x4 dl = *reinterpret_cast<const f32x4*>(&lds_d[cur][t * 32 + 8 * e + 4 * h]);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const float p = __builtin_amdgcn_exp2f(fmaf(sc[4 * e + i], g.c, -ls[i]));
+                            sc[4 * e + i] = p;
+                            dp[4 * e + i] = p * (dp[4 * e + i] - dl[i]);
+                        }
+                    }
+                    if (edge) {
+#pragma unroll
+                        for (int i = 0; i < 16; ++i)
+                            if (key >= lds_lim[cur][t * 32 + 8 * (i / 4) + 4 * h + i % 4]) sc[i] = dp[i] = 0.f;
+                    }
+                    AttnProb<T> p, ds;
+                    p.set(sc);
+                    ds.set(dp);
+#pragma unroll
+                    for (int db = 0; db < L::DB; ++db) {
+                        attn_mma_t<DP>(av[db], lds_g[cur], t * 32, db, lane, p);
+                        attn_mma_t<DP>(ak[db], lds_q[cur], t * 32, db, lane, ds);
+                    }
+                }
+            }
+            if (it + 1 < tiles) {
+                qs.store(lds_q[cur ^ 1]);
+                gs.store(lds_g[cur ^ 1]);
+                store_row(cur ^ 1);
+            }
+            __syncthreads();
+        }
+    }
+    if (key >= s.room) return;
+    // a key in the room behind lk: its column repeated the last key's
+    const float live = key < s.lk ? 1.f : 0.f;
+    if (live == 0.f)
+#pragma unroll
+        for (int db = 0; db < L::DB; ++db) ak[db] = av[db] = (f32x16)(0.f);
+    const size_t at = ((size_t)(s.k0 + key) * g.Hk + hk) * g.D;
+    attn_store_row<T, L::DB>(dk + at, ak, g.scale, h, g.D);
+    attn_store_row<T, L::DB>(dv + at, av, 1.f, h, g.D);
+}
+
+struct Bwd {
+    AttnGeom g;
+    AttnTensor q, k, v, o, go;
+    const float* lse;
+    void *dq, *dk, *dv;
+    float* delta;
+    bool vec;
+    hipStream_t stream;
+};
+
+template <typename T, int DP, int NWQ, int TK, int NWK, int TQ, bool VEC> void launch_v(const Bwd& a) {
+    const int sq = attn_slots((long long)a.g.Nq * a.g.G, a.g.B, NWQ == 8 ? 8 : 7), sk = attn_slots(a.g.Nk, a.g.B, NWK == 8 ? 8 : 7);
+    if (a.g.Nq)
+        hipLaunchKernelGGL((packed_attn_dq_kernel<T, DP, NWQ, TK, VEC>), dim3(sq * a.g.Hk), dim3(NWQ * 64), 0, a.stream, a.g, a.q, a.k, a.v, a.o, a.go,
+                           a.lse, (T*)a.dq, a.delta, sq);
+    if (a.g.Nk)
+        hipLaunchKernelGGL((packed_attn_dkv_kernel<T, DP, NWK, TQ, VEC>), dim3(sk * a.g.Hk), dim3(NWK * 64), 0, a.stream, a.g, a.q, a.k, a.v, a.go, a.lse,
+                           a.delta, (T*)a.dk, (T*)a.dv, sk);
+}
+template <typename T, int DP, int NWQ, int TK, int NWK, int TQ> void launch(const Bwd& a) {
+    if (a.vec) launch_v<T, DP, NWQ, TK, NWK, TQ, true>(a);
+    else launch_v<T, DP, NWQ, TK, NWK, TQ, false>(a);
+}
+
+}  // namespace
+
+extern "C" int uncr_packed_attn_bwd(const void* q, long long q_ts, long long q_hs, const void* k, long long k_ts, long long k_hs, const void* v,
+                                    long long v_ts, long long v_hs, const void* out, long long o_ts, long long o_hs, const void* dout,
+                                    long long do_ts, long long do_hs, const float* lse, void* dq, void* dk, void* dv, float* delta,
+                                    const int* off_q, const int* off_k, const int* k_len, float temperature, int causal, int B, int Nq, int Nk,
+                                    int Hq, int Hk, int D, int act, hipStream_t stream) {
+    Bwd a;
+    const int rc = attn_geom(a.g, off_q, off_k, k_len, temperature, causal, B, Nq, Nk, Hq, Hk, D, act);
+    if (rc != UNCR_OK) return rc;
+    if (Nq && (!q || !out || !dout || !lse || !dq || !delta)) return UNCR_EINVAL;
+    if (Nk && (!k || !v || !dk || !dv)) return UNCR_EINVAL;
+    if ((D & 3) == 0) {         // the epilogue's 4-element stores
+        const uintptr_t align = (act ? 2 : 4) * 4;
+        if ((uintptr_t)dq % align || (uintptr_t)dk % align || (uintptr_t)dv % align) return UNCR_EINVAL;
+    }
+    a.q = {q, q_ts, q_hs}; a.k = {k, k_ts, k_hs}; a.v = {v, v_ts, v_hs}; a.o = {out, o_ts, o_hs}; a.go = {dout, do_ts, do_hs};
+    a.lse = lse; a.dq = dq; a.dk = dk; a.dv = dv; a.delta = delta; a.stream = stream;
+    const AttnTensor all[] = {a.q, a.k, a.v, a.o, a.go};
+    a.vec = attn_aligned(all, 5, D, act);
+    if (act) {
+        if (D <= 32) launch<__bf16, 32, 4, 64, 4, 64>(a);
+        else if (D <= 64) launch<__bf16, 64, 4, 64, 4, 64>(a);
+        else launch<__bf16, 128, 8, 64, 4, 64>(a);
+    } else {
+        if (D <= 32) launch<float, 32, 4, 64, 4, 64>(a);
+        else if (D <= 64) launch<float, 64, 4, 64, 4, 64>(a);
+        else launch<float, 128, 4, 32, 4, 32>(a);
+    }
+    UNCR_LAUNCH_CHECK();
+    return UNCR_OK;
+}

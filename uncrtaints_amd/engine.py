@@ -2242,6 +2242,40 @@ def headnorm_rotary_backward(gq: Tensor, gk: Tensor, q: Tensor, k: Tensor, wq: T
     return dq, dk, dwq, dwk
 
 
+def packed_attention_forward(q: Tensor, k: Tensor, v: Tensor, off_q: Tensor, off_k: Tensor, k_len: Optional[Tensor], temperature: float,
+                             causal: bool, want_lse: bool, out: Optional[Tensor] = None):
+    """q [Nq, Hq, D], k / v [Nk, Hk, D] -> out [Nq, Hq, D] (rows of no sequence: zeros, or as they were in a given `out`), lse [Nq, Hq] or None"""
+    q, k, v = _token_rows(q), _token_rows(k), _token_rows(v)
+    Nq, Hq, D = q.shape
+    Nk, Hk, _ = k.shape
+    with _on(q.device):
+        fill = out is None
+        if fill:
+            out = torch.empty((Nq, Hq, D), device=q.device, dtype=q.dtype)
+        lse = _f32((Nq, Hq), q.device) if want_lse else None
+        hb.call("uncr_packed_attn_fwd", q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(),
+                v.stride(0), v.stride(1), out.data_ptr(), out.stride(0), out.stride(1), lse, off_q, off_k, k_len, float(temperature),
+                int(causal), int(fill), off_q.numel() - 1, Nq, Nk, Hq, Hk, D, _dt(q), _stream())
+    return out, lse
+
+
+def packed_attention_backward(dout: Tensor, q: Tensor, k: Tensor, v: Tensor, out: Tensor, lse: Tensor, off_q: Tensor, off_k: Tensor,
+                              k_len: Optional[Tensor], temperature: float, causal: bool):
+    """-> dq [Nq, Hq, D], dk, dv [Nk, Hk, D] in the storage type"""
+    q, k, v, dout = _token_rows(q), _token_rows(k), _token_rows(v), _token_rows(dout)
+    Nq, Hq, D = q.shape
+    Nk, Hk, _ = k.shape
+    with _on(q.device):
+        dq = torch.empty((Nq, Hq, D), device=q.device, dtype=q.dtype)
+        dk, dv = torch.empty((Nk, Hk, D), device=q.device, dtype=q.dtype), torch.empty((Nk, Hk, D), device=q.device, dtype=q.dtype)
+        delta = _f32((Nq, Hq), q.device)
+        hb.call("uncr_packed_attn_bwd", q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(),
+                v.stride(0), v.stride(1), out.data_ptr(), out.stride(0), out.stride(1), dout.data_ptr(), dout.stride(0), dout.stride(1),
+                lse, dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), delta, off_q, off_k, k_len, float(temperature), int(causal),
+                off_q.numel() - 1, Nq, Nk, Hq, Hk, D, _dt(q), _stream())
+    return dq, dk, dv
+
+
 # ------------------------------------------------------------------------------------------------
 # out_conv + output nonlinearities (uncrtaints.py:381,432-445)
 # ------------------------------------------------------------------------------------------------

@@ -4,6 +4,8 @@ are one learned vector per head and whose keys are the dates of one pixel.
     qkv projection [tokens, heads, d] -> HeadNormRotary (queries and keys) -> PackedAttention
 
 Tokens of all series lie behind one another, without padding: series b owns the rows offsets[b] .. offsets[b + 1] - 1."""
+import math
+
 import torch
 import torch.nn as nn
 
@@ -61,3 +63,95 @@ class HeadNormRotary(nn.Module):
         qo, ko = _HeadNormRotaryFn.apply(q.reshape(-1, *q.shape[-2:]), k.reshape(-1, *k.shape[-2:]), self.q_weight, self.k_weight,
                                          self.eps, plan)
         return qo.view(q.shape), ko.view(k.shape)
+
+
+class _PackedAttentionFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, off_q, off_k, k_len, temperature, causal):
+        out, lse = E.packed_attention_forward(q, k, v, off_q, off_k, k_len, temperature, causal, True)
+        ctx.save_for_backward(q, k, v, out, lse, off_q, off_k, k_len)
+        ctx.temperature, ctx.causal = temperature, causal
+        ctx.mark_non_differentiable(lse)
+        return out, lse
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dout, _):
+        q, k, v, out, lse, off_q, off_k, k_len = ctx.saved_tensors
+        grads = E.packed_attention_backward(dout, q, k, v, out, lse, off_q, off_k, k_len, ctx.temperature, ctx.causal)
+        return (*grads, None, None, None, None, None)
+
+
+def pack_offsets(lengths, device):
+    """[B] sequence lengths (Python numbers) -> [B + 1] int32 row offsets on the device"""
+    offsets = [0]
+    for n in lengths:
+        if n < 0:
+            raise ValueError(f"length {n}: must not be negative")
+        offsets.append(offsets[-1] + int(n))
+    return torch.tensor(offsets, dtype=torch.int32, device=device)
+
+
+class PackedAttention(nn.Module):
+    """softmax(q k^T / temperature) v within each sequence of a packed batch, heads in groups.
+
+    causal: row i of a sequence's Lq queries sees its keys j <= i + Lk - Lq (the last query sees every key), otherwise all Lk.
+    temperature: default sqrt(d), as in the L-TAE classes.
+
+    forward(q [Nq, heads, d], k [Nk, kv_heads, d], v [Nk, kv_heads, d], offsets_q, offsets_k=None, k_len=None, ...) -> out [Nq, heads, d]
+      heads is a multiple of kv_heads: query head i reads key head i // (heads // kv_heads).  d is at most 128.  fp32 or bf16; the softmax and
+      all sums are fp32 either way.  Inputs may be strided (slices of one projection, a cache of any layout with d contiguous).
+      offsets_q, offsets_k [B + 1]: int32 on the device, not decreasing; sequence b owns rows offsets[b] .. offsets[b + 1] - 1 (`pack_offsets`).
+      Without offsets_k the keys lie like the queries.  They are not read on the host; offsets outside the tensors are clamped on the device.
+      k_len [B]: int32, used rows of each key sequence; the rest is room in a cache, never read into a result.
+      A row that sees no key is 0 and takes no part in any gradient.  Rows of no sequence are zeros, in the gradients too.
+      out: written in place of a new tensor (only without gradients); rows of no sequence stay as they were.
+      return_lse: also the logarithm of each row's sum of exponentials [Nq, heads], fp32, without a gradient; -inf where a row sees nothing.
+
+    Serving: one query row per sequence (offsets_q = 0, 1, 2, ...) against a cache [B * room, kv_heads, d] with offsets_k = b * room and k_len."""
+
+    def __init__(self, causal=False, temperature=None):
+        super().__init__()
+        if temperature is not None and not (temperature > 0.0 and math.isfinite(temperature)):
+            raise ValueError(f"temperature {temperature}: must be positive")
+        self.causal, self.temperature = bool(causal), temperature
+
+    def forward(self, q, k, v, offsets_q, offsets_k=None, k_len=None, max_q=None, max_k=None, out=None, return_lse=False):
+        if q.dim() != 3 or k.dim() != 3 or v.dim() != 3:
+            raise ValueError(f"expected tokens [N, heads, d], got {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
+        if k.shape != v.shape or q.shape[2] != k.shape[2]:
+            raise ValueError(f"q {tuple(q.shape)}, k {tuple(k.shape)} and v {tuple(v.shape)} do not belong together")
+        d, heads, kv_heads = q.shape[2], q.shape[1], k.shape[1]
+        if d == 0 or d > 128:
+            raise ValueError(f"head size {d}: 1 to 128 are built")
+        if kv_heads == 0 or heads == 0 or heads % kv_heads:
+            raise ValueError(f"{heads} query heads are not a multiple of {kv_heads} key heads")
+        if offsets_k is None:
+            if q.shape[0] != k.shape[0]:
+                raise ValueError(f"{q.shape[0]} query rows and {k.shape[0]} key rows need offsets_k")
+            offsets_k = offsets_q
+        for name, t in (("offsets_q", offsets_q), ("offsets_k", offsets_k), ("k_len", k_len)):
+            if t is None:
+                continue
+            if t.dtype != torch.int32 or t.dim() != 1 or not t.is_contiguous():
+                raise ValueError(f"{name}: a contiguous int32 vector is required, got {t.dtype} {tuple(t.shape)}")
+        n = offsets_q.numel() - 1
+        if n < 1 or offsets_k.numel() != n + 1 or (k_len is not None and k_len.numel() != n):
+            raise ValueError("offsets_q and offsets_k need B + 1 entries, k_len B, with at least one sequence")
+        for name, m in (("max_q", max_q), ("max_k", max_k)):
+            if m is not None and m < 0:
+                raise ValueError(f"{name} {m}: must not be negative")
+        E.check_tokens(q=q, k=k, v=v)
+        E.check_device(q=q, offsets_q=offsets_q, offsets_k=offsets_k, k_len=k_len)
+        temperature = math.sqrt(d) if self.temperature is None else float(self.temperature)
+        if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+            if out is not None:
+                raise ValueError("out is for calls without gradients")
+            res, lse = _PackedAttentionFn.apply(q, k, v, offsets_q, offsets_k, k_len, temperature, self.causal)
+        else:
+            if out is not None:
+                E.check_tokens(q=q, out=out)
+                if out.shape != q.shape or not out.is_contiguous():
+                    raise ValueError(f"out {tuple(out.shape)}: a contiguous tensor of q's shape {tuple(q.shape)} is required")
+            res, lse = E.packed_attention_forward(q, k, v, offsets_q, offsets_k, k_len, temperature, self.causal, return_lse, out)
+        return (res, lse) if return_lse else res
