@@ -107,17 +107,24 @@ __global__ __launch_bounds__(NW * 64) void packed_attn_dq_kernel(const AttnGeom 
     if (row0 + col < rows) attn_store_row<T, L::DB>(dq + at * g.D, acc, g.scale, h, g.D);
 }
 
-template <typename T, int DP, int NW, int TQ, bool VEC>
-__global__ __launch_bounds__(NW * 64) void packed_attn_dkv_kernel(const AttnGeom g, const AttnTensor q, const AttnTensor k, const AttnTensor v,
-                                                                  const AttnTensor go, const float* __restrict__ lse,
-                                                                  const float* __restrict__ delta, T* __restrict__ dk, T* __restrict__ dv,
-                                                                  int slots) {
+// A block owns 128 keys, 32 for each of four pairs of waves.  The first wave of a pair holds its keys' K and the sum dV, the second V and dK:
+//   first:  S = Q K^T, P = exp2(S c - lse), P to LDS, dV^T += dOut^T P          second, one tile behind:  dP = dOut V^T, dS, dK^T += Q^T dS
+// Both make half of the products and hold half of the accumulators (one wave with both needs 470 registers and leaves one wave per SIMD with
+// nothing to run beside it); the exponentials of one wave run beside the products of the other.  P crosses in the accumulator layout, lane
+// by lane, in fp32.  Q and dOut tiles rotate through three buffers: the one being filled and those of the two roles.
+template <typename T, int DP, bool VEC>
+__global__ __launch_bounds__(512) void packed_attn_dkv_kernel(const AttnGeom g, const AttnTensor q, const AttnTensor k, const AttnTensor v,
+                                                              const AttnTensor go, const float* __restrict__ lse,
+                                                              const float* __restrict__ delta, T* __restrict__ dk, T* __restrict__ dv,
+                                                              int slots) {
     typedef AttnTile<T, DP> L;
-    constexpr int NT = NW * 64, BN = NW * 32, SHIFT = NW == 8 ? 8 : 7;
-    __shared__ alignas(16) char lds_q[2][TQ * L::RB], lds_g[2][TQ * L::RB];
-    __shared__ alignas(16) float lds_l[2][TQ], lds_d[2][TQ];
-    __shared__ alignas(16) int lds_lim[2][TQ];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5, col = lane & 31;
+    constexpr int NT = 512, BN = 128, SHIFT = 7, TQ = 32;
+    __shared__ alignas(16) char lds_q[3][TQ * L::RB], lds_g[3][TQ * L::RB];
+    __shared__ f32x4 lds_p[2][4][4][64];
+    __shared__ alignas(16) float lds_l[3][TQ], lds_d[3][TQ];
+    __shared__ alignas(16) int lds_lim[3][TQ];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5, col = lane & 31, pair = wave & 3;
+    const bool second = wave >= 4;
     attn_fill_outside<T>(g.off_k, g.B, g.Nk, dk, (long long)g.Hk * g.D, g.D, g.Hk, g.D, nullptr, blockIdx.x, gridDim.x);
     attn_fill_outside<T>(g.off_k, g.B, g.Nk, dv, (long long)g.Hk * g.D, g.D, g.Hk, g.D, nullptr, blockIdx.x, gridDim.x);
     const int hk = blockIdx.x % g.Hk;
@@ -126,27 +133,23 @@ __global__ __launch_bounds__(NW * 64) void packed_attn_dkv_kernel(const AttnGeom
     if (!attn_find(g.off_k, g.B, g.Nk, 1, SHIFT, (int)(blockIdx.x / g.Hk), b, tile)) return;
     const AttnSeq s = attn_seq(g, b);
     if (tile * BN >= s.room) return;
-    const int key0 = tile * BN + wave * 32, key = key0 + col;
+    const int key0 = tile * BN + pair * 32, key = key0 + col;
     const int rows = s.lq * g.G, shift = s.lk - s.lq;
-    f32x16 ak[L::DB], av[L::DB];
+    f32x16 acc[L::DB];
 #pragma unroll
-    for (int db = 0; db < L::DB; ++db) ak[db] = av[db] = (f32x16)(0.f);
+    for (int db = 0; db < L::DB; ++db) acc[db] = (f32x16)(0.f);
 
     // rows [start, rows) see a key of this block; keys behind lk are room in a cache that nothing sees
     int start = g.causal ? min(max(tile * BN - shift, 0), s.lq) * g.G : 0;
     if (tile * BN >= s.lk) start = rows;
     const int tiles = (rows - start + TQ - 1) / TQ;
     if (tiles > 0) {
-        typename L::Frag kf[L::KS], vf[L::KS];
+        typename L::Frag own[L::KS];
         {
-            const size_t at = (size_t)(s.k0 + min(key, s.lk - 1));
-            const T* kr = (const T*)k.p + at * k.ts + (size_t)hk * k.hs;
-            const T* vr = (const T*)v.p + at * v.ts + (size_t)hk * v.hs;
+            const AttnTensor& x = second ? v : k;
+            const T* r = (const T*)x.p + (size_t)(s.k0 + min(key, s.lk - 1)) * x.ts + (size_t)hk * x.hs;
 #pragma unroll
-            for (int i = 0; i < L::KS; ++i) {
-                kf[i] = L::template fetch<VEC>(kr, 2 * i + h, g.D);
-                vf[i] = L::template fetch<VEC>(vr, 2 * i + h, g.D);
-            }
+            for (int i = 0; i < L::KS; ++i) own[i] = L::template fetch<VEC>(r, 2 * i + h, g.D);
         }
         const T* qb = (const T*)q.p + (size_t)s.q0 * q.ts + (size_t)hk * g.G * q.hs;
         const T* gb = (const T*)go.p + (size_t)s.q0 * go.ts + (size_t)hk * g.G * go.hs;
@@ -167,82 +170,84 @@ __global__ __launch_bounds__(NW * 64) void packed_attn_dkv_kernel(const AttnGeom
                 flim = g.causal ? (int)t + shift + 1 : s.lk;
             }
         };
-        auto store_row = [&](int buf) {
+        auto store = [&](int buf) {
+            qs.store(lds_q[buf]);
+            gs.store(lds_g[buf]);
             if (threadIdx.x < TQ) {
                 lds_l[buf][threadIdx.x] = fl;
                 lds_d[buf][threadIdx.x] = fd;
                 lds_lim[buf][threadIdx.x] = flim;
             }
         };
-        qs.fetch_packed(qb, q.ts, q.hs, start, rows - 1, g.G, g.D);
-        gs.fetch_packed(gb, go.ts, go.hs, start, rows - 1, g.G, g.D);
-        fetch_row(start);
-        qs.store(lds_q[0]);
-        gs.store(lds_g[0]);
-        store_row(0);
+        auto fetch = [&](int r0) {
+            qs.fetch_packed(qb, q.ts, q.hs, r0, rows - 1, g.G, g.D);
+            gs.fetch_packed(gb, go.ts, go.hs, r0, rows - 1, g.G, g.D);
+            fetch_row(r0);
+        };
+        // the tile's last row sees keys below its limit: a pair whose keys all lie behind has nothing to do with the tile
+        auto seen = [&](int it) {
+            const int last = min(start + it * TQ + TQ, rows) - 1;
+            return key0 < s.lk && (!g.causal || key0 < last / g.G + shift + 1);
+        };
+        fetch(start);
+        store(0);
         __syncthreads();
-        for (int it = 0; it < tiles; ++it) {
-            const int r0 = start + it * TQ, cur = it & 1;
-            if (it + 1 < tiles) {
-                qs.fetch_packed(qb, q.ts, q.hs, r0 + TQ, rows - 1, g.G, g.D);
-                gs.fetch_packed(gb, go.ts, go.hs, r0 + TQ, rows - 1, g.G, g.D);
-                fetch_row(r0 + TQ);
-            }
-            // the tile's last row sees keys below `see`: a wave whose keys all lie behind has nothing to do
-            const int see = g.causal ? min(r0 + TQ, rows) - 1 : 0, first = g.causal ? lds_lim[cur][0] : s.lk;
-            if (key0 < s.lk && (!g.causal || key0 < see / g.G + shift + 1)) {
-                const bool edge = g.causal && first < key0 + 32;
+        int cur = 0, prev = 2, next = 1;
+        for (int it = 0; it <= tiles; ++it) {
+            if (it + 1 < tiles) fetch(start + (it + 1) * TQ);
+            if (!second) {
+                if (it < tiles && seen(it)) {
+                    f32x16 sc = (f32x16)(0.f);
 #pragma unroll
-                for (int t = 0; t < TQ / 32; ++t) {
-                    f32x16 sc = (f32x16)(0.f), dp = (f32x16)(0.f);
-#pragma unroll
-                    for (int i = 0; i < L::KS; ++i) {
-                        attn_mma(sc, L::frag(lds_q[cur], t * 32 + col, i, h), kf[i]);
-                        attn_mma(dp, L::frag(lds_g[cur], t * 32 + col, i, h), vf[i]);
-                    }
+                    for (int i = 0; i < L::KS; ++i) attn_mma(sc, L::frag(lds_q[cur], col, i, h), own[i]);
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        const f32x4 ls = *reinterpret_cast<const f32x4*>(&lds_l[cur][t * 32 + 8 * e + 4 * h]);
-                        const f32x4 dl = *reinterpret_cast<const f32x4*>(&lds_d[cur][t * 32 + 8 * e + 4 * h]);
+                        const f32x4 ls = *reinterpret_cast<const f32x4*>(&lds_l[cur][8 * e + 4 * h]);
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const float p = __builtin_amdgcn_exp2f(fmaf(sc[4 * e + i], g.c, -ls[i]));
-                            sc[4 * e + i] = p;
-                            dp[4 * e + i] = p * (dp[4 * e + i] - dl[i]);
-                        }
+                        for (int i = 0; i < 4; ++i) sc[4 * e + i] = __builtin_amdgcn_exp2f(fmaf(sc[4 * e + i], g.c, -ls[i]));
                     }
-                    if (edge) {
+                    if (g.causal && lds_lim[cur][0] < key0 + 32) {
 #pragma unroll
                         for (int i = 0; i < 16; ++i)
-                            if (key >= lds_lim[cur][t * 32 + 8 * (i / 4) + 4 * h + i % 4]) sc[i] = dp[i] = 0.f;
+                            if (key >= lds_lim[cur][8 * (i / 4) + 4 * h + i % 4]) sc[i] = 0.f;
                     }
-                    AttnProb<T> p, ds;
-                    p.set(sc);
-                    ds.set(dp);
 #pragma unroll
-                    for (int db = 0; db < L::DB; ++db) {
-                        attn_mma_t<DP>(av[db], lds_g[cur], t * 32, db, lane, p);
-                        attn_mma_t<DP>(ak[db], lds_q[cur], t * 32, db, lane, ds);
-                    }
+                    for (int e = 0; e < 4; ++e) lds_p[it & 1][pair][e][lane] = (f32x4){sc[4 * e], sc[4 * e + 1], sc[4 * e + 2], sc[4 * e + 3]};
+                    AttnProb<T> p;
+                    p.set(sc);
+#pragma unroll
+                    for (int db = 0; db < L::DB; ++db) attn_mma_t<DP>(acc[db], lds_g[cur], 0, db, lane, p);
                 }
+            } else if (it > 0 && seen(it - 1)) {
+                f32x16 dp = (f32x16)(0.f);
+#pragma unroll
+                for (int i = 0; i < L::KS; ++i) attn_mma(dp, L::frag(lds_g[prev], col, i, h), own[i]);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const f32x4 dl = *reinterpret_cast<const f32x4*>(&lds_d[prev][8 * e + 4 * h]);
+                    const f32x4 p = lds_p[(it - 1) & 1][pair][e][lane];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) dp[4 * e + i] = p[i] * (dp[4 * e + i] - dl[i]);
+                }
+                AttnProb<T> ds;
+                ds.set(dp);
+#pragma unroll
+                for (int db = 0; db < L::DB; ++db) attn_mma_t<DP>(acc[db], lds_q[prev], 0, db, lane, ds);
             }
-            if (it + 1 < tiles) {
-                qs.store(lds_q[cur ^ 1]);
-                gs.store(lds_g[cur ^ 1]);
-                store_row(cur ^ 1);
-            }
+            if (it + 1 < tiles) store(next);
             __syncthreads();
+            const int t = prev;
+            prev = cur;
+            cur = next;
+            next = t;
         }
     }
     if (key >= s.room) return;
     // a key in the room behind lk: its column repeated the last key's
-    const float live = key < s.lk ? 1.f : 0.f;
-    if (live == 0.f)
+    if (key >= s.lk)
 #pragma unroll
-        for (int db = 0; db < L::DB; ++db) ak[db] = av[db] = (f32x16)(0.f);
-    const size_t at = ((size_t)(s.k0 + key) * g.Hk + hk) * g.D;
-    attn_store_row<T, L::DB>(dk + at, ak, g.scale, h, g.D);
-    attn_store_row<T, L::DB>(dv + at, av, 1.f, h, g.D);
+        for (int db = 0; db < L::DB; ++db) acc[db] = (f32x16)(0.f);
+    attn_store_row<T, L::DB>((second ? dk : dv) + ((size_t)(s.k0 + key) * g.Hk + hk) * g.D, acc, second ? g.scale : 1.f, h, g.D);
 }
 
 struct Bwd {
@@ -255,18 +260,18 @@ struct Bwd {
     hipStream_t stream;
 };
 
-template <typename T, int DP, int NWQ, int TK, int NWK, int TQ, bool VEC> void launch_v(const Bwd& a) {
-    const int sq = attn_slots((long long)a.g.Nq * a.g.G, a.g.B, NWQ == 8 ? 8 : 7), sk = attn_slots(a.g.Nk, a.g.B, NWK == 8 ? 8 : 7);
+template <typename T, int DP, int NW, int TK, bool VEC> void launch_v(const Bwd& a) {
+    const int sq = attn_slots((long long)a.g.Nq * a.g.G, a.g.B, NW == 8 ? 8 : 7), sk = attn_slots(a.g.Nk, a.g.B, 7);
     if (a.g.Nq)
-        hipLaunchKernelGGL((packed_attn_dq_kernel<T, DP, NWQ, TK, VEC>), dim3(sq * a.g.Hk), dim3(NWQ * 64), 0, a.stream, a.g, a.q, a.k, a.v, a.o, a.go,
+        hipLaunchKernelGGL((packed_attn_dq_kernel<T, DP, NW, TK, VEC>), dim3(sq * a.g.Hk), dim3(NW * 64), 0, a.stream, a.g, a.q, a.k, a.v, a.o, a.go,
                            a.lse, (T*)a.dq, a.delta, sq);
     if (a.g.Nk)
-        hipLaunchKernelGGL((packed_attn_dkv_kernel<T, DP, NWK, TQ, VEC>), dim3(sk * a.g.Hk), dim3(NWK * 64), 0, a.stream, a.g, a.q, a.k, a.v, a.go, a.lse,
+        hipLaunchKernelGGL((packed_attn_dkv_kernel<T, DP, VEC>), dim3(sk * a.g.Hk), dim3(512), 0, a.stream, a.g, a.q, a.k, a.v, a.go, a.lse,
                            a.delta, (T*)a.dk, (T*)a.dv, sk);
 }
-template <typename T, int DP, int NWQ, int TK, int NWK, int TQ> void launch(const Bwd& a) {
-    if (a.vec) launch_v<T, DP, NWQ, TK, NWK, TQ, true>(a);
-    else launch_v<T, DP, NWQ, TK, NWK, TQ, false>(a);
+template <typename T, int DP, int NW, int TK> void launch(const Bwd& a) {
+    if (a.vec) launch_v<T, DP, NW, TK, true>(a);
+    else launch_v<T, DP, NW, TK, false>(a);
 }
 
 }  // namespace
@@ -290,13 +295,13 @@ extern "C" int uncr_packed_attn_bwd(const void* q, long long q_ts, long long q_h
     const AttnTensor all[] = {a.q, a.k, a.v, a.o, a.go};
     a.vec = attn_aligned(all, 5, D, act);
     if (act) {
-        if (D <= 32) launch<__bf16, 32, 4, 64, 4, 64>(a);
-        else if (D <= 64) launch<__bf16, 64, 4, 64, 4, 64>(a);
-        else launch<__bf16, 128, 8, 64, 4, 64>(a);
+        if (D <= 32) launch<__bf16, 32, 4, 64>(a);
+        else if (D <= 64) launch<__bf16, 64, 4, 64>(a);
+        else launch<__bf16, 128, 8, 64>(a);
     } else {
-        if (D <= 32) launch<float, 32, 4, 64, 4, 64>(a);
-        else if (D <= 64) launch<float, 64, 4, 64, 4, 64>(a);
-        else launch<float, 128, 4, 32, 4, 32>(a);
+        if (D <= 32) launch<float, 32, 4, 64>(a);
+        else if (D <= 64) launch<float, 64, 4, 64>(a);
+        else launch<float, 128, 4, 32>(a);
     }
     UNCR_LAUNCH_CHECK();
     return UNCR_OK;
