@@ -209,6 +209,15 @@ def test_longer_sequences(d, dtype, causal):
 
 @gpu
 @BOTH
+@pytest.mark.parametrize("hq,hk", [(2, 2), (4, 1), (6, 2)])
+def test_long_causal_sequences_of_very_different_lengths(hq, hk, dtype):
+    """Tiles in descending order of work: every tile of every sequence once, whatever the lengths."""
+    _run([700, 0, 1, 1300, 257, 512], [700, 0, 1, 1300, 257, 512], hq, hk, 32, True, dtype)
+    _run([1400, 30, 900, 0], [600, 1100, 900, 300], hq, hk, 32, True, dtype, room=[640, 1500, 900, 640], front=5, behind=60)
+
+
+@gpu
+@BOTH
 def test_large_scores_and_a_temperature(dtype):
     """Scores of +-several hundred: the running maximum is passed by many powers of two from tile to tile."""
     _run([300], [300], 2, 2, 64, True, dtype, scale=40.0, temperature=2.0)

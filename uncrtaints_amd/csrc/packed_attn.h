@@ -14,6 +14,8 @@
 // LDS tiles are [rows][DP] in 16-byte chunks, chunk c of a row at place c ^ swizzle(row): 16 consecutive rows at one chunk (operand A) and
 // 4 rows x 64 bytes (transposed operand X) then touch all 64 banks once.
 #pragma once
+#include <limits.h>
+
 #include "common.h"
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
@@ -28,7 +30,7 @@ struct AttnGeom {
     const int* off_k;       // [B + 1]
     const int* k_len;       // [B] used rows of each key sequence, or null
     int B, Nq, Nk, Hq, Hk, G, D;
-    int causal, fill;
+    int causal, fill, sorted;
     float c;                // log2(e) / temperature
     float scale;            // 1 / temperature
 };
@@ -67,6 +69,58 @@ __device__ __forceinline__ bool attn_find(const int* off, int B, int N, int per,
     b = lo;
     tile = slot - attn_slot(off, lo, N, per, shift);
     return tile >= 0;
+}
+// The same tiles in descending order of their causal work, for a few long sequences: with tiles in the order of the sequences a long one
+// that comes late keeps some blocks busy long after the others have ended (five sequences of 2832 to 5000 tokens, 16/4 heads of 128, dK/dV:
+// 1210 -> 950 us).  Tile j, counted from its sequence's heaviest, has v = lk * G - rows * j (rows of the group it meets, up
+// to a constant); the block numbered n looks for the largest v that at least n + 1 tiles reach -- 64 candidates at a time, one per lane --
+// and among the tiles that have it takes them in the order of the sequences.
+constexpr int ATTN_SORT_MAX_B = 64;
+template <bool KEYS> __device__ __forceinline__ bool attn_find_sorted(const AttnGeom& g, int rows, int n, int& b, int& tile) {
+    __shared__ int top[ATTN_SORT_MAX_B], tiles[ATTN_SORT_MAX_B];
+    const int lane = threadIdx.x & 63;
+    if (threadIdx.x < (unsigned)g.B) {
+        const AttnSeq s = attn_seq(g, threadIdx.x);
+        top[threadIdx.x] = s.lk * g.G;
+        tiles[threadIdx.x] = ((KEYS ? s.room : s.lq * g.G) + rows - 1) / rows;
+    }
+    __syncthreads();
+    const int unit = KEYS ? rows * g.G : rows;
+    int lo = INT_MAX, hi = INT_MIN, total = 0;
+    for (int i = 0; i < g.B; ++i) {
+        if (!tiles[i]) continue;
+        total += tiles[i];
+        hi = max(hi, top[i]);
+        lo = min(lo, top[i] - unit * (tiles[i] - 1));
+    }
+    if (n >= total) return false;
+    // tiles with v >= x
+    auto reach = [&](int x) {
+        int c = 0;
+        for (int i = 0; i < g.B; ++i)
+            if (top[i] >= x) c += min(tiles[i], (top[i] - x) / unit + 1);
+        return c;
+    };
+    // reach(lo) = total > n: the largest x in [lo, hi] with reach(x) > n
+    while (lo < hi) {
+        const int step = (int)(((unsigned)hi - (unsigned)lo) / 64u) + 1;
+        const long long x = (long long)lo + (long long)step * lane;
+        const int cnt = __popcll(__ballot(x <= hi && reach((int)x) > n));      // lane 0 always
+        lo += step * (cnt - 1);
+        hi = (int)min((long long)hi, (long long)lo + step - 1);
+    }
+    n -= reach(lo + 1);
+    for (b = 0; b < g.B; ++b) {
+        const int d = top[b] - lo;
+        if (d >= 0 && d % unit == 0 && d / unit < tiles[b] && n-- == 0) break;
+    }
+    if (b >= g.B) return false;
+    tile = KEYS ? (top[b] - lo) / unit : tiles[b] - 1 - (top[b] - lo) / unit;
+    return true;
+}
+// Sorting costs a block about 2 us: for causal sequences of at least four tiles on average
+static inline bool attn_sorts(const AttnGeom& g, long long rows, int per_tile) {
+    return g.causal && g.B <= ATTN_SORT_MAX_B && rows / per_tile >= 4ll * g.B && (long long)g.Nk * g.G < (1ll << 29) && (long long)g.G * per_tile < (1 << 20);
 }
 static inline int attn_slots(long long rows, int B, int shift) { return (int)(rows >> shift) + B; }
 
@@ -108,13 +162,38 @@ template <typename T, int DP> struct AttnTile {
     }
 };
 
-// acc (32 x 32) += A * B over one step
+// Operands are fetched from LDS in one go and used after it (`attn_fence` keeps the compiler from sinking each read to its use, where
+// every product waits for the latency of its own operand)
+__device__ __forceinline__ void attn_fence() { __builtin_amdgcn_sched_barrier(0); }
+
+// operand A of a 32-row product: all of a row's chunks this lane half holds
+template <typename T, int DP> struct AttnRows {
+    typedef AttnTile<T, DP> L;
+    typename L::Frag f[L::KS];
+    __device__ __forceinline__ void fetch(const char* tile, int row, int h) {
+#pragma unroll
+        for (int i = 0; i < L::KS; ++i) f[i] = L::frag(tile, row, i, h);
+    }
+    // 16 bytes at a time from a row in global memory
+    template <bool VEC> __device__ __forceinline__ void fetch_global(const T* row, int h, int D) {
+#pragma unroll
+        for (int i = 0; i < L::KS; ++i) f[i] = L::template fetch<VEC>(row, 2 * i + h, D);
+    }
+};
+
 __device__ __forceinline__ void attn_mma(f32x16& acc, const bf16x8& a, const bf16x8& b) {
     acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, acc, 0, 0, 0);
 }
 __device__ __forceinline__ void attn_mma(f32x16& acc, const f32x4& a, const f32x4& b) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) acc = __builtin_amdgcn_mfma_f32_32x32x2f32(a[i], b[i], acc, 0, 0, 0);
+}
+// acc (32 rows of A x 32 columns of B) = A * B
+template <typename T, int DP> __device__ __forceinline__ f32x16 attn_product(const AttnRows<T, DP>& a, const AttnRows<T, DP>& b) {
+    f32x16 acc = (f32x16)(0.f);
+#pragma unroll
+    for (int i = 0; i < AttnTile<T, DP>::KS; ++i) attn_mma(acc, a.f[i], b.f[i]);
+    return acc;
 }
 
 // The C registers of a 32-row product as the B operand of the next one (bf16: rounded once, to nearest even)
@@ -136,32 +215,42 @@ template <> struct AttnProb<float> {
     __device__ __forceinline__ void set(const f32x16& p) { v = p; }
 };
 
-// acc[32 of DP][32 columns] += X^T * P over the 32 rows row0 .. row0 + 31 of the tile X
-template <int DP> __device__ __forceinline__ void attn_mma_t(f32x16& acc, const char* tile, int row0, int db, int lane, const AttnProb<__bf16>& p) {
+// X^T (32 of DP x 32 rows) from the rows row0 .. row0 + 31 of a tile, in the row order of AttnProb, and acc += X^T * P
+template <typename T, int DP> struct AttnCols;
+template <int DP> struct AttnCols<__bf16, DP> {
     typedef AttnTile<__bf16, DP> L;
-    const int g = lane >> 4, l = lane & 15;
-    const int chunk = db * 4 + (g & 1) * 2 + ((l & 3) >> 1), low = (l & 1) * 8;
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-        const int row = row0 + 16 * u + 4 * (g >> 1) + (l >> 2);
+    bf16x8 f[2];
+    __device__ __forceinline__ void fetch(const char* tile, int row0, int db, int lane) {
         typedef __attribute__((address_space(3))) s16x4 lds4;
-        const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(tile + L::place(row, chunk) + low));
-        const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(tile + L::place(row + 8, chunk) + low));
-        const bf16x4 x = __builtin_bit_cast(bf16x4, a), y = __builtin_bit_cast(bf16x4, b);
-        const bf16x8 f = __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
-        acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f, p.v[u], acc, 0, 0, 0);
-    }
-}
-template <int DP> __device__ __forceinline__ void attn_mma_t(f32x16& acc, const char* tile, int row0, int db, int lane, const AttnProb<float>& p) {
-    typedef AttnTile<float, DP> L;
-    const int col = lane & 31, h = lane >> 5;
+        const int g = lane >> 4, l = lane & 15;
+        const int chunk = db * 4 + (g & 1) * 2 + ((l & 3) >> 1), low = (l & 1) * 8;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-        const int row = row0 + 8 * (i / 4) + 4 * h + i % 4;
-        const float x = *reinterpret_cast<const float*>(tile + L::place(row, db * 8 + (col >> 2)) + (col & 3) * 4);
-        acc = __builtin_amdgcn_mfma_f32_32x32x2f32(x, p.v[i], acc, 0, 0, 0);
+        for (int u = 0; u < 2; ++u) {
+            const int row = row0 + 16 * u + 4 * (g >> 1) + (l >> 2);
+            const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(tile + L::place(row, chunk) + low));
+            const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(tile + L::place(row + 8, chunk) + low));
+            f[u] = __builtin_shufflevector(__builtin_bit_cast(bf16x4, a), __builtin_bit_cast(bf16x4, b), 0, 1, 2, 3, 4, 5, 6, 7);
+        }
     }
-}
+    __device__ __forceinline__ void mma(f32x16& acc, const AttnProb<__bf16>& p) const {
+#pragma unroll
+        for (int u = 0; u < 2; ++u) acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f[u], p.v[u], acc, 0, 0, 0);
+    }
+};
+template <int DP> struct AttnCols<float, DP> {
+    typedef AttnTile<float, DP> L;
+    float f[16];
+    __device__ __forceinline__ void fetch(const char* tile, int row0, int db, int lane) {
+        const int col = lane & 31, h = lane >> 5;
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+            f[i] = *reinterpret_cast<const float*>(tile + L::place(row0 + 8 * (i / 4) + 4 * h + i % 4, db * 8 + (col >> 2)) + (col & 3) * 4);
+    }
+    __device__ __forceinline__ void mma(f32x16& acc, const AttnProb<float>& p) const {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc = __builtin_amdgcn_mfma_f32_32x32x2f32(f[i], p.v[i], acc, 0, 0, 0);
+    }
+};
 
 // A block's share of a tile on its way from global memory to LDS: fetched into registers while the previous tile is computed on
 template <typename T, int DP, int ROWS, int NT, bool VEC> struct AttnStage {
@@ -177,16 +266,6 @@ template <typename T, int DP, int ROWS, int NT, bool VEC> struct AttnStage {
             f[i] = L::template fetch<VEC>(base + (size_t)min(row0 + c / L::NCH, last) * ts, c % L::NCH, D);
         }
     }
-    // packed rows: token r / G, head r % G
-    __device__ __forceinline__ void fetch_packed(const T* base, long long ts, long long hs, int row0, int last, int G, int D) {
-#pragma unroll
-        for (int i = 0; i < CNT; ++i) {
-            const int c = threadIdx.x + i * NT;
-            if ((ROWS * L::NCH) % NT && c >= ROWS * L::NCH) break;
-            const unsigned r = min(row0 + c / L::NCH, last), t = r / (unsigned)G;
-            f[i] = L::template fetch<VEC>(base + (size_t)t * ts + (size_t)(r - t * G) * hs, c % L::NCH, D);
-        }
-    }
     __device__ __forceinline__ void store(char* tile) const {
 #pragma unroll
         for (int i = 0; i < CNT; ++i) {
@@ -194,6 +273,28 @@ template <typename T, int DP, int ROWS, int NT, bool VEC> struct AttnStage {
             if ((ROWS * L::NCH) % NT && c >= ROWS * L::NCH) break;
             *reinterpret_cast<typename L::Frag*>(tile + L::place(c / L::NCH, c % L::NCH)) = f[i];
         }
+    }
+};
+
+// Element `row` of packed rows (token row / G, head row % G) on its way towards the first row, `step` rows at a time, without a division
+template <typename P> struct AttnCursor {
+    P* p;
+    int head;
+    long long back, wrap;      // a step: `step / G` tokens and `step % G` heads back; a head below 0 is G heads on, a token before
+    int less, G;
+    __device__ __forceinline__ void set(P* base, long long ts, long long hs, int row, int step, int G_) {
+        G = G_;
+        const int t = row / G;
+        head = row - t * G;
+        p = base + (long long)t * ts + (long long)head * hs;
+        less = step % G;
+        back = (long long)(step / G) * ts + (long long)less * hs;
+        wrap = (long long)G * hs - ts;
+    }
+    __device__ __forceinline__ void move() {
+        p -= back;
+        head -= less;
+        if (head < 0) { head += G; p += wrap; }
     }
 };
 

@@ -19,7 +19,8 @@ __global__ __launch_bounds__(NW * 64) void packed_attn_fwd_kernel(const AttnGeom
     const int hk = blockIdx.x % g.Hk;
     int b, tile;
     // the last tiles of a causal sequence are the longest: they start first
-    if (!attn_find(g.off_q, g.B, g.Nq, g.G, SHIFT, slots - 1 - (int)(blockIdx.x / g.Hk), b, tile)) return;
+    if (g.sorted ? !attn_find_sorted<false>(g, BM, blockIdx.x / g.Hk, b, tile)
+                 : !attn_find(g.off_q, g.B, g.Nq, g.G, SHIFT, slots - 1 - (int)(blockIdx.x / g.Hk), b, tile)) return;
     const AttnSeq s = attn_seq(g, b);
     const int rows = s.lq * g.G;
     if (tile * BM >= rows) return;
@@ -31,12 +32,8 @@ __global__ __launch_bounds__(NW * 64) void packed_attn_fwd_kernel(const AttnGeom
     const int limit = limit_of(row);
     const int wave_lo = limit_of(row0), wave_hi = row0 < rows ? limit_of(row0 + 31) : 0, block_hi = limit_of(tile * BM + BM - 1);
 
-    typename L::Frag qf[L::KS];
-    {
-        const T* qr = (const T*)q.p + (size_t)(s.q0 + tok) * q.ts + (size_t)head * q.hs;
-#pragma unroll
-        for (int i = 0; i < L::KS; ++i) qf[i] = L::template fetch<VEC>(qr, 2 * i + h, g.D);
-    }
+    AttnRows<T, DP> qf;
+    qf.template fetch_global<VEC>((const T*)q.p + (size_t)(s.q0 + tok) * q.ts + (size_t)head * q.hs, h, g.D);
     f32x16 acc[L::DB];
 #pragma unroll
     for (int db = 0; db < L::DB; ++db) acc[db] = (f32x16)(0.f);
@@ -65,9 +62,10 @@ __global__ __launch_bounds__(NW * 64) void packed_attn_fwd_kernel(const AttnGeom
             f32x16 sc[TK / 32];
 #pragma unroll
             for (int t = 0; t < TK / 32; ++t) {
-                sc[t] = (f32x16)(0.f);
-#pragma unroll
-                for (int i = 0; i < L::KS; ++i) attn_mma(sc[t], L::frag(tk, t * 32 + col, i, h), qf[i]);
+                AttnRows<T, DP> kf;
+                kf.fetch(tk, t * 32 + col, h);
+                attn_fence();
+                sc[t] = attn_product(kf, qf);
             }
             if (j0 + TK > wave_lo) {
 #pragma unroll
@@ -102,7 +100,11 @@ __global__ __launch_bounds__(NW * 64) void packed_attn_fwd_kernel(const AttnGeom
                 AttnProb<T> p;
                 p.set(sc[t]);
 #pragma unroll
-                for (int db = 0; db < L::DB; ++db) attn_mma_t<DP>(acc[db], tv, t * 32, db, lane, p);
+                for (int db = 0; db < L::DB; ++db) {
+                    AttnCols<T, DP> vf;
+                    vf.fetch(tv, t * 32, db, lane);
+                    vf.mma(acc[db], p);
+                }
             }
         }
         if (it + 1 < tiles) {
@@ -119,10 +121,11 @@ __global__ __launch_bounds__(NW * 64) void packed_attn_fwd_kernel(const AttnGeom
 }
 
 template <typename T, int DP, int NW, int TK>
-void launch(const AttnGeom& g, const AttnTensor& q, const AttnTensor& k, const AttnTensor& v, void* out, long long o_ts, long long o_hs, float* lse,
+void launch(AttnGeom g, const AttnTensor& q, const AttnTensor& k, const AttnTensor& v, void* out, long long o_ts, long long o_hs, float* lse,
             bool vec, hipStream_t stream) {
     constexpr int SHIFT = NW == 8 ? 8 : 7;
     const int slots = attn_slots((long long)g.Nq * g.G, g.B, SHIFT);
+    g.sorted = attn_sorts(g, (long long)g.Nq * g.G, 1 << SHIFT);
     if (vec) hipLaunchKernelGGL((packed_attn_fwd_kernel<T, DP, NW, TK, true>), dim3(slots * g.Hk), dim3(NW * 64), 0, stream, g, q, k, v, (T*)out, o_ts, o_hs, lse, slots);
     else hipLaunchKernelGGL((packed_attn_fwd_kernel<T, DP, NW, TK, false>), dim3(slots * g.Hk), dim3(NW * 64), 0, stream, g, q, k, v, (T*)out, o_ts, o_hs, lse, slots);
 }

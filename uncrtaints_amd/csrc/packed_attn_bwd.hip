@@ -20,7 +20,8 @@ __global__ __launch_bounds__(NW * 64) void packed_attn_dq_kernel(const AttnGeom 
     attn_fill_outside<T>(g.off_q, g.B, g.Nq, dq, (long long)g.Hq * g.D, g.D, g.Hq, g.D, nullptr, blockIdx.x, gridDim.x);
     const int hk = blockIdx.x % g.Hk;
     int b, tile;
-    if (!attn_find(g.off_q, g.B, g.Nq, g.G, SHIFT, slots - 1 - (int)(blockIdx.x / g.Hk), b, tile)) return;
+    if (g.sorted ? !attn_find_sorted<false>(g, BM, blockIdx.x / g.Hk, b, tile)
+                 : !attn_find(g.off_q, g.B, g.Nq, g.G, SHIFT, slots - 1 - (int)(blockIdx.x / g.Hk), b, tile)) return;
     const AttnSeq s = attn_seq(g, b);
     const int rows = s.lq * g.G;
     if (tile * BM >= rows) return;
@@ -31,20 +32,17 @@ __global__ __launch_bounds__(NW * 64) void packed_attn_dq_kernel(const AttnGeom 
     const int limit = limit_of(row);
     const int wave_lo = limit_of(row0), wave_hi = row0 < rows ? limit_of(row0 + 31) : 0, block_hi = limit_of(tile * BM + BM - 1);
 
-    typename L::Frag qf[L::KS], gf[L::KS];
+    AttnRows<T, DP> qf, gf;
+    qf.template fetch_global<VEC>((const T*)q.p + (size_t)(s.q0 + tok) * q.ts + (size_t)head * q.hs, h, g.D);
+    gf.template fetch_global<VEC>((const T*)go.p + (size_t)(s.q0 + tok) * go.ts + (size_t)head * go.hs, h, g.D);
     float dl = 0.f;
     {
-        const T* qr = (const T*)q.p + (size_t)(s.q0 + tok) * q.ts + (size_t)head * q.hs;
-        const T* gr = (const T*)go.p + (size_t)(s.q0 + tok) * go.ts + (size_t)head * go.hs;
-        const T* orow = (const T*)o.p + (size_t)(s.q0 + tok) * o.ts + (size_t)head * o.hs;
+        AttnRows<T, DP> of;
+        of.template fetch_global<VEC>((const T*)o.p + (size_t)(s.q0 + tok) * o.ts + (size_t)head * o.hs, h, g.D);
 #pragma unroll
-        for (int i = 0; i < L::KS; ++i) {
-            qf[i] = L::template fetch<VEC>(qr, 2 * i + h, g.D);
-            gf[i] = L::template fetch<VEC>(gr, 2 * i + h, g.D);
-            const typename L::Frag of = L::template fetch<VEC>(orow, 2 * i + h, g.D);
+        for (int i = 0; i < L::KS; ++i)
 #pragma unroll
-            for (int e = 0; e < L::EPC; ++e) dl = fmaf((float)gf[i][e], (float)of[e], dl);
-        }
+            for (int e = 0; e < L::EPC; ++e) dl = fmaf((float)gf.f[i][e], (float)of.f[i][e], dl);
     }
     dl += attn_other_half(dl);
     const size_t at = (size_t)(s.q0 + tok) * g.Hq + head;
@@ -79,12 +77,13 @@ __global__ __launch_bounds__(NW * 64) void packed_attn_dq_kernel(const AttnGeom 
             const bool edge = j0 + TK > wave_lo;
 #pragma unroll
             for (int t = 0; t < TK / 32; ++t) {
-                f32x16 sc = (f32x16)(0.f), dp = (f32x16)(0.f);
-#pragma unroll
-                for (int i = 0; i < L::KS; ++i) {
-                    attn_mma(sc, L::frag(tk, t * 32 + col, i, h), qf[i]);
-                    attn_mma(dp, L::frag(tv, t * 32 + col, i, h), gf[i]);
-                }
+                AttnRows<T, DP> x;
+                x.fetch(tk, t * 32 + col, h);
+                attn_fence();
+                f32x16 sc = attn_product(x, qf);
+                x.fetch(tv, t * 32 + col, h);
+                attn_fence();
+                const f32x16 dp = attn_product(x, gf);
 #pragma unroll
                 for (int i = 0; i < 16; ++i) sc[i] = __builtin_amdgcn_exp2f(fmaf(sc[i], g.c, -ls)) * (dp[i] - dl);
                 if (edge) {
@@ -95,7 +94,11 @@ __global__ __launch_bounds__(NW * 64) void packed_attn_dq_kernel(const AttnGeom 
                 AttnProb<T> p;
                 p.set(sc);
 #pragma unroll
-                for (int db = 0; db < L::DB; ++db) attn_mma_t<DP>(acc[db], tk, t * 32, db, lane, p);
+                for (int db = 0; db < L::DB; ++db) {
+                    AttnCols<T, DP> kf;
+                    kf.fetch(tk, t * 32, db, lane);
+                    kf.mma(acc[db], p);
+                }
             }
         }
         if (it + 1 < tiles) {
@@ -119,10 +122,10 @@ __global__ __launch_bounds__(512) void packed_attn_dkv_kernel(const AttnGeom g, 
                                                               int slots) {
     typedef AttnTile<T, DP> L;
     constexpr int NT = 512, BN = 128, SHIFT = 7, TQ = 32;
+    constexpr bool EARLY = L::RB <= 256;       // registers for the transposed operand beside the first product (not for fp32 rows of 512 bytes)
     __shared__ alignas(16) char lds_q[3][TQ * L::RB], lds_g[3][TQ * L::RB];
     __shared__ f32x4 lds_p[2][4][4][64];
     __shared__ alignas(16) float lds_l[3][TQ], lds_d[3][TQ];
-    __shared__ alignas(16) int lds_lim[3][TQ];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5, col = lane & 31, pair = wave & 3;
     const bool second = wave >= 4;
     attn_fill_outside<T>(g.off_k, g.B, g.Nk, dk, (long long)g.Hk * g.D, g.D, g.Hk, g.D, nullptr, blockIdx.x, gridDim.x);
@@ -130,7 +133,8 @@ __global__ __launch_bounds__(512) void packed_attn_dkv_kernel(const AttnGeom g, 
     const int hk = blockIdx.x % g.Hk;
     int b, tile;
     // the first keys of a causal sequence are seen by the most rows: they start first
-    if (!attn_find(g.off_k, g.B, g.Nk, 1, SHIFT, (int)(blockIdx.x / g.Hk), b, tile)) return;
+    if (g.sorted ? !attn_find_sorted<true>(g, BN, blockIdx.x / g.Hk, b, tile)
+                 : !attn_find(g.off_k, g.B, g.Nk, 1, SHIFT, (int)(blockIdx.x / g.Hk), b, tile)) return;
     const AttnSeq s = attn_seq(g, b);
     if (tile * BN >= s.room) return;
     const int key0 = tile * BN + pair * 32, key = key0 + col;
@@ -144,97 +148,140 @@ __global__ __launch_bounds__(512) void packed_attn_dkv_kernel(const AttnGeom g, 
     if (tile * BN >= s.lk) start = rows;
     const int tiles = (rows - start + TQ - 1) / TQ;
     if (tiles > 0) {
-        typename L::Frag own[L::KS];
+        AttnRows<T, DP> own;
         {
             const AttnTensor& x = second ? v : k;
-            const T* r = (const T*)x.p + (size_t)(s.k0 + min(key, s.lk - 1)) * x.ts + (size_t)hk * x.hs;
-#pragma unroll
-            for (int i = 0; i < L::KS; ++i) own[i] = L::template fetch<VEC>(r, 2 * i + h, g.D);
+            own.template fetch_global<VEC>((const T*)x.p + (size_t)(s.k0 + min(key, s.lk - 1)) * x.ts + (size_t)hk * x.hs, h, g.D);
         }
         const T* qb = (const T*)q.p + (size_t)s.q0 * q.ts + (size_t)hk * g.G * q.hs;
         const T* gb = (const T*)go.p + (size_t)s.q0 * go.ts + (size_t)hk * g.G * go.hs;
         const float* lb = lse + (size_t)s.q0 * g.Hq + hk * g.G;
         const float* db_ = delta + (size_t)s.q0 * g.Hq + hk * g.G;
-        AttnStage<T, DP, TQ, NT, VEC> qs, gs;
+        // from the last rows to the first: the blocks of a causal sequence then walk over the same rows at the same time, and find them in L2
+        auto row_of = [&](int it) { return start + (tiles - 1 - it) * TQ; };
+        constexpr int CNT = (TQ * L::NCH + NT - 1) / NT;
+        typename L::Frag qs[CNT], gs[CNT];
+        AttnCursor<const T> cq[CNT], cg[CNT];
+        AttnCursor<const float> cl, cd;
         float fl = INFINITY, fd = 0.f;
-        int flim = 0;
-        // a row's lse in powers of two, its delta, and how many keys it sees; rows behind the last and rows that see nothing: lse = +inf
-        auto fetch_row = [&](int r0) {
+        // the first tile repeats the last row behind it: lse = +inf leaves those rows (and rows that saw nothing) without probabilities
+#pragma unroll
+        for (int i = 0; i < CNT; ++i) {
+            const int c = threadIdx.x + i * NT, r = row_of(0) + min(c / L::NCH, TQ - 1);
+            const int t = min(r, rows - 1) / g.G, hd = min(r, rows - 1) - t * g.G;
+            qs[i] = L::template fetch<VEC>(qb + (size_t)t * q.ts + (size_t)hd * q.hs, c % L::NCH, g.D);
+            gs[i] = L::template fetch<VEC>(gb + (size_t)t * go.ts + (size_t)hd * go.hs, c % L::NCH, g.D);
+            cq[i].set(qb, q.ts, q.hs, r, TQ, g.G);
+            cg[i].set(gb, go.ts, go.hs, r, TQ, g.G);
+        }
+        {
+            const int r = row_of(0) + (int)(threadIdx.x & (TQ - 1));
+            cl.set(lb, g.Hq, 1, r, TQ, g.G);
+            cd.set(db_, g.Hq, 1, r, TQ, g.G);
+            if (r < rows) {
+                fl = *cl.p * 1.4426950408889634f;
+                if (fl == -INFINITY) fl = INFINITY;
+                fd = *cd.p;
+            }
+        }
+        auto fetch = [&]() {
+#pragma unroll
+            for (int i = 0; i < CNT; ++i) {
+                cq[i].move();
+                cg[i].move();
+                const int c = threadIdx.x + i * NT;
+                if ((TQ * L::NCH) % NT && c >= TQ * L::NCH) break;
+                qs[i] = L::template fetch<VEC>(cq[i].p, c % L::NCH, g.D);
+                gs[i] = L::template fetch<VEC>(cg[i].p, c % L::NCH, g.D);
+            }
             if (threadIdx.x < TQ) {
-                const unsigned r = r0 + threadIdx.x;
-                const unsigned rr = min((int)r, rows - 1), t = rr / (unsigned)g.G;
-                const size_t at = (size_t)t * g.Hq + (rr - t * g.G);
-                fl = lb[at] * 1.4426950408889634f;
-                if (fl == -INFINITY || (int)r >= rows) fl = INFINITY;
-                fd = (int)r >= rows ? 0.f : db_[at];
-                flim = g.causal ? (int)t + shift + 1 : s.lk;
+                cl.move();
+                cd.move();
+                fl = *cl.p;
+                fd = *cd.p;
             }
         };
-        auto store = [&](int buf) {
-            qs.store(lds_q[buf]);
-            gs.store(lds_g[buf]);
+        auto store = [&](int buf, bool raw) {
+#pragma unroll
+            for (int i = 0; i < CNT; ++i) {
+                const int c = threadIdx.x + i * NT;
+                if ((TQ * L::NCH) % NT && c >= TQ * L::NCH) break;
+                *reinterpret_cast<typename L::Frag*>(lds_q[buf] + L::place(c / L::NCH, c % L::NCH)) = qs[i];
+                *reinterpret_cast<typename L::Frag*>(lds_g[buf] + L::place(c / L::NCH, c % L::NCH)) = gs[i];
+            }
             if (threadIdx.x < TQ) {
-                lds_l[buf][threadIdx.x] = fl;
+                lds_l[buf][threadIdx.x] = !raw ? fl : fl == -INFINITY ? INFINITY : fl * 1.4426950408889634f;
                 lds_d[buf][threadIdx.x] = fd;
-                lds_lim[buf][threadIdx.x] = flim;
             }
         };
-        auto fetch = [&](int r0) {
-            qs.fetch_packed(qb, q.ts, q.hs, r0, rows - 1, g.G, g.D);
-            gs.fetch_packed(gb, go.ts, go.hs, r0, rows - 1, g.G, g.D);
-            fetch_row(r0);
-        };
-        // the tile's last row sees keys below its limit: a pair whose keys all lie behind has nothing to do with the tile
-        auto seen = [&](int it) {
-            const int last = min(start + it * TQ + TQ, rows) - 1;
-            return key0 < s.lk && (!g.causal || key0 < last / g.G + shift + 1);
-        };
-        fetch(start);
-        store(0);
+        // causal: a key is seen by the rows from (key - shift) * G on.  Tiles before `seen` have none for this pair's keys, tiles from
+        // `whole` on see all of them
+        const int first = g.causal ? max(key - shift, 0) * g.G : 0;
+        const int seen = key0 >= s.lk ? rows : g.causal ? max(key0 - shift, 0) * g.G : 0, whole = g.causal ? max(key0 + 31 - shift, 0) * g.G : 0;
+        store(0, false);
         __syncthreads();
         int cur = 0, prev = 2, next = 1;
         for (int it = 0; it <= tiles; ++it) {
-            if (it + 1 < tiles) fetch(start + (it + 1) * TQ);
+            if (it + 1 < tiles) fetch();
             if (!second) {
-                if (it < tiles && seen(it)) {
-                    f32x16 sc = (f32x16)(0.f);
+                const int r0 = row_of(it);
+                if (it < tiles && min(r0 + TQ, rows) > seen) {
+                    AttnRows<T, DP> x;
+                    x.fetch(lds_q[cur], col, h);
+                    f32x4 ls[4];
 #pragma unroll
-                    for (int i = 0; i < L::KS; ++i) attn_mma(sc, L::frag(lds_q[cur], col, i, h), own[i]);
+                    for (int e = 0; e < 4; ++e) ls[e] = *reinterpret_cast<const f32x4*>(&lds_l[cur][8 * e + 4 * h]);
+                    attn_fence();
+                    f32x16 sc = attn_product(x, own);
+                    AttnCols<T, DP> y[L::DB];
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const f32x4 ls = *reinterpret_cast<const f32x4*>(&lds_l[cur][8 * e + 4 * h]);
+                    for (int db = 0; db < L::DB; ++db)
+                        if (EARLY) y[db].fetch(lds_g[cur], 0, db, lane);
+                    attn_fence();
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) sc[4 * e + i] = __builtin_amdgcn_exp2f(fmaf(sc[4 * e + i], g.c, -ls[i]));
-                    }
-                    if (g.causal && lds_lim[cur][0] < key0 + 32) {
+                    for (int i = 0; i < 16; ++i) sc[i] = __builtin_amdgcn_exp2f(fmaf(sc[i], g.c, -ls[i / 4][i % 4]));
+                    if (r0 < whole) {
 #pragma unroll
                         for (int i = 0; i < 16; ++i)
-                            if (key >= lds_lim[cur][8 * (i / 4) + 4 * h + i % 4]) sc[i] = 0.f;
+                            if (r0 + 8 * (i / 4) + 4 * h + i % 4 < first) sc[i] = 0.f;
                     }
 #pragma unroll
                     for (int e = 0; e < 4; ++e) lds_p[it & 1][pair][e][lane] = (f32x4){sc[4 * e], sc[4 * e + 1], sc[4 * e + 2], sc[4 * e + 3]};
                     AttnProb<T> p;
                     p.set(sc);
 #pragma unroll
-                    for (int db = 0; db < L::DB; ++db) attn_mma_t<DP>(acc[db], lds_g[cur], 0, db, lane, p);
+                    for (int db = 0; db < L::DB; ++db) {
+                        if (!EARLY) y[db].fetch(lds_g[cur], 0, db, lane);
+                        y[db].mma(acc[db], p);
+                    }
                 }
-            } else if (it > 0 && seen(it - 1)) {
-                f32x16 dp = (f32x16)(0.f);
-#pragma unroll
-                for (int i = 0; i < L::KS; ++i) attn_mma(dp, L::frag(lds_g[prev], col, i, h), own[i]);
+            } else if (it > 0 && min(row_of(it - 1) + TQ, rows) > seen) {
+                AttnRows<T, DP> x;
+                x.fetch(lds_g[prev], col, h);
+                f32x4 dl[4], p[4];
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const f32x4 dl = *reinterpret_cast<const f32x4*>(&lds_d[prev][8 * e + 4 * h]);
-                    const f32x4 p = lds_p[(it - 1) & 1][pair][e][lane];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) dp[4 * e + i] = p[i] * (dp[4 * e + i] - dl[i]);
+                    dl[e] = *reinterpret_cast<const f32x4*>(&lds_d[prev][8 * e + 4 * h]);
+                    p[e] = lds_p[(it - 1) & 1][pair][e][lane];
                 }
+                attn_fence();
+                f32x16 dp = attn_product(x, own);
+                AttnCols<T, DP> y[L::DB];
+#pragma unroll
+                for (int db = 0; db < L::DB; ++db)
+                    if (EARLY) y[db].fetch(lds_q[prev], 0, db, lane);
+                attn_fence();
+#pragma unroll
+                for (int i = 0; i < 16; ++i) dp[i] = p[i / 4][i % 4] * (dp[i] - dl[i / 4][i % 4]);
                 AttnProb<T> ds;
                 ds.set(dp);
 #pragma unroll
-                for (int db = 0; db < L::DB; ++db) attn_mma_t<DP>(acc[db], lds_q[prev], 0, db, lane, ds);
+                for (int db = 0; db < L::DB; ++db) {
+                    if (!EARLY) y[db].fetch(lds_q[prev], 0, db, lane);
+                    y[db].mma(acc[db], ds);
+                }
             }
-            if (it + 1 < tiles) store(next);
+            if (it + 1 < tiles) store(next, true);
             __syncthreads();
             const int t = prev;
             prev = cur;
@@ -261,12 +308,15 @@ struct Bwd {
 };
 
 template <typename T, int DP, int NW, int TK, bool VEC> void launch_v(const Bwd& a) {
+    AttnGeom gq = a.g, gk = a.g;
+    gq.sorted = attn_sorts(a.g, (long long)a.g.Nq * a.g.G, NW * 32);
+    gk.sorted = attn_sorts(a.g, a.g.Nk, 128);
     const int sq = attn_slots((long long)a.g.Nq * a.g.G, a.g.B, NW == 8 ? 8 : 7), sk = attn_slots(a.g.Nk, a.g.B, 7);
     if (a.g.Nq)
-        hipLaunchKernelGGL((packed_attn_dq_kernel<T, DP, NW, TK, VEC>), dim3(sq * a.g.Hk), dim3(NW * 64), 0, a.stream, a.g, a.q, a.k, a.v, a.o, a.go,
+        hipLaunchKernelGGL((packed_attn_dq_kernel<T, DP, NW, TK, VEC>), dim3(sq * a.g.Hk), dim3(NW * 64), 0, a.stream, gq, a.q, a.k, a.v, a.o, a.go,
                            a.lse, (T*)a.dq, a.delta, sq);
     if (a.g.Nk)
-        hipLaunchKernelGGL((packed_attn_dkv_kernel<T, DP, VEC>), dim3(sk * a.g.Hk), dim3(512), 0, a.stream, a.g, a.q, a.k, a.v, a.go, a.lse,
+        hipLaunchKernelGGL((packed_attn_dkv_kernel<T, DP, VEC>), dim3(sk * a.g.Hk), dim3(512), 0, a.stream, gk, a.q, a.k, a.v, a.go, a.lse,
                            a.delta, (T*)a.dk, (T*)a.dv, sk);
 }
 template <typename T, int DP, int NW, int TK> void launch(const Bwd& a) {
