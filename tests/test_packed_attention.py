@@ -457,7 +457,7 @@ def test_entry_points_refuse_bad_sizes():
     bwd = hb.lib().fn["uncr_packed_attn_bwd"]
     names = [n for _, n in hb.parse_header()["uncr_packed_attn_bwd"]]
     ok2 = dict.fromkeys(names, 0)
-    ok2.update(q=16, k=16, v=16, out=16, dout=16, lse=16, dq=16, dk=16, dv=16, delta=16, off_q=16, off_k=16, k_len=None, temperature=1.0, B=1, Nq=2, Nk=2, Hq=4,
+    ok2.update(q=16, k=16, v=16, out=16, dout=16, lse=16, dq=16, dk=16, dv=16, rowstat=16, off_q=16, off_k=16, k_len=None, temperature=1.0, B=1, Nq=2, Nk=2, Hq=4,
                Hk=2, D=8, stream=None)
-    for kw in (dict(Hq=5), dict(D=200), dict(lse=None), dict(delta=None), dict(dq=None), dict(dk=None), dict(v=None), dict(dk=24 - 4), dict(act=-1)):
+    for kw in (dict(Hq=5), dict(D=200), dict(lse=None), dict(rowstat=None), dict(dq=None), dict(dk=None), dict(v=None), dict(dk=24 - 4), dict(act=-1)):
         assert bwd(*{**ok2, **kw}.values()) < 0, kw

@@ -200,6 +200,13 @@ template <typename T, int DP> __device__ __forceinline__ f32x16 attn_product(con
 template <typename T> struct AttnProb;
 template <> struct AttnProb<__bf16> {
     bf16x8 v[2];
+    __device__ __forceinline__ float get(int i) const { return (float)v[i / 8][i % 8]; }
+    __device__ __forceinline__ void save(f32x4* at, int lane) const {
+        for (int u = 0; u < 2; ++u) at[u * 64 + lane] = __builtin_bit_cast(f32x4, v[u]);
+    }
+    __device__ __forceinline__ void load(const f32x4* at, int lane) {
+        for (int u = 0; u < 2; ++u) v[u] = __builtin_bit_cast(bf16x8, at[u * 64 + lane]);
+    }
     __device__ __forceinline__ void set(const f32x16& p) {
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
@@ -212,6 +219,19 @@ template <> struct AttnProb<__bf16> {
 };
 template <> struct AttnProb<float> {
     f32x16 v;
+    __device__ __forceinline__ float get(int i) const { return v[i]; }
+    __device__ __forceinline__ void save(f32x4* at, int lane) const {
+#pragma unroll
+        for (int u = 0; u < 4; ++u) at[u * 64 + lane] = (f32x4){v[4 * u], v[4 * u + 1], v[4 * u + 2], v[4 * u + 3]};
+    }
+    __device__ __forceinline__ void load(const f32x4* at, int lane) {
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const f32x4 x = at[u * 64 + lane];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[4 * u + i] = x[i];
+        }
+    }
     __device__ __forceinline__ void set(const f32x16& p) { v = p; }
 };
 
@@ -252,26 +272,51 @@ template <int DP> struct AttnCols<float, DP> {
     }
 };
 
-// A block's share of a tile on its way from global memory to LDS: fetched into registers while the previous tile is computed on
+// 16 bytes per lane from global memory straight to LDS, lane i at `lds` + 16 i (`lds` the same for the wave); 4 bytes per lane likewise.  No
+// registers are held and no LDS writes issued on the way.  The compiler does not see these loads: attn_arrived() waits for them, and it may
+// only wait longer for its own loads than it thinks, never shorter.
+__device__ __forceinline__ void attn_dma16(void* lds, const void* src) {
+    const unsigned at = __builtin_amdgcn_readfirstlane((unsigned)(size_t)(__attribute__((address_space(3))) char*)lds);
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(at), "v"(src) : "memory", "m0");
+}
+__device__ __forceinline__ void attn_dma4(void* lds, const void* src) {
+    const unsigned at = __builtin_amdgcn_readfirstlane((unsigned)(size_t)(__attribute__((address_space(3))) char*)lds);
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(at), "v"(src) : "memory", "m0");
+}
+__device__ __forceinline__ void attn_arrived() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+
+static __device__ const f32x4 attn_zeros = {0.f, 0.f, 0.f, 0.f};      // what chunks behind D are loaded from
+
+// A block's share of a tile on its way from global memory to LDS while the previous tile is computed on: straight (VEC), or through registers,
+// element by element
 template <typename T, int DP, int ROWS, int NT, bool VEC> struct AttnStage {
     typedef AttnTile<T, DP> L;
     static constexpr int CNT = (ROWS * L::NCH + NT - 1) / NT;
-    typename L::Frag f[CNT];
-    // rows row0 ..: those behind `last` repeat it (their products are masked)
-    __device__ __forceinline__ void fetch(const T* base, long long ts, int row0, int last, int D) {
-#pragma unroll
-        for (int i = 0; i < CNT; ++i) {
-            const int c = threadIdx.x + i * NT;
-            if ((ROWS * L::NCH) % NT && c >= ROWS * L::NCH) break;
-            f[i] = L::template fetch<VEC>(base + (size_t)min(row0 + c / L::NCH, last) * ts, c % L::NCH, D);
+    typename L::Frag f[VEC ? 1 : CNT];
+    static __device__ __forceinline__ bool idle(int c) { return (ROWS * L::NCH) % NT && c >= ROWS * L::NCH; }
+    // the chunk of a row that belongs at place c of the tile
+    static __device__ __forceinline__ int chunk(int c) { return (c % L::NCH) ^ L::swizzle(c / L::NCH); }
+    __device__ __forceinline__ void begin(int i, char* tile, const T* row, int D) {
+        const int c = threadIdx.x + i * NT;
+        if (idle(c)) return;
+        if (VEC) {
+            const T* p = row + chunk(c) * L::EPC;
+            attn_dma16(tile + (c & ~63) * 16, chunk(c) * L::EPC < D ? (const void*)p : (const void*)&attn_zeros);
+        } else {
+            f[i] = L::template fetch<false>(row, chunk(c), D);
         }
     }
-    __device__ __forceinline__ void store(char* tile) const {
+    // rows row0 ..: those behind `last` repeat it (their products are masked)
+    __device__ __forceinline__ void begin(char* tile, const T* base, long long ts, int row0, int last, int D) {
+#pragma unroll
+        for (int i = 0; i < CNT; ++i) begin(i, tile, base + (size_t)min(row0 + (int)(threadIdx.x + i * NT) / L::NCH, last) * ts, D);
+    }
+    __device__ __forceinline__ void finish(char* tile) const {
+        if (VEC) return;
 #pragma unroll
         for (int i = 0; i < CNT; ++i) {
             const int c = threadIdx.x + i * NT;
-            if ((ROWS * L::NCH) % NT && c >= ROWS * L::NCH) break;
-            *reinterpret_cast<typename L::Frag*>(tile + L::place(c / L::NCH, c % L::NCH)) = f[i];
+            if (!idle(c)) *reinterpret_cast<typename L::Frag*>(tile + c * 16) = f[i];
         }
     }
 };

@@ -44,17 +44,18 @@ __global__ __launch_bounds__(NW * 64) void packed_attn_fwd_kernel(const AttnGeom
     const int tiles = (block_hi + TK - 1) / TK;
     AttnStage<T, DP, TK, NT, VEC> ks, vs;
     if (tiles) {
-        ks.fetch(kb, k.ts, 0, s.lk - 1, g.D);
-        vs.fetch(vb, v.ts, 0, s.lk - 1, g.D);
-        ks.store(lds_k[0]);
-        vs.store(lds_v[0]);
+        ks.begin(lds_k[0], kb, k.ts, 0, s.lk - 1, g.D);
+        vs.begin(lds_v[0], vb, v.ts, 0, s.lk - 1, g.D);
+        ks.finish(lds_k[0]);
+        vs.finish(lds_v[0]);
     }
+    attn_arrived();
     __syncthreads();
     for (int it = 0; it < tiles; ++it) {
         const int j0 = it * TK;
         if (it + 1 < tiles) {
-            ks.fetch(kb, k.ts, j0 + TK, s.lk - 1, g.D);
-            vs.fetch(vb, v.ts, j0 + TK, s.lk - 1, g.D);
+            ks.begin(lds_k[(it + 1) & 1], kb, k.ts, j0 + TK, s.lk - 1, g.D);
+            vs.begin(lds_v[(it + 1) & 1], vb, v.ts, j0 + TK, s.lk - 1, g.D);
         }
         if (j0 < wave_hi) {
             const char* tk = lds_k[it & 1];
@@ -108,9 +109,10 @@ __global__ __launch_bounds__(NW * 64) void packed_attn_fwd_kernel(const AttnGeom
             }
         }
         if (it + 1 < tiles) {
-            ks.store(lds_k[(it + 1) & 1]);
-            vs.store(lds_v[(it + 1) & 1]);
+            ks.finish(lds_k[(it + 1) & 1]);
+            vs.finish(lds_v[(it + 1) & 1]);
         }
+        attn_arrived();
         __syncthreads();
     }
     l += attn_other_half(l);

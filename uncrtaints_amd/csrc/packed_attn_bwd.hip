@@ -12,7 +12,7 @@ namespace {
 template <typename T, int DP, int NW, int TK, bool VEC>
 __global__ __launch_bounds__(NW * 64) void packed_attn_dq_kernel(const AttnGeom g, const AttnTensor q, const AttnTensor k, const AttnTensor v,
                                                                  const AttnTensor o, const AttnTensor go, const float* __restrict__ lse,
-                                                                 T* __restrict__ dq, float* __restrict__ delta, int slots) {
+                                                                 T* __restrict__ dq, float* __restrict__ rowstat, int slots) {
     typedef AttnTile<T, DP> L;
     constexpr int NT = NW * 64, BM = NW * 32, SHIFT = NW == 8 ? 8 : 7;
     __shared__ alignas(16) char lds_k[2][TK * L::RB], lds_v[2][TK * L::RB];
@@ -46,10 +46,13 @@ __global__ __launch_bounds__(NW * 64) void packed_attn_dq_kernel(const AttnGeom 
     }
     dl += attn_other_half(dl);
     const size_t at = (size_t)(s.q0 + tok) * g.Hq + head;
-    if (h == 0 && row0 + col < rows) delta[at] = dl;
     // a row that saw nothing has lse = -inf: +inf makes its probabilities 0
     float ls = lse[at] * 1.4426950408889634f;
     if (ls == -INFINITY) ls = INFINITY;
+    if (h == 0 && row0 + col < rows) {          // for the dK/dV kernel: lse in powers of two, and delta behind it
+        rowstat[at] = ls;
+        rowstat[(size_t)g.Nq * g.Hq + at] = dl;
+    }
 
     f32x16 acc[L::DB];
 #pragma unroll
@@ -59,17 +62,18 @@ __global__ __launch_bounds__(NW * 64) void packed_attn_dq_kernel(const AttnGeom 
     const int tiles = (block_hi + TK - 1) / TK;
     AttnStage<T, DP, TK, NT, VEC> ks, vs;
     if (tiles) {
-        ks.fetch(kb, k.ts, 0, s.lk - 1, g.D);
-        vs.fetch(vb, v.ts, 0, s.lk - 1, g.D);
-        ks.store(lds_k[0]);
-        vs.store(lds_v[0]);
+        ks.begin(lds_k[0], kb, k.ts, 0, s.lk - 1, g.D);
+        vs.begin(lds_v[0], vb, v.ts, 0, s.lk - 1, g.D);
+        ks.finish(lds_k[0]);
+        vs.finish(lds_v[0]);
     }
+    attn_arrived();
     __syncthreads();
     for (int it = 0; it < tiles; ++it) {
         const int j0 = it * TK;
         if (it + 1 < tiles) {
-            ks.fetch(kb, k.ts, j0 + TK, s.lk - 1, g.D);
-            vs.fetch(vb, v.ts, j0 + TK, s.lk - 1, g.D);
+            ks.begin(lds_k[(it + 1) & 1], kb, k.ts, j0 + TK, s.lk - 1, g.D);
+            vs.begin(lds_v[(it + 1) & 1], vb, v.ts, j0 + TK, s.lk - 1, g.D);
         }
         if (j0 < wave_hi) {
             const char* tk = lds_k[it & 1];
@@ -102,9 +106,10 @@ __global__ __launch_bounds__(NW * 64) void packed_attn_dq_kernel(const AttnGeom 
             }
         }
         if (it + 1 < tiles) {
-            ks.store(lds_k[(it + 1) & 1]);
-            vs.store(lds_v[(it + 1) & 1]);
+            ks.finish(lds_k[(it + 1) & 1]);
+            vs.finish(lds_v[(it + 1) & 1]);
         }
+        attn_arrived();
         __syncthreads();
     }
     if (row0 + col < rows) attn_store_row<T, L::DB>(dq + at * g.D, acc, g.scale, h, g.D);
@@ -114,18 +119,17 @@ __global__ __launch_bounds__(NW * 64) void packed_attn_dq_kernel(const AttnGeom 
 //   first:  S = Q K^T, P = exp2(S c - lse), P to LDS, dV^T += dOut^T P          second, one tile behind:  dP = dOut V^T, dS, dK^T += Q^T dS
 // Both make half of the products and hold half of the accumulators (one wave with both needs 470 registers and leaves one wave per SIMD with
 // nothing to run beside it); the exponentials of one wave run beside the products of the other.  P crosses in the accumulator layout, lane
-// by lane, in fp32.  Q and dOut tiles rotate through three buffers: the one being filled and those of the two roles.
+// by lane, in the storage type: bf16 rounds it once for both products it takes part in.  Q and dOut tiles rotate through three buffers: the one being filled and those of the two roles.
 template <typename T, int DP, bool VEC>
 __global__ __launch_bounds__(512) void packed_attn_dkv_kernel(const AttnGeom g, const AttnTensor q, const AttnTensor k, const AttnTensor v,
-                                                              const AttnTensor go, const float* __restrict__ lse,
-                                                              const float* __restrict__ delta, T* __restrict__ dk, T* __restrict__ dv,
-                                                              int slots) {
+                                                              const AttnTensor go, const float* __restrict__ rowstat,
+                                                              T* __restrict__ dk, T* __restrict__ dv, int slots) {
     typedef AttnTile<T, DP> L;
-    constexpr int NT = 512, BN = 128, SHIFT = 7, TQ = 32;
+    constexpr int NT = 512, BN = 128, SHIFT = 7, TQ = sizeof(T) == 2 ? 64 : 32;
     constexpr bool EARLY = L::RB <= 256;       // registers for the transposed operand beside the first product (not for fp32 rows of 512 bytes)
     __shared__ alignas(16) char lds_q[3][TQ * L::RB], lds_g[3][TQ * L::RB];
-    __shared__ f32x4 lds_p[2][4][4][64];
-    __shared__ alignas(16) float lds_l[3][TQ], lds_d[3][TQ];
+    __shared__ f32x4 lds_p[2][4][TQ / 32][sizeof(AttnProb<T>) / 16][64];
+    __shared__ alignas(16) float lds_s[3][2][64];       // lse in powers of two and delta of a tile's rows
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5, col = lane & 31, pair = wave & 3;
     const bool second = wave >= 4;
     attn_fill_outside<T>(g.off_k, g.B, g.Nk, dk, (long long)g.Hk * g.D, g.D, g.Hk, g.D, nullptr, blockIdx.x, gridDim.x);
@@ -155,133 +159,121 @@ __global__ __launch_bounds__(512) void packed_attn_dkv_kernel(const AttnGeom g, 
         }
         const T* qb = (const T*)q.p + (size_t)s.q0 * q.ts + (size_t)hk * g.G * q.hs;
         const T* gb = (const T*)go.p + (size_t)s.q0 * go.ts + (size_t)hk * g.G * go.hs;
-        const float* lb = lse + (size_t)s.q0 * g.Hq + hk * g.G;
-        const float* db_ = delta + (size_t)s.q0 * g.Hq + hk * g.G;
+        const float* lb = rowstat + (second ? (size_t)g.Nq * g.Hq : 0) + (size_t)s.q0 * g.Hq + hk * g.G;
         // from the last rows to the first: the blocks of a causal sequence then walk over the same rows at the same time, and find them in L2
         auto row_of = [&](int it) { return start + (tiles - 1 - it) * TQ; };
-        constexpr int CNT = (TQ * L::NCH + NT - 1) / NT;
-        typename L::Frag qs[CNT], gs[CNT];
-        AttnCursor<const T> cq[CNT], cg[CNT];
-        AttnCursor<const float> cl, cd;
-        float fl = INFINITY, fd = 0.f;
-        // the first tile repeats the last row behind it: lse = +inf leaves those rows (and rows that saw nothing) without probabilities
+        typedef AttnStage<T, DP, TQ, NT, VEC> Stage;
+        Stage qs, gs;
+        AttnCursor<const T> cq[Stage::CNT], cg[Stage::CNT];
+        AttnCursor<const float> cl;
+        // lse (first waves) and delta (second waves) of 64 rows go to LDS in fours of waves, 16 rows each
+        const int lrow = pair * 16 + (lane & 15);
+        const bool lme = lane < 16 && lrow < TQ;
+        // the first tile repeats the last row behind it, and masks it
 #pragma unroll
-        for (int i = 0; i < CNT; ++i) {
-            const int c = threadIdx.x + i * NT, r = row_of(0) + min(c / L::NCH, TQ - 1);
+        for (int i = 0; i < Stage::CNT; ++i) {
+            const int r = row_of(0) + min((int)(threadIdx.x + i * NT) / L::NCH, TQ - 1);
             const int t = min(r, rows - 1) / g.G, hd = min(r, rows - 1) - t * g.G;
-            qs[i] = L::template fetch<VEC>(qb + (size_t)t * q.ts + (size_t)hd * q.hs, c % L::NCH, g.D);
-            gs[i] = L::template fetch<VEC>(gb + (size_t)t * go.ts + (size_t)hd * go.hs, c % L::NCH, g.D);
+            qs.begin(i, lds_q[0], qb + (size_t)t * q.ts + (size_t)hd * q.hs, g.D);
+            gs.begin(i, lds_g[0], gb + (size_t)t * go.ts + (size_t)hd * go.hs, g.D);
             cq[i].set(qb, q.ts, q.hs, r, TQ, g.G);
             cg[i].set(gb, go.ts, go.hs, r, TQ, g.G);
         }
         {
-            const int r = row_of(0) + (int)(threadIdx.x & (TQ - 1));
+            const int r = row_of(0) + min(lrow, TQ - 1), t = min(r, rows - 1) / g.G;
+            if (lme) attn_dma4(&lds_s[0][second][pair * 16], lb + (size_t)t * g.Hq + (min(r, rows - 1) - t * g.G));
             cl.set(lb, g.Hq, 1, r, TQ, g.G);
-            cd.set(db_, g.Hq, 1, r, TQ, g.G);
-            if (r < rows) {
-                fl = *cl.p * 1.4426950408889634f;
-                if (fl == -INFINITY) fl = INFINITY;
-                fd = *cd.p;
-            }
         }
-        auto fetch = [&]() {
+        auto begin = [&](int buf) {
 #pragma unroll
-            for (int i = 0; i < CNT; ++i) {
+            for (int i = 0; i < Stage::CNT; ++i) {
                 cq[i].move();
                 cg[i].move();
-                const int c = threadIdx.x + i * NT;
-                if ((TQ * L::NCH) % NT && c >= TQ * L::NCH) break;
-                qs[i] = L::template fetch<VEC>(cq[i].p, c % L::NCH, g.D);
-                gs[i] = L::template fetch<VEC>(cg[i].p, c % L::NCH, g.D);
+                qs.begin(i, lds_q[buf], cq[i].p, g.D);
+                gs.begin(i, lds_g[buf], cg[i].p, g.D);
             }
-            if (threadIdx.x < TQ) {
-                cl.move();
-                cd.move();
-                fl = *cl.p;
-                fd = *cd.p;
-            }
+            cl.move();
+            if (lme) attn_dma4(&lds_s[buf][second][pair * 16], cl.p);
         };
-        auto store = [&](int buf, bool raw) {
-#pragma unroll
-            for (int i = 0; i < CNT; ++i) {
-                const int c = threadIdx.x + i * NT;
-                if ((TQ * L::NCH) % NT && c >= TQ * L::NCH) break;
-                *reinterpret_cast<typename L::Frag*>(lds_q[buf] + L::place(c / L::NCH, c % L::NCH)) = qs[i];
-                *reinterpret_cast<typename L::Frag*>(lds_g[buf] + L::place(c / L::NCH, c % L::NCH)) = gs[i];
-            }
-            if (threadIdx.x < TQ) {
-                lds_l[buf][threadIdx.x] = !raw ? fl : fl == -INFINITY ? INFINITY : fl * 1.4426950408889634f;
-                lds_d[buf][threadIdx.x] = fd;
-            }
+        auto finish = [&](int buf) {
+            qs.finish(lds_q[buf]);
+            gs.finish(lds_g[buf]);
+            attn_arrived();
         };
         // causal: a key is seen by the rows from (key - shift) * G on.  Tiles before `seen` have none for this pair's keys, tiles from
         // `whole` on see all of them
         const int first = g.causal ? max(key - shift, 0) * g.G : 0;
         const int seen = key0 >= s.lk ? rows : g.causal ? max(key0 - shift, 0) * g.G : 0, whole = g.causal ? max(key0 + 31 - shift, 0) * g.G : 0;
-        store(0, false);
+        finish(0);
         __syncthreads();
         int cur = 0, prev = 2, next = 1;
         for (int it = 0; it <= tiles; ++it) {
-            if (it + 1 < tiles) fetch();
+            if (it + 1 < tiles) begin(next);
             if (!second) {
                 const int r0 = row_of(it);
                 if (it < tiles && min(r0 + TQ, rows) > seen) {
-                    AttnRows<T, DP> x;
-                    x.fetch(lds_q[cur], col, h);
-                    f32x4 ls[4];
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) ls[e] = *reinterpret_cast<const f32x4*>(&lds_l[cur][8 * e + 4 * h]);
-                    attn_fence();
-                    f32x16 sc = attn_product(x, own);
-                    AttnCols<T, DP> y[L::DB];
+                    for (int t = 0; t < TQ / 32; ++t) {
+                        AttnRows<T, DP> x;
+                        x.fetch(lds_q[cur], t * 32 + col, h);
+                        attn_fence();
+                        f32x16 sc = attn_product(x, own);
+                        f32x4 ls[4];
 #pragma unroll
-                    for (int db = 0; db < L::DB; ++db)
-                        if (EARLY) y[db].fetch(lds_g[cur], 0, db, lane);
-                    attn_fence();
+                        for (int e = 0; e < 4; ++e) ls[e] = *reinterpret_cast<const f32x4*>(&lds_s[cur][0][t * 32 + 8 * e + 4 * h]);
+                        AttnCols<T, DP> y[L::DB];
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) sc[i] = __builtin_amdgcn_exp2f(fmaf(sc[i], g.c, -ls[i / 4][i % 4]));
-                    if (r0 < whole) {
+                        for (int db = 0; db < L::DB; ++db)
+                            if (EARLY) y[db].fetch(lds_g[cur], t * 32, db, lane);
+                        attn_fence();
 #pragma unroll
-                        for (int i = 0; i < 16; ++i)
-                            if (r0 + 8 * (i / 4) + 4 * h + i % 4 < first) sc[i] = 0.f;
-                    }
+                        for (int i = 0; i < 16; ++i) sc[i] = __builtin_amdgcn_exp2f(fmaf(sc[i], g.c, -ls[i / 4][i % 4]));
+                        if (r0 < whole || r0 + TQ > rows) {
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) lds_p[it & 1][pair][e][lane] = (f32x4){sc[4 * e], sc[4 * e + 1], sc[4 * e + 2], sc[4 * e + 3]};
-                    AttnProb<T> p;
-                    p.set(sc);
+                            for (int i = 0; i < 16; ++i) {
+                                const int r = r0 + t * 32 + 8 * (i / 4) + 4 * h + i % 4;
+                                if (r < first || r >= rows) sc[i] = 0.f;
+                            }
+                        }
+                        AttnProb<T> p;
+                        p.set(sc);
+                        p.save(&lds_p[it & 1][pair][t][0][0], lane);
 #pragma unroll
-                    for (int db = 0; db < L::DB; ++db) {
-                        if (!EARLY) y[db].fetch(lds_g[cur], 0, db, lane);
-                        y[db].mma(acc[db], p);
+                        for (int db = 0; db < L::DB; ++db) {
+                            if (!EARLY) y[db].fetch(lds_g[cur], t * 32, db, lane);
+                            y[db].mma(acc[db], p);
+                        }
                     }
                 }
             } else if (it > 0 && min(row_of(it - 1) + TQ, rows) > seen) {
-                AttnRows<T, DP> x;
-                x.fetch(lds_g[prev], col, h);
-                f32x4 dl[4], p[4];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    dl[e] = *reinterpret_cast<const f32x4*>(&lds_d[prev][8 * e + 4 * h]);
-                    p[e] = lds_p[(it - 1) & 1][pair][e][lane];
-                }
-                attn_fence();
-                f32x16 dp = attn_product(x, own);
-                AttnCols<T, DP> y[L::DB];
+                for (int t = 0; t < TQ / 32; ++t) {
+                    AttnRows<T, DP> x;
+                    x.fetch(lds_g[prev], t * 32 + col, h);
+                    attn_fence();
+                    f32x16 dp = attn_product(x, own);
+                    f32x4 dl[4];
 #pragma unroll
-                for (int db = 0; db < L::DB; ++db)
-                    if (EARLY) y[db].fetch(lds_q[prev], 0, db, lane);
-                attn_fence();
+                    for (int e = 0; e < 4; ++e) dl[e] = *reinterpret_cast<const f32x4*>(&lds_s[prev][1][t * 32 + 8 * e + 4 * h]);
+                    AttnProb<T> p;
+                    p.load(&lds_p[(it - 1) & 1][pair][t][0][0], lane);
+                    AttnCols<T, DP> y[L::DB];
 #pragma unroll
-                for (int i = 0; i < 16; ++i) dp[i] = p[i / 4][i % 4] * (dp[i] - dl[i / 4][i % 4]);
-                AttnProb<T> ds;
-                ds.set(dp);
+                    for (int db = 0; db < L::DB; ++db)
+                        if (EARLY) y[db].fetch(lds_q[prev], t * 32, db, lane);
+                    attn_fence();
 #pragma unroll
-                for (int db = 0; db < L::DB; ++db) {
-                    if (!EARLY) y[db].fetch(lds_q[prev], 0, db, lane);
-                    y[db].mma(acc[db], ds);
+                    for (int i = 0; i < 16; ++i) dp[i] = p.get(i) * (dp[i] - dl[i / 4][i % 4]);
+                    AttnProb<T> ds;
+                    ds.set(dp);
+#pragma unroll
+                    for (int db = 0; db < L::DB; ++db) {
+                        if (!EARLY) y[db].fetch(lds_q[prev], t * 32, db, lane);
+                        y[db].mma(acc[db], ds);
+                    }
                 }
             }
-            if (it + 1 < tiles) store(next, true);
+            if (it + 1 < tiles) finish(next);
             __syncthreads();
             const int t = prev;
             prev = cur;
@@ -302,7 +294,7 @@ struct Bwd {
     AttnTensor q, k, v, o, go;
     const float* lse;
     void *dq, *dk, *dv;
-    float* delta;
+    float* rowstat;
     bool vec;
     hipStream_t stream;
 };
@@ -314,10 +306,10 @@ template <typename T, int DP, int NW, int TK, bool VEC> void launch_v(const Bwd&
     const int sq = attn_slots((long long)a.g.Nq * a.g.G, a.g.B, NW == 8 ? 8 : 7), sk = attn_slots(a.g.Nk, a.g.B, 7);
     if (a.g.Nq)
         hipLaunchKernelGGL((packed_attn_dq_kernel<T, DP, NW, TK, VEC>), dim3(sq * a.g.Hk), dim3(NW * 64), 0, a.stream, gq, a.q, a.k, a.v, a.o, a.go,
-                           a.lse, (T*)a.dq, a.delta, sq);
+                           a.lse, (T*)a.dq, a.rowstat, sq);
     if (a.g.Nk)
-        hipLaunchKernelGGL((packed_attn_dkv_kernel<T, DP, VEC>), dim3(sk * a.g.Hk), dim3(512), 0, a.stream, gk, a.q, a.k, a.v, a.go, a.lse,
-                           a.delta, (T*)a.dk, (T*)a.dv, sk);
+        hipLaunchKernelGGL((packed_attn_dkv_kernel<T, DP, VEC>), dim3(sk * a.g.Hk), dim3(512), 0, a.stream, gk, a.q, a.k, a.v, a.go,
+                           a.rowstat, (T*)a.dk, (T*)a.dv, sk);
 }
 template <typename T, int DP, int NW, int TK> void launch(const Bwd& a) {
     if (a.vec) launch_v<T, DP, NW, TK, true>(a);
@@ -328,20 +320,20 @@ template <typename T, int DP, int NW, int TK> void launch(const Bwd& a) {
 
 extern "C" int uncr_packed_attn_bwd(const void* q, long long q_ts, long long q_hs, const void* k, long long k_ts, long long k_hs, const void* v,
                                     long long v_ts, long long v_hs, const void* out, long long o_ts, long long o_hs, const void* dout,
-                                    long long do_ts, long long do_hs, const float* lse, void* dq, void* dk, void* dv, float* delta,
+                                    long long do_ts, long long do_hs, const float* lse, void* dq, void* dk, void* dv, float* rowstat,
                                     const int* off_q, const int* off_k, const int* k_len, float temperature, int causal, int B, int Nq, int Nk,
                                     int Hq, int Hk, int D, int act, hipStream_t stream) {
     Bwd a;
     const int rc = attn_geom(a.g, off_q, off_k, k_len, temperature, causal, B, Nq, Nk, Hq, Hk, D, act);
     if (rc != UNCR_OK) return rc;
-    if (Nq && (!q || !out || !dout || !lse || !dq || !delta)) return UNCR_EINVAL;
+    if (Nq && (!q || !out || !dout || !lse || !dq || !rowstat)) return UNCR_EINVAL;
     if (Nk && (!k || !v || !dk || !dv)) return UNCR_EINVAL;
     if ((D & 3) == 0) {         // the epilogue's 4-element stores
         const uintptr_t align = (act ? 2 : 4) * 4;
         if ((uintptr_t)dq % align || (uintptr_t)dk % align || (uintptr_t)dv % align) return UNCR_EINVAL;
     }
     a.q = {q, q_ts, q_hs}; a.k = {k, k_ts, k_hs}; a.v = {v, v_ts, v_hs}; a.o = {out, o_ts, o_hs}; a.go = {dout, do_ts, do_hs};
-    a.lse = lse; a.dq = dq; a.dk = dk; a.dv = dv; a.delta = delta; a.stream = stream;
+    a.lse = lse; a.dq = dq; a.dk = dk; a.dv = dv; a.rowstat = rowstat; a.stream = stream;
     const AttnTensor all[] = {a.q, a.k, a.v, a.o, a.go};
     a.vec = attn_aligned(all, 5, D, act);
     if (act) {

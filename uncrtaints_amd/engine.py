@@ -2268,10 +2268,10 @@ def packed_attention_backward(dout: Tensor, q: Tensor, k: Tensor, v: Tensor, out
     with _on(q.device):
         dq = torch.empty((Nq, Hq, D), device=q.device, dtype=q.dtype)
         dk, dv = torch.empty((Nk, Hk, D), device=q.device, dtype=q.dtype), torch.empty((Nk, Hk, D), device=q.device, dtype=q.dtype)
-        delta = _f32((Nq, Hq), q.device)
+        rowstat = _f32((2, Nq, Hq), q.device)
         hb.call("uncr_packed_attn_bwd", q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(),
                 v.stride(0), v.stride(1), out.data_ptr(), out.stride(0), out.stride(1), dout.data_ptr(), dout.stride(0), dout.stride(1),
-                lse, dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), delta, off_q, off_k, k_len, float(temperature), int(causal),
+                lse, dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), rowstat, off_q, off_k, k_len, float(temperature), int(causal),
                 off_q.numel() - 1, Nq, Nk, Hq, Hk, D, _dt(q), _stream())
     return dq, dk, dv
 
