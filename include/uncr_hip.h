@@ -595,18 +595,21 @@ int uncr_headnorm_rotary_bwd(const void* q, long long q_ts, long long q_hs, cons
  * is room in a cache.  off_q, off_k [B+1], k_len [B]: int32, device.  causal: row i of Lq sees keys j <= i + Lk - Lq.
  *   out = softmax(q k^T / temperature) v;  a row that sees nothing: 0.  lse [Nq][Hq] (nullable): log of the row's sum, -inf where it sees
  *   nothing.  Query rows of no sequence: zeros (lse -inf) with fill != 0, left as they are without.
- * Offsets are clamped into the tensors on the device.  Rows of no sequence and keys behind k_len are never multiplied. */
+ * Offsets are clamped into the tensors on the device.  Rows of no sequence and keys behind k_len are never multiplied.
+ * max_q, max_k: the longest sequences as far as the caller knows, 0 otherwise; they choose among kernels (few rows per sequence, short
+ * sequences) and never change what is computed.  work: float [work_floats] workspace of at least uncr_packed_attn_work(...) floats. */
+int uncr_packed_attn_work(int max_q, int max_k, int B, int Nq, int Nk, int Hq, int Hk, int D, int act);
 int uncr_packed_attn_fwd(const void* q, long long q_ts, long long q_hs, const void* k, long long k_ts, long long k_hs, const void* v,
                          long long v_ts, long long v_hs, void* out, long long o_ts, long long o_hs, float* lse, const int* off_q,
-                         const int* off_k, const int* k_len, float temperature, int causal, int fill, int B, int Nq, int Nk, int Hq, int Hk,
-                         int D, int act, hipStream_t stream);
+                         const int* off_k, const int* k_len, float temperature, int causal, int fill, int max_q, int max_k, float* work,
+                         long long work_floats, int B, int Nq, int Nk, int Hq, int Hk, int D, int act, hipStream_t stream);
 /* gradients dq, dk, dv (contiguous; zeros for rows of no sequence and keys behind k_len) from dout, the forward's inputs, out and lse;
  * rowstat: float [2][Nq][Hq] workspace */
 int uncr_packed_attn_bwd(const void* q, long long q_ts, long long q_hs, const void* k, long long k_ts, long long k_hs, const void* v,
                          long long v_ts, long long v_hs, const void* out, long long o_ts, long long o_hs, const void* dout, long long do_ts,
                          long long do_hs, const float* lse, void* dq, void* dk, void* dv, float* rowstat, const int* off_q, const int* off_k,
-                         const int* k_len, float temperature, int causal, int B, int Nq, int Nk, int Hq, int Hk, int D, int act,
-                         hipStream_t stream);
+                         const int* k_len, float temperature, int causal, int max_q, int max_k, int B, int Nq, int Nk, int Hq, int Hk, int D,
+                         int act, hipStream_t stream);
 
 #ifdef __cplusplus
 }

@@ -111,7 +111,7 @@ def _run(lq, lk, hq, hk, d, causal, dtype, room=None, front=0, behind=0, tempera
     temp = temperature if temperature is not None else math.sqrt(d)
     qd, kd, vd = (place(t).detach().requires_grad_(train) for t in (q, k, v))
     k_len = torch.tensor(lk, dtype=torch.int32, device=DEV) if room is not None else None
-    hint = dict(max_q=max(lq), max_k=max(lk)) if hints else {}
+    hint = {} if not hints else dict(max_q=max(lq), max_k=max(lk)) if hints is True else dict(max_q=hints[0], max_k=hints[1])
     out, lse = m(qd, kd, vd, off_q.to(DEV), off_k.to(DEV), k_len=k_len, return_lse=True, **hint)
     grads = torch.autograd.grad(out, (qd, kd, vd), place(do)) if train else ()
     want = {n: (torch.zeros(*sh, dtype=torch.float64), torch.zeros(*sh, dtype=torch.float64))
@@ -233,6 +233,26 @@ def test_single_tokens_over_a_cache(lens, hq, hk, d, dtype):
 
 @gpu
 @BOTH
+@pytest.mark.parametrize("hq,hk,d", [(8, 2, 128), (4, 4, 64), (2, 1, 16), (3, 3, 33)])
+def test_single_tokens_over_long_caches(hq, hk, d, dtype):
+    """Ranges of keys for blocks of their own, whose partial results are joined; sequences that end in the first range, or have no keys."""
+    _run([1] * 5, [9000, 31, 0, 4097, 1025], hq, hk, d, True, dtype, room=[9001, 40, 3, 4097, 1030], train=False, front=1, behind=4)
+    _run([3, 0, 2], [6000, 500, 2], hq, hk, d, True, dtype, room=[6000, 500, 8], train=False, hints=False)
+
+
+@gpu
+@MASK
+@BOTH
+@pytest.mark.parametrize("hq,hk,d", [(16, 16, 16), (4, 2, 32), (6, 1, 64), (2, 2, 5), (8, 4, 20)])
+def test_short_sequences(hq, hk, d, dtype, causal):
+    """A wave per sequence and key head, up to two tiles on either side."""
+    lengths = [30, 2, 0, 1, 8, 31, 32, 33, 10, 5]
+    _run(lengths, lengths, hq, hk, d, causal, dtype)
+    _run([5, 10, 0, 7, 3], [60, 4, 9, 0, 33], hq, hk, d, causal, dtype, room=[64, 6, 9, 3, 64], front=4, behind=9)
+
+
+@gpu
+@BOTH
 @pytest.mark.parametrize("lq", [[2, 3, 1], [1, 0, 9], [40, 1, 1]])
 @pytest.mark.parametrize("hints", [True, False])
 def test_a_few_tokens_over_a_cache(lq, hints, dtype):
@@ -241,14 +261,11 @@ def test_a_few_tokens_over_a_cache(lq, hints, dtype):
 
 @gpu
 @BOTH
-def test_hints_that_are_too_small_change_nothing(dtype):
-    from uncrtaints_amd.src.backbones.packed_attention import PackedAttention, pack_offsets
-    q, k, v = (torch.randn(300, n, 64, generator=_gen(n)).to(dtype).to(DEV) for n in (4, 2, 3))
-    v = v[:, :2]
-    off = pack_offsets([200, 100], DEV)
-    m = PackedAttention(causal=True)
-    a, b = m(q, k, v, off), m(q, k, v, off, max_q=1, max_k=1)
-    assert float((a.float() - b.float()).abs().max()) <= 4 * torch.finfo(dtype).eps * float(v.float().abs().max())
+@pytest.mark.parametrize("hints", [(1, 1), (1, 4000), (1, 0), (300, 1)])
+def test_wrong_hints_change_nothing(hints, dtype):
+    """Any kernel gives the right result for any lengths, forward and backward."""
+    _run([200, 100, 0, 33], [200, 100, 7, 500], 4, 2, 64, True, dtype, hints=hints)
+    _run([200, 70], [130, 90], 3, 3, 16, False, dtype, hints=hints)
 
 
 @gpu
@@ -446,14 +463,14 @@ def test_entry_points_refuse_bad_sizes():
     names = [n for _, n in hb.parse_header()["uncr_packed_attn_fwd"]]
     ok = dict.fromkeys(names, 0)
     ok.update(q=16, k=16, v=16, out=16, off_q=16, off_k=16, lse=None, k_len=None, temperature=1.0, B=1, Nq=0, Nk=4, Hq=4, Hk=2, D=8, stream=None)
-    if "work" in ok:
-        ok["work"] = None
+    ok["work"] = None
     call = lambda **kw: fwd(*{**ok, **kw}.values())
     assert call() == 0
     for kw in (dict(B=0), dict(Nq=-1), dict(Nk=-1), dict(Hq=3), dict(Hk=0), dict(D=0), dict(D=129), dict(act=2), dict(temperature=0.0), dict(temperature=math.nan),
                dict(off_q=None), dict(off_k=None), dict(Nq=1 << 30, Hq=8), dict(Nq=2, q=None), dict(Nq=2, out=None), dict(Nq=2, k=None),
-               dict(Nq=2, out=18)):
+               dict(Nq=2, out=18), dict(Nq=2, Nk=40000, max_q=1, max_k=20000), dict(Nq=2, Nk=40000, max_q=1, max_k=20000, work=16, work_floats=99)):
         assert call(**kw) < 0, kw
+    assert hb.query("uncr_packed_attn_work", 1, 20000, 1, 2, 40000, 4, 2, 8, 0) > 99 and hb.query("uncr_packed_attn_work", 1, 100, 1, 2, 200, 4, 2, 8, 0) == 0
     bwd = hb.lib().fn["uncr_packed_attn_bwd"]
     names = [n for _, n in hb.parse_header()["uncr_packed_attn_bwd"]]
     ok2 = dict.fromkeys(names, 0)

@@ -134,12 +134,13 @@ template <typename T, int DP> struct AttnTile {
     static constexpr int NCH = DP / EPC;                  // chunks per row
     static constexpr int RB = NCH * 16;                   // bytes per row
     static constexpr int KS = NCH / 2;                    // operand steps over DP: a step is one chunk of each lane half
-    static constexpr int DB = DP / 32;                    // 32-wide blocks of DP
+    static constexpr int DB = DP < 32 ? 1 : DP / 32;      // 32-wide blocks of DP (DP = 16: half a block, its other half repeats the first)
 
     static __device__ __forceinline__ int swizzle(int row) {
         if (NCH >= 16) return ((row & 3) << 2) | ((row >> 2) & 3);
         if (NCH == 8) return (((row >> 1) & 1) << 2) | ((row >> 2) & 3);
-        return (row >> 2) & 3;
+        if (NCH == 4) return (row >> 2) & 3;
+        return (row >> 3) & 1;
     }
     static __device__ __forceinline__ int place(int row, int chunk) { return row * RB + ((chunk ^ swizzle(row)) << 4); }
 
@@ -243,7 +244,7 @@ template <int DP> struct AttnCols<__bf16, DP> {
     __device__ __forceinline__ void fetch(const char* tile, int row0, int db, int lane) {
         typedef __attribute__((address_space(3))) s16x4 lds4;
         const int g = lane >> 4, l = lane & 15;
-        const int chunk = db * 4 + (g & 1) * 2 + ((l & 3) >> 1), low = (l & 1) * 8;
+        const int chunk = (db * 4 + (g & 1) * 2 + ((l & 3) >> 1)) & (L::NCH - 1), low = (l & 1) * 8;
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
             const int row = row0 + 16 * u + 4 * (g >> 1) + (l >> 2);
@@ -264,7 +265,7 @@ template <int DP> struct AttnCols<float, DP> {
         const int col = lane & 31, h = lane >> 5;
 #pragma unroll
         for (int i = 0; i < 16; ++i)
-            f[i] = *reinterpret_cast<const float*>(tile + L::place(row0 + 8 * (i / 4) + 4 * h + i % 4, db * 8 + (col >> 2)) + (col & 3) * 4);
+            f[i] = *reinterpret_cast<const float*>(tile + L::place(row0 + 8 * (i / 4) + 4 * h + i % 4, (db * 8 + (col >> 2)) & (L::NCH - 1)) + (col & 3) * 4);
     }
     __device__ __forceinline__ void mma(f32x16& acc, const AttnProb<float>& p) const {
 #pragma unroll
@@ -285,19 +286,25 @@ __device__ __forceinline__ void attn_dma4(void* lds, const void* src) {
 }
 __device__ __forceinline__ void attn_arrived() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
+// waits for all but the last N of a wave's own loads / for its own LDS accesses (a tile that only one wave uses needs no barrier)
+template <int N> __device__ __forceinline__ void attn_arrived_but() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
+__device__ __forceinline__ void attn_own_lds() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+
 static __device__ const f32x4 attn_zeros = {0.f, 0.f, 0.f, 0.f};      // what chunks behind D are loaded from
 
 // A block's share of a tile on its way from global memory to LDS while the previous tile is computed on: straight (VEC), or through registers,
 // element by element
+// (NT = 64: a wave's own tile)
 template <typename T, int DP, int ROWS, int NT, bool VEC> struct AttnStage {
     typedef AttnTile<T, DP> L;
     static constexpr int CNT = (ROWS * L::NCH + NT - 1) / NT;
     typename L::Frag f[VEC ? 1 : CNT];
+    static __device__ __forceinline__ int me() { return NT == 64 ? threadIdx.x & 63 : threadIdx.x; }
     static __device__ __forceinline__ bool idle(int c) { return (ROWS * L::NCH) % NT && c >= ROWS * L::NCH; }
     // the chunk of a row that belongs at place c of the tile
     static __device__ __forceinline__ int chunk(int c) { return (c % L::NCH) ^ L::swizzle(c / L::NCH); }
     __device__ __forceinline__ void begin(int i, char* tile, const T* row, int D) {
-        const int c = threadIdx.x + i * NT;
+        const int c = me() + i * NT;
         if (idle(c)) return;
         if (VEC) {
             const T* p = row + chunk(c) * L::EPC;
@@ -309,13 +316,21 @@ template <typename T, int DP, int ROWS, int NT, bool VEC> struct AttnStage {
     // rows row0 ..: those behind `last` repeat it (their products are masked)
     __device__ __forceinline__ void begin(char* tile, const T* base, long long ts, int row0, int last, int D) {
 #pragma unroll
-        for (int i = 0; i < CNT; ++i) begin(i, tile, base + (size_t)min(row0 + (int)(threadIdx.x + i * NT) / L::NCH, last) * ts, D);
+        for (int i = 0; i < CNT; ++i) begin(i, tile, base + (size_t)min(row0 + (me() + i * NT) / L::NCH, last) * ts, D);
+    }
+    // packed rows: token r / G, head r % G
+    __device__ __forceinline__ void begin_packed(char* tile, const T* base, long long ts, long long hs, int row0, int last, int G, int D) {
+#pragma unroll
+        for (int i = 0; i < CNT; ++i) {
+            const int r = min(row0 + (me() + i * NT) / L::NCH, last), t = r / G;
+            begin(i, tile, base + (size_t)t * ts + (size_t)(r - t * G) * hs, D);
+        }
     }
     __device__ __forceinline__ void finish(char* tile) const {
         if (VEC) return;
 #pragma unroll
         for (int i = 0; i < CNT; ++i) {
-            const int c = threadIdx.x + i * NT;
+            const int c = me() + i * NT;
             if (!idle(c)) *reinterpret_cast<typename L::Frag*>(tile + c * 16) = f[i];
         }
     }
@@ -379,7 +394,74 @@ template <typename T> __device__ __forceinline__ void attn_fill_outside(const in
     }
 }
 
+// The running softmax of a wave's 32 rows over tiles of 32 keys: m is a reference for the exponents (see packed_attn.hip)
+template <typename T, int DP> struct AttnRun {
+    typedef AttnTile<T, DP> L;
+    f32x16 acc[L::DB];
+    float m, l;
+    __device__ __forceinline__ void reset() {
+#pragma unroll
+        for (int db = 0; db < L::DB; ++db) acc[db] = (f32x16)(0.f);
+        m = -INFINITY;
+        l = 0.f;
+    }
+    __device__ __forceinline__ void move(float mx) {
+        if (__any(mx > m + 8.f)) {
+            const float mn = fmaxf(m, mx), f = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+            m = mn;
+            l *= f;
+#pragma unroll
+            for (int db = 0; db < L::DB; ++db)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) acc[db][i] *= f;
+        }
+    }
+    // keys j0 .. j0 + 31 of which those below `limit` are this lane's row's
+    __device__ __forceinline__ void tile(const char* tk, const char* tv, const AttnRows<T, DP>& q, float c, int j0, int limit, bool edge, int lane) {
+        const int col = lane & 31, h = lane >> 5;
+        AttnRows<T, DP> k;
+        k.fetch(tk, col, h);
+        attn_fence();
+        f32x16 s = attn_product(k, q);
+        if (edge) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+                if (j0 + 8 * (i / 4) + 4 * h + i % 4 >= limit) s[i] = -INFINITY;
+        }
+        float mx = s[0];
+#pragma unroll
+        for (int i = 1; i < 16; ++i) mx = fmaxf(mx, s[i]);
+        move(fmaxf(mx, attn_other_half(mx)) * c);
+        const float ref = m == -INFINITY ? 0.f : m;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], c, -ref));
+            l += s[i];
+        }
+        AttnProb<T> p;
+        p.set(s);
+#pragma unroll
+        for (int db = 0; db < L::DB; ++db) {
+            AttnCols<T, DP> v;
+            v.fetch(tv, 0, db, lane);
+            v.mma(acc[db], p);
+        }
+    }
+};
+__device__ __forceinline__ float attn_lse(float m, float l) {      // m in powers of two
+    return l > 0.f || l != l ? (m + __builtin_amdgcn_logf(l)) * 0.69314718055994531f : -INFINITY;
+}
+__device__ __forceinline__ float attn_inv(float l) { return l > 0.f || l != l ? 1.f / l : 0.f; }
+
 // host side (packed_attn.hip)
 int attn_geom(AttnGeom& g, const int* off_q, const int* off_k, const int* k_len, float temperature, int causal, int B, int Nq, int Nk, int Hq,
               int Hk, int D, int act);
 bool attn_aligned(const AttnTensor* t, int n, int D, int act);
+// packed_attn_rows.hip: kernels whose unit is a wave, for few rows per sequence
+struct AttnSplit { int waves, chunk, splits; };     // waves that share a task, keys per block, blocks per sequence (1: no partial results)
+AttnSplit attn_split(const AttnGeom& g, int max_q, int max_k, int act);
+bool attn_short(const AttnGeom& g, int max_q, int max_k);
+void attn_rows_fwd(const AttnGeom& g, const AttnSplit& s, const AttnTensor& q, const AttnTensor& k, const AttnTensor& v, void* out, long long o_ts,
+                   long long o_hs, float* lse, float* work, int act, bool vec, hipStream_t stream);
+void attn_short_bwd(const AttnGeom& g, const AttnTensor& q, const AttnTensor& k, const AttnTensor& v, const AttnTensor& o, const AttnTensor& go,
+                    const float* lse, void* dq, void* dk, void* dv, int act, bool vec, hipStream_t stream);

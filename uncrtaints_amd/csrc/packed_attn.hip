@@ -157,10 +157,19 @@ bool attn_aligned(const AttnTensor* t, int n, int D, int act) {
     return ok;
 }
 
+extern "C" int uncr_packed_attn_work(int max_q, int max_k, int B, int Nq, int Nk, int Hq, int Hk, int D, int act) {
+    AttnGeom g;
+    static const int none = 0;
+    if (attn_geom(g, &none, &none, nullptr, 1.f, 0, B, Nq, Nk, Hq, Hk, D, act) != UNCR_OK) return 0;
+    const AttnSplit s = attn_split(g, max_q, max_k, act);
+    return s.waves && s.splits > 1 ? (int)((long long)s.splits * Nq * Hq * (D + 2)) : 0;
+}
+
 extern "C" int uncr_packed_attn_fwd(const void* q, long long q_ts, long long q_hs, const void* k, long long k_ts, long long k_hs, const void* v,
                                     long long v_ts, long long v_hs, void* out, long long o_ts, long long o_hs, float* lse, const int* off_q,
-                                    const int* off_k, const int* k_len, float temperature, int causal, int fill, int B, int Nq, int Nk, int Hq,
-                                    int Hk, int D, int act, hipStream_t stream) {
+                                    const int* off_k, const int* k_len, float temperature, int causal, int fill, int max_q, int max_k,
+                                    float* work, long long work_floats, int B, int Nq, int Nk, int Hq, int Hk, int D, int act,
+                                    hipStream_t stream) {
     AttnGeom g;
     const int rc = attn_geom(g, off_q, off_k, k_len, temperature, causal, B, Nq, Nk, Hq, Hk, D, act);
     if (rc != UNCR_OK) return rc;
@@ -174,7 +183,11 @@ extern "C" int uncr_packed_attn_fwd(const void* q, long long q_ts, long long q_h
         const int size = (act ? 2 : 4) * 4;
         if ((uintptr_t)out % size || (o_ts * size / 4) % size || (o_hs * size / 4) % size) return UNCR_EINVAL;
     }
-    if (act) {
+    const AttnSplit split = attn_split(g, max_q, max_k, act);
+    if (split.waves) {
+        if (split.splits > 1 && (!work || work_floats < (long long)split.splits * Nq * Hq * (D + 2))) return UNCR_EINVAL;
+        attn_rows_fwd(g, split, tq, tk, tv, out, o_ts, o_hs, lse, work, act, vec, stream);
+    } else if (act) {
         if (D <= 32) launch<__bf16, 32, 4, 64>(g, tq, tk, tv, out, o_ts, o_hs, lse, vec, stream);
         else if (D <= 64) launch<__bf16, 64, 4, 64>(g, tq, tk, tv, out, o_ts, o_hs, lse, vec, stream);
         else launch<__bf16, 128, 8, 64>(g, tq, tk, tv, out, o_ts, o_hs, lse, vec, stream);

@@ -321,8 +321,8 @@ template <typename T, int DP, int NW, int TK> void launch(const Bwd& a) {
 extern "C" int uncr_packed_attn_bwd(const void* q, long long q_ts, long long q_hs, const void* k, long long k_ts, long long k_hs, const void* v,
                                     long long v_ts, long long v_hs, const void* out, long long o_ts, long long o_hs, const void* dout,
                                     long long do_ts, long long do_hs, const float* lse, void* dq, void* dk, void* dv, float* rowstat,
-                                    const int* off_q, const int* off_k, const int* k_len, float temperature, int causal, int B, int Nq, int Nk,
-                                    int Hq, int Hk, int D, int act, hipStream_t stream) {
+                                    const int* off_q, const int* off_k, const int* k_len, float temperature, int causal, int max_q,
+                                    int max_k, int B, int Nq, int Nk, int Hq, int Hk, int D, int act, hipStream_t stream) {
     Bwd a;
     const int rc = attn_geom(a.g, off_q, off_k, k_len, temperature, causal, B, Nq, Nk, Hq, Hk, D, act);
     if (rc != UNCR_OK) return rc;
@@ -336,7 +336,10 @@ extern "C" int uncr_packed_attn_bwd(const void* q, long long q_ts, long long q_h
     a.lse = lse; a.dq = dq; a.dk = dk; a.dv = dv; a.rowstat = rowstat; a.stream = stream;
     const AttnTensor all[] = {a.q, a.k, a.v, a.o, a.go};
     a.vec = attn_aligned(all, 5, D, act);
-    if (act) {
+    if (Nq == 0 && Nk == 0) return UNCR_OK;
+    if (attn_short(a.g, max_q, max_k)) {
+        attn_short_bwd(a.g, a.q, a.k, a.v, a.o, a.go, lse, dq, dk, dv, act, a.vec, stream);
+    } else if (act) {
         if (D <= 32) launch<__bf16, 32, 4, 64>(a);
         else if (D <= 64) launch<__bf16, 64, 4, 64>(a);
         else launch<__bf16, 128, 8, 64>(a);

@@ -1,0 +1,440 @@
+// Attention over packed token sequences where a sequence has few query rows (a token or a handful per series over a cache; the short series
+// of single pixels).  The unit is a WAVE with 32 rows (G heads of a group x tokens) and its own tiles of 32 keys in LDS, filled straight
+// from global memory while the previous tile is computed on; nothing waits for another wave on the way.
+//   cache:  bound by the read of keys and values.  `waves` waves of a block take every waves-th tile of a range of keys and join their sums
+//           in LDS; a long cache is cut into ranges of `chunk` keys for blocks of their own, whose unnormalised sums, maxima and sums of
+//           exponentials are joined by a second launch.
+//   short:  both sides are at most two tiles: each wave has a sequence and head of its own (a block of the kernels in packed_attn.hip
+//           would leave three of its four waves without rows), and the backward makes all three gradients in one pass over one tile.
+#include "packed_attn.h"
+
+namespace {
+
+template <typename T, int DP, int NW, bool SHARE, bool VEC>
+__global__ __launch_bounds__(NW * 64) void packed_attn_rows_kernel(const AttnGeom g, const AttnTensor q, const AttnTensor k, const AttnTensor v,
+                                                                   T* __restrict__ out, long long o_ts, long long o_hs, float* __restrict__ lse,
+                                                                   float* __restrict__ work, int chunk, int splits, int tasks) {
+    typedef AttnTile<T, DP> L;
+    typedef AttnStage<T, DP, 32, 64, VEC> Stage;
+    constexpr int NBUF = SHARE ? 2 : 1, TILE = 32 * L::RB;
+    __shared__ alignas(16) char lds[NW][NBUF][2][TILE];
+    __shared__ float lds_m[NW][32], lds_l[NW][32];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5, col = lane & 31;
+    if (g.fill) attn_fill_outside<T>(g.off_q, g.B, g.Nq, out, o_ts, o_hs, g.Hq, g.D, lse, blockIdx.x, gridDim.x);
+    const int task = SHARE ? blockIdx.x : blockIdx.x * NW + wave;
+    if (task >= tasks) return;
+    const int hk = task % g.Hk, split = SHARE ? task / g.Hk % splits : 0, slot = SHARE ? task / g.Hk / splits : task / g.Hk;
+    int b, part;
+    if (!attn_find(g.off_q, g.B, g.Nq, g.G, 5, slot, b, part)) return;
+    const AttnSeq s = attn_seq(g, b);
+    const int rows = s.lq * g.G, row0 = part * 32;
+    if (row0 >= rows) return;
+    const int row = min(row0 + col, rows - 1), tok = row / g.G, head = hk * g.G + row - tok * g.G;
+    const int shift = s.lk - s.lq;
+    auto limit_of = [&](int r) { return g.causal ? min(max(min(r, rows - 1) / g.G + shift + 1, 0), s.lk) : s.lk; };
+    const int limit = limit_of(row), lo = limit_of(row0), hi = limit_of(row0 + 31);
+    // this block's keys: ranges of `chunk`, longer ones if `splits` of those do not reach the end
+    const int range = SHARE ? max(chunk, ((s.lk + splits - 1) / splits + 31) & ~31) : s.lk;
+    const int begin = split * range, end = min(hi, begin + range);
+
+    AttnRows<T, DP> qf;
+    qf.template fetch_global<VEC>((const T*)q.p + (size_t)(s.q0 + tok) * q.ts + (size_t)head * q.hs, h, g.D);
+    AttnRun<T, DP> run;
+    run.reset();
+    const T* kb = (const T*)k.p + (size_t)s.k0 * k.ts + (size_t)hk * k.hs;
+    const T* vb = (const T*)v.p + (size_t)s.k0 * v.ts + (size_t)hk * v.hs;
+    Stage ks, vs;
+    constexpr int STEP = SHARE ? NW * 32 : 32;
+    int j0 = begin + (SHARE ? wave * 32 : 0), buf = 0;
+    if (j0 < end) {
+        ks.begin(lds[wave][0][0], kb, k.ts, j0, s.lk - 1, g.D);
+        vs.begin(lds[wave][0][1], vb, v.ts, j0, s.lk - 1, g.D);
+        ks.finish(lds[wave][0][0]);
+        vs.finish(lds[wave][0][1]);
+    }
+    for (; j0 < end; j0 += STEP) {
+        const bool more = j0 + STEP < end;
+        if (NBUF == 2 && more) {
+            attn_own_lds();
+            ks.begin(lds[wave][buf ^ 1][0], kb, k.ts, j0 + STEP, s.lk - 1, g.D);
+            vs.begin(lds[wave][buf ^ 1][1], vb, v.ts, j0 + STEP, s.lk - 1, g.D);
+            attn_arrived_but<VEC ? 2 * Stage::CNT : 0>();
+        } else {
+            attn_arrived();
+        }
+        attn_own_lds();
+        run.tile(lds[wave][buf][0], lds[wave][buf][1], qf, g.c, j0, limit, j0 + 32 > lo, lane);
+        if (more) {
+            attn_own_lds();
+            if (NBUF == 1) {
+                ks.begin(lds[wave][0][0], kb, k.ts, j0 + STEP, s.lk - 1, g.D);
+                vs.begin(lds[wave][0][1], vb, v.ts, j0 + STEP, s.lk - 1, g.D);
+            }
+            ks.finish(lds[wave][NBUF == 2 ? buf ^ 1 : 0][0]);
+            vs.finish(lds[wave][NBUF == 2 ? buf ^ 1 : 0][1]);
+        }
+        if (NBUF == 2) buf ^= 1;
+    }
+    float l = run.l + attn_other_half(run.l), m = run.m;
+    if (!SHARE) {
+        if (row0 + col >= rows) return;
+        attn_store_row<T, L::DB>(out + (size_t)(s.q0 + tok) * o_ts + (size_t)head * o_hs, run.acc, attn_inv(l), h, g.D);
+        if (lse && h == 0) lse[(size_t)(s.q0 + tok) * g.Hq + head] = attn_lse(m, l);
+        return;
+    }
+    // the waves' sums, brought to one reference and added in LDS: [wave][row][DP] over the tiles, which no wave needs any more
+    if (h == 0) {
+        lds_m[wave][col] = m;
+        lds_l[wave][col] = l;
+    }
+    __syncthreads();
+    float mm = -INFINITY, ll = 0.f;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) mm = fmaxf(mm, lds_m[w][col]);
+    const float ref = mm == -INFINITY ? 0.f : mm;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) ll += lds_l[w][col] * __builtin_amdgcn_exp2f(lds_m[w][col] - ref);
+    const float f = __builtin_amdgcn_exp2f(m - ref);
+    const int live = min(rows - row0, 32);
+    constexpr int WB = NBUF * 2 * TILE / 4, ROWS = WB / DP < 32 ? WB / DP : 32;       // floats of a wave's tiles; rows of DP they hold
+    float* mine = (float*)&lds[wave][0][0][0];
+    for (int r0 = 0; r0 < live; r0 += ROWS) {
+        if (r0) __syncthreads();
+        if (col >= r0 && col < r0 + ROWS && col < live) {
+#pragma unroll
+            for (int db = 0; db < L::DB; ++db)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int d = db * 32 + 8 * e + 4 * h;
+                    if (d < DP)
+                        *reinterpret_cast<f32x4*>(mine + (col - r0) * DP + d) =
+                            (f32x4){run.acc[db][4 * e] * f, run.acc[db][4 * e + 1] * f, run.acc[db][4 * e + 2] * f, run.acc[db][4 * e + 3] * f};
+                }
+        }
+        __syncthreads();
+        const int n = min(live - r0, ROWS);
+        for (int i = threadIdx.x; i < n * DP; i += NW * 64) {
+            const int r = i / DP, d = i % DP;
+            if (d >= g.D) continue;
+            float a = 0.f, lr = 0.f, mr = -INFINITY;
+#pragma unroll
+            for (int w = 0; w < NW; ++w) {
+                a += *((const float*)&lds[w][0][0][0] + i);
+                mr = fmaxf(mr, lds_m[w][r0 + r]);
+            }
+            const int rr = row0 + r0 + r, t = rr / g.G;
+            const size_t at = (size_t)(s.q0 + t) * g.Hq + hk * g.G + rr - t * g.G;
+            if (splits > 1) {
+                if (mr != -INFINITY) work[((size_t)split * g.Nq * g.Hq + at) * g.D + d] = a;
+            } else {
+                const float rf = mr == -INFINITY ? 0.f : mr;
+#pragma unroll
+                for (int w = 0; w < NW; ++w) lr += lds_l[w][r0 + r] * __builtin_amdgcn_exp2f(lds_m[w][r0 + r] - rf);
+                out[(size_t)(s.q0 + t) * o_ts + (size_t)(hk * g.G + rr - t * g.G) * o_hs + d] = (T)(a * attn_inv(lr));
+            }
+        }
+    }
+    if (wave == 0 && h == 0 && col < live) {
+        const size_t at = (size_t)(s.q0 + tok) * g.Hq + head;
+        if (splits > 1) {
+            float* ml = work + (size_t)splits * g.Nq * g.Hq * g.D + ((size_t)split * g.Nq * g.Hq + at) * 2;
+            ml[0] = mm;
+            ml[1] = ll;
+        } else if (lse) {
+            lse[at] = attn_lse(mm, ll);
+        }
+    }
+}
+
+// out = sum over the splits of exp2(m - max m) (their sums), over the same sum of their l: one wave per row
+template <typename T>
+__global__ __launch_bounds__(256) void packed_attn_join_kernel(const AttnGeom g, const float* __restrict__ work, int splits, T* __restrict__ out,
+                                                               long long o_ts, long long o_hs, float* __restrict__ lse) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const long long at = (long long)blockIdx.x * 4 + wave;
+    if (at >= (long long)g.Nq * g.Hq) return;
+    const int tok = (int)(at / g.Hq), head = (int)(at % g.Hq);
+    // is the row one of a sequence's?  (tokens are looked up as tiles of one row would be: slot = token + sequence)
+    int lo = 0, n = g.B;
+    while (n > 1) {
+        const int step = (n + 63) >> 6;
+        const bool in = lane * step < n && g.off_q[lo + lane * step] <= tok;
+        const int cnt = max(__popcll(__ballot(in)), 1);
+        lo += (cnt - 1) * step;
+        n = min(step, n - (cnt - 1) * step);
+    }
+    const AttnSeq s = attn_seq(g, lo);
+    if (tok < s.q0 || tok >= s.q0 + s.lq) return;
+    const size_t rows = (size_t)g.Nq * g.Hq;
+    const float* ml = work + (size_t)splits * rows * g.D;
+    const float m = lane < splits ? ml[((size_t)lane * rows + at) * 2] : -INFINITY;
+    float l = lane < splits ? ml[((size_t)lane * rows + at) * 2 + 1] : 0.f;
+    float mm = m;
+#pragma unroll
+    for (int d = 32; d; d >>= 1) mm = fmaxf(mm, __shfl_xor(mm, d));
+    const float f = mm == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mm);
+    l = m == -INFINITY ? 0.f : l * f;
+#pragma unroll
+    for (int d = 32; d; d >>= 1) l += __shfl_xor(l, d);
+    const float inv = attn_inv(l);
+    for (int d = lane; d < ((g.D + 63) & ~63); d += 64) {
+        float a = 0.f;
+        for (int i = 0; i < splits; ++i) {
+            const float fi = __shfl(f, i), mi = __shfl(m, i);
+            if (mi != -INFINITY && d < g.D) a = fmaf(work[((size_t)i * rows + at) * g.D + d], fi, a);
+        }
+        if (d < g.D) out[(size_t)tok * o_ts + (size_t)head * o_hs + d] = (T)(a * inv);
+    }
+    if (lse && lane == 0) lse[at] = attn_lse(mm, l);
+}
+
+// All gradients of short sequences, a wave per sequence and key head.  One tile of keys: P and dS are made once per tile of rows (columns:
+// rows), give dQ as they are, and cross a 32 x 32 patch of LDS to become columns of keys for dK and dV.  More keys than a tile (the caller
+// said otherwise): the same for every tile of keys, and dQ in a second round.
+template <typename T, int DP, int NW, bool VEC>
+__global__ __launch_bounds__(NW * 64) void packed_attn_short_bwd_kernel(const AttnGeom g, const AttnTensor q, const AttnTensor k, const AttnTensor v,
+                                                                        const AttnTensor o, const AttnTensor go, const float* __restrict__ lse,
+                                                                        T* __restrict__ dq, T* __restrict__ dk, T* __restrict__ dv) {
+    typedef AttnTile<T, DP> L;
+    typedef AttnStage<T, DP, 32, 64, VEC> Stage;
+    constexpr int TILE = 32 * L::RB, PS = 36;
+    __shared__ alignas(16) char lds[NW][4][TILE];
+    __shared__ alignas(16) float patch[NW][32 * PS];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5, col = lane & 31;
+    attn_fill_outside<T>(g.off_q, g.B, g.Nq, dq, (long long)g.Hq * g.D, g.D, g.Hq, g.D, nullptr, blockIdx.x, gridDim.x);
+    attn_fill_outside<T>(g.off_k, g.B, g.Nk, dk, (long long)g.Hk * g.D, g.D, g.Hk, g.D, nullptr, blockIdx.x, gridDim.x);
+    attn_fill_outside<T>(g.off_k, g.B, g.Nk, dv, (long long)g.Hk * g.D, g.D, g.Hk, g.D, nullptr, blockIdx.x, gridDim.x);
+    const int task = blockIdx.x * NW + wave, b = task / g.Hk, hk = task - b * g.Hk;
+    if (b >= g.B) return;
+    const AttnSeq s = attn_seq(g, b);
+    const int rows = s.lq * g.G, shift = s.lk - s.lq;
+    char *tk = lds[wave][0], *tv = lds[wave][1], *tq = lds[wave][2], *tg = lds[wave][3];
+    float* pt = patch[wave];
+    const T* kb = (const T*)k.p + (size_t)s.k0 * k.ts + (size_t)hk * k.hs;
+    const T* vb = (const T*)v.p + (size_t)s.k0 * v.ts + (size_t)hk * v.hs;
+    const T* qb = (const T*)q.p + (size_t)s.q0 * q.ts + (size_t)hk * g.G * q.hs;
+    const T* gb = (const T*)go.p + (size_t)s.q0 * go.ts + (size_t)hk * g.G * go.hs;
+    Stage s0, s1;
+    auto load_keys = [&](int j0) {
+        attn_own_lds();
+        s0.begin(tk, kb, k.ts, j0, s.lk - 1, g.D);
+        s1.begin(tv, vb, v.ts, j0, s.lk - 1, g.D);
+        s0.finish(tk);
+        s1.finish(tv);
+    };
+    float ls = INFINITY, dl = 0.f;
+    size_t at = 0;
+    auto load_rows = [&](int r0) {
+        attn_own_lds();
+        s0.begin_packed(tq, qb, q.ts, q.hs, r0, rows - 1, g.G, g.D);
+        s1.begin_packed(tg, gb, go.ts, go.hs, r0, rows - 1, g.G, g.D);
+        const int row = min(r0 + col, rows - 1), t = row / g.G, hd = hk * g.G + row - t * g.G;
+        at = (size_t)(s.q0 + t) * g.Hq + hd;
+        AttnRows<T, DP> of;
+        of.template fetch_global<VEC>((const T*)o.p + (size_t)(s.q0 + t) * o.ts + (size_t)hd * o.hs, h, g.D);
+        ls = lse[at] * 1.4426950408889634f;
+        if (ls == -INFINITY || r0 + col >= rows) ls = INFINITY;      // a row that saw nothing, a row behind the last: no probabilities
+        s0.finish(tq);
+        s1.finish(tg);
+        attn_arrived();
+        attn_own_lds();
+        AttnRows<T, DP> gf;
+        gf.fetch(tg, col, h);
+        dl = 0.f;
+#pragma unroll
+        for (int i = 0; i < L::KS; ++i)
+#pragma unroll
+            for (int e = 0; e < L::EPC; ++e) dl = fmaf((float)gf.f[i][e], (float)of.f[i][e], dl);
+        dl += attn_other_half(dl);
+    };
+    f32x16 p, ds;
+    auto scores = [&](int r0, int j0) {
+        AttnRows<T, DP> x, y;
+        x.fetch(tk, col, h);
+        y.fetch(tq, col, h);
+        p = attn_product(x, y);
+        x.fetch(tv, col, h);
+        y.fetch(tg, col, h);
+        ds = attn_product(x, y);
+        const int row = min(r0 + col, rows - 1), limit = g.causal ? min(row / g.G + shift + 1, s.lk) : s.lk;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const bool in = j0 + 8 * (i / 4) + 4 * h + i % 4 < limit && r0 + col < rows;
+            p[i] = in ? __builtin_amdgcn_exp2f(fmaf(p[i], g.c, -ls)) : 0.f;
+            ds[i] = in ? p[i] * (ds[i] - dl) : 0.f;
+        }
+    };
+    auto turn = [&](f32x16& x) {          // columns: rows -> columns: keys
+        attn_own_lds();
+#pragma unroll
+        for (int e = 0; e < 4; ++e) *reinterpret_cast<f32x4*>(pt + col * PS + 8 * e + 4 * h) = (f32x4){x[4 * e], x[4 * e + 1], x[4 * e + 2], x[4 * e + 3]};
+        attn_own_lds();
+#pragma unroll
+        for (int i = 0; i < 16; ++i) x[i] = pt[(8 * (i / 4) + 4 * h + i % 4) * PS + col];
+    };
+    auto add_dq = [&](f32x16 (&a)[L::DB]) {
+        AttnProb<T> w;
+        w.set(ds);
+#pragma unroll
+        for (int db = 0; db < L::DB; ++db) {
+            AttnCols<T, DP> x;
+            x.fetch(tk, 0, db, lane);
+            x.mma(a[db], w);
+        }
+    };
+    auto store_dq = [&](int r0, const f32x16 (&a)[L::DB]) {
+        if (r0 + col < rows) attn_store_row<T, L::DB>(dq + at * g.D, a, g.scale, h, g.D);
+    };
+    const bool single = s.lk <= 32;
+    for (int j0 = 0; j0 < s.room; j0 += 32) {
+        f32x16 ak[L::DB], av[L::DB];
+#pragma unroll
+        for (int db = 0; db < L::DB; ++db) ak[db] = av[db] = (f32x16)(0.f);
+        if (j0 < s.lk && rows) {
+            load_keys(j0);
+            for (int r0 = 0; r0 < rows; r0 += 32) {
+                load_rows(r0);
+                scores(r0, j0);
+                if (single) {
+                    f32x16 aq[L::DB];
+#pragma unroll
+                    for (int db = 0; db < L::DB; ++db) aq[db] = (f32x16)(0.f);
+                    add_dq(aq);
+                    store_dq(r0, aq);
+                }
+                AttnProb<T> w;
+                turn(p);
+                w.set(p);
+#pragma unroll
+                for (int db = 0; db < L::DB; ++db) {
+                    AttnCols<T, DP> x;
+                    x.fetch(tg, 0, db, lane);
+                    x.mma(av[db], w);
+                }
+                turn(ds);
+                w.set(ds);
+#pragma unroll
+                for (int db = 0; db < L::DB; ++db) {
+                    AttnCols<T, DP> x;
+                    x.fetch(tq, 0, db, lane);
+                    x.mma(ak[db], w);
+                }
+            }
+        }
+        if (j0 + col < s.room) {
+            if (j0 + col >= s.lk)
+#pragma unroll
+                for (int db = 0; db < L::DB; ++db) ak[db] = av[db] = (f32x16)(0.f);
+            const size_t ka = ((size_t)(s.k0 + j0 + col) * g.Hk + hk) * g.D;
+            attn_store_row<T, L::DB>(dk + ka, ak, g.scale, h, g.D);
+            attn_store_row<T, L::DB>(dv + ka, av, 1.f, h, g.D);
+        }
+    }
+    if (single && s.lk > 0) return;
+    for (int r0 = 0; r0 < rows; r0 += 32) {
+        f32x16 aq[L::DB];
+#pragma unroll
+        for (int db = 0; db < L::DB; ++db) aq[db] = (f32x16)(0.f);
+        load_rows(r0);
+        for (int j0 = 0; j0 < s.lk; j0 += 32) {
+            load_keys(j0);
+            attn_arrived();
+            attn_own_lds();
+            scores(r0, j0);
+            add_dq(aq);
+        }
+        store_dq(r0, aq);
+    }
+}
+
+struct Rows {
+    AttnGeom g;
+    AttnSplit s;
+    AttnTensor q, k, v;
+    void* out;
+    long long o_ts, o_hs;
+    float *lse, *work;
+    hipStream_t stream;
+};
+
+template <typename T, int DP, int NW, bool SHARE, bool VEC> void launch(const Rows& a) {
+    const int tasks = attn_slots((long long)a.g.Nq * a.g.G, a.g.B, 5) * a.g.Hk * (SHARE ? a.s.splits : 1);
+    hipLaunchKernelGGL((packed_attn_rows_kernel<T, DP, NW, SHARE, VEC>), dim3(SHARE ? tasks : (tasks + NW - 1) / NW), dim3(NW * 64), 0, a.stream, a.g, a.q,
+                       a.k, a.v, (T*)a.out, a.o_ts, a.o_hs, a.lse, a.work, a.s.chunk, a.s.splits, tasks);
+    if (SHARE && a.s.splits > 1)
+        hipLaunchKernelGGL((packed_attn_join_kernel<T>), dim3((unsigned)(((long long)a.g.Nq * a.g.Hq + 3) / 4)), dim3(256), 0, a.stream, a.g, a.work,
+                           a.s.splits, (T*)a.out, a.o_ts, a.o_hs, a.lse);
+}
+template <typename T, int DP, bool VEC> void launch_n(const Rows& a) {
+    constexpr int NW = DP * sizeof(T) <= 128 ? 8 : DP * sizeof(T) <= 256 ? 4 : 2;      // a wave's four tiles are 128 rows: 128 KB of LDS per block
+    if (DP == 128 || a.s.waves > 1) launch<T, DP, NW, true, VEC>(a);
+    else launch<T, DP < 128 ? DP : 64, 4, false, VEC>(a);             // attn_short: heads up to 64
+}
+template <typename T, bool VEC> void launch_d(const Rows& a) {
+    if (a.g.D <= 16) launch_n<T, 16, VEC>(a);
+    else if (a.g.D <= 32) launch_n<T, 32, VEC>(a);
+    else if (a.g.D <= 64) launch_n<T, 64, VEC>(a);
+    else launch_n<T, 128, VEC>(a);
+}
+
+struct Short {
+    AttnGeom g;
+    AttnTensor q, k, v, o, go;
+    const float* lse;
+    void *dq, *dk, *dv;
+    hipStream_t stream;
+};
+template <typename T, int DP, bool VEC> void launch_short(const Short& a) {
+    hipLaunchKernelGGL((packed_attn_short_bwd_kernel<T, DP, 4, VEC>), dim3((a.g.B * a.g.Hk + 3) / 4), dim3(256), 0, a.stream, a.g, a.q, a.k, a.v, a.o, a.go,
+                       a.lse, (T*)a.dq, (T*)a.dk, (T*)a.dv);
+}
+template <typename T, bool VEC> void launch_short_d(const Short& a) {
+    if (a.g.D <= 16) launch_short<T, 16, VEC>(a);
+    else if (a.g.D <= 32) launch_short<T, 32, VEC>(a);
+    else launch_short<T, 64, VEC>(a);
+}
+
+}  // namespace
+
+// Sequences of at most 64 rows and 64 keys by the caller's word (a wrong word costs time, not results), of heads up to 64
+bool attn_short(const AttnGeom& g, int max_q, int max_k) {
+    return max_q > 0 && max_k > 0 && (long long)max_q * g.G <= 64 && max_k <= 64 && g.D <= 64;
+}
+
+// Who shares a task.  Up to 32 rows per sequence (by the caller's word, else on average) are one wave's rows; more are better off in the
+// kernels of packed_attn.hip.  Without ranges (splits = 1) up to 8 tiles per wave; then ranges of 1024 keys, shorter ones while the launch
+// has fewer than two blocks per CU, down to a tile per wave.
+AttnSplit attn_split(const AttnGeom& g, int max_q, int max_k, int act) {
+    AttnSplit s = {0, 0, 1};
+    const long long rows = (long long)(max_q > 0 ? max_q : (g.Nq + g.B - 1) / g.B) * g.G;
+    const long long keys = max_k > 0 ? max_k : (g.Nk + g.B - 1) / g.B;
+    if (attn_short(g, max_q, max_k)) { s.waves = 1; return s; }
+    if (rows > 32) return s;
+    const int dp = g.D <= 16 ? 16 : g.D <= 32 ? 32 : g.D <= 64 ? 64 : 128, bytes = dp * (act ? 2 : 4);
+    s.waves = bytes <= 128 ? 8 : bytes <= 256 ? 4 : 2;
+    if (keys <= 32ll * 8 * s.waves) return s;
+    const long long tasks = attn_slots((long long)g.Nq * g.G, g.B, 5) * (long long)g.Hk;
+    int chunk = 1024;
+    while (chunk > 32 * s.waves && tasks * ((keys + chunk - 1) / chunk) < 512) chunk >>= 1;
+    long long n = (keys + chunk - 1) / chunk;
+    if (n > 64) n = 64;
+    // partial results of a launch are kept under 2^28 floats
+    while (n > 1 && (n * g.Nq * g.Hq * (g.D + 2) > (1ll << 28) || n * tasks > (1ll << 30))) n >>= 1;
+    s.chunk = (int)(((keys + n - 1) / n + 31) / 32 * 32);
+    s.splits = (int)n;
+    return s;
+}
+
+void attn_rows_fwd(const AttnGeom& g, const AttnSplit& s, const AttnTensor& q, const AttnTensor& k, const AttnTensor& v, void* out, long long o_ts,
+                   long long o_hs, float* lse, float* work, int act, bool vec, hipStream_t stream) {
+    const Rows a = {g, s, q, k, v, out, o_ts, o_hs, lse, work, stream};
+    if (act) vec ? launch_d<__bf16, true>(a) : launch_d<__bf16, false>(a);
+    else vec ? launch_d<float, true>(a) : launch_d<float, false>(a);
+}
+
+void attn_short_bwd(const AttnGeom& g, const AttnTensor& q, const AttnTensor& k, const AttnTensor& v, const AttnTensor& o, const AttnTensor& go,
+                    const float* lse, void* dq, void* dk, void* dv, int act, bool vec, hipStream_t stream) {
+    const Short a = {g, q, k, v, o, go, lse, dq, dk, dv, stream};
+    if (act) vec ? launch_short_d<__bf16, true>(a) : launch_short_d<__bf16, false>(a);
+    else vec ? launch_short_d<float, true>(a) : launch_short_d<float, false>(a);
+}

@@ -2243,7 +2243,7 @@ def headnorm_rotary_backward(gq: Tensor, gk: Tensor, q: Tensor, k: Tensor, wq: T
 
 
 def packed_attention_forward(q: Tensor, k: Tensor, v: Tensor, off_q: Tensor, off_k: Tensor, k_len: Optional[Tensor], temperature: float,
-                             causal: bool, want_lse: bool, out: Optional[Tensor] = None):
+                             causal: bool, want_lse: bool, out: Optional[Tensor] = None, max_q: int = 0, max_k: int = 0):
     """q [Nq, Hq, D], k / v [Nk, Hk, D] -> out [Nq, Hq, D] (rows of no sequence: zeros, or as they were in a given `out`), lse [Nq, Hq] or None"""
     q, k, v = _token_rows(q), _token_rows(k), _token_rows(v)
     Nq, Hq, D = q.shape
@@ -2253,14 +2253,17 @@ def packed_attention_forward(q: Tensor, k: Tensor, v: Tensor, off_q: Tensor, off
         if fill:
             out = torch.empty((Nq, Hq, D), device=q.device, dtype=q.dtype)
         lse = _f32((Nq, Hq), q.device) if want_lse else None
+        B = off_q.numel() - 1
+        n_work = hb.query("uncr_packed_attn_work", max_q, max_k, B, Nq, Nk, Hq, Hk, D, _dt(q))
+        work = _f32((n_work,), q.device) if n_work else None
         hb.call("uncr_packed_attn_fwd", q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(),
                 v.stride(0), v.stride(1), out.data_ptr(), out.stride(0), out.stride(1), lse, off_q, off_k, k_len, float(temperature),
-                int(causal), int(fill), off_q.numel() - 1, Nq, Nk, Hq, Hk, D, _dt(q), _stream())
+                int(causal), int(fill), max_q, max_k, work, n_work, B, Nq, Nk, Hq, Hk, D, _dt(q), _stream())
     return out, lse
 
 
 def packed_attention_backward(dout: Tensor, q: Tensor, k: Tensor, v: Tensor, out: Tensor, lse: Tensor, off_q: Tensor, off_k: Tensor,
-                              k_len: Optional[Tensor], temperature: float, causal: bool):
+                              k_len: Optional[Tensor], temperature: float, causal: bool, max_q: int = 0, max_k: int = 0):
     """-> dq [Nq, Hq, D], dk, dv [Nk, Hk, D] in the storage type"""
     q, k, v, dout = _token_rows(q), _token_rows(k), _token_rows(v), _token_rows(dout)
     Nq, Hq, D = q.shape
@@ -2272,7 +2275,7 @@ def packed_attention_backward(dout: Tensor, q: Tensor, k: Tensor, v: Tensor, out
         hb.call("uncr_packed_attn_bwd", q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(),
                 v.stride(0), v.stride(1), out.data_ptr(), out.stride(0), out.stride(1), dout.data_ptr(), dout.stride(0), dout.stride(1),
                 lse, dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), rowstat, off_q, off_k, k_len, float(temperature), int(causal),
-                off_q.numel() - 1, Nq, Nk, Hq, Hk, D, _dt(q), _stream())
+                max_q, max_k, off_q.numel() - 1, Nq, Nk, Hq, Hk, D, _dt(q), _stream())
     return dq, dk, dv
 
 

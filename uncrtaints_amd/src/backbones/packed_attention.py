@@ -67,10 +67,10 @@ class HeadNormRotary(nn.Module):
 
 class _PackedAttentionFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, v, off_q, off_k, k_len, temperature, causal):
-        out, lse = E.packed_attention_forward(q, k, v, off_q, off_k, k_len, temperature, causal, True)
+    def forward(ctx, q, k, v, off_q, off_k, k_len, temperature, causal, max_q, max_k):
+        out, lse = E.packed_attention_forward(q, k, v, off_q, off_k, k_len, temperature, causal, True, None, max_q, max_k)
         ctx.save_for_backward(q, k, v, out, lse, off_q, off_k, k_len)
-        ctx.temperature, ctx.causal = temperature, causal
+        ctx.args = temperature, causal, max_q, max_k
         ctx.mark_non_differentiable(lse)
         return out, lse
 
@@ -78,8 +78,8 @@ class _PackedAttentionFn(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, dout, _):
         q, k, v, out, lse, off_q, off_k, k_len = ctx.saved_tensors
-        grads = E.packed_attention_backward(dout, q, k, v, out, lse, off_q, off_k, k_len, ctx.temperature, ctx.causal)
-        return (*grads, None, None, None, None, None)
+        grads = E.packed_attention_backward(dout, q, k, v, out, lse, off_q, off_k, k_len, *ctx.args)
+        return (*grads, *(None,) * 7)
 
 
 def pack_offsets(lengths, device):
@@ -105,6 +105,8 @@ class PackedAttention(nn.Module):
       Without offsets_k the keys lie like the queries.  They are not read on the host; offsets outside the tensors are clamped on the device.
       k_len [B]: int32, used rows of each key sequence; the rest is room in a cache, never read into a result.
       A row that sees no key is 0 and takes no part in any gradient.  Rows of no sequence are zeros, in the gradients too.
+      max_q, max_k: the longest sequences as far as the program knows them; they choose among the kernels (few rows per sequence over a cache,
+      short sequences) and change nothing else: a wrong one costs time.
       out: written in place of a new tensor (only without gradients); rows of no sequence stay as they were.
       return_lse: also the logarithm of each row's sum of exponentials [Nq, heads], fp32, without a gradient; -inf where a row sees nothing.
 
@@ -130,6 +132,7 @@ class PackedAttention(nn.Module):
             if q.shape[0] != k.shape[0]:
                 raise ValueError(f"{q.shape[0]} query rows and {k.shape[0]} key rows need offsets_k")
             offsets_k = offsets_q
+            max_k = max_q if max_k is None else max_k
         for name, t in (("offsets_q", offsets_q), ("offsets_k", offsets_k), ("k_len", k_len)):
             if t is None:
                 continue
@@ -143,15 +146,16 @@ class PackedAttention(nn.Module):
                 raise ValueError(f"{name} {m}: must not be negative")
         E.check_tokens(q=q, k=k, v=v)
         E.check_device(q=q, offsets_q=offsets_q, offsets_k=offsets_k, k_len=k_len)
+        hints = int(max_q or 0), int(max_k or 0)
         temperature = math.sqrt(d) if self.temperature is None else float(self.temperature)
         if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
             if out is not None:
                 raise ValueError("out is for calls without gradients")
-            res, lse = _PackedAttentionFn.apply(q, k, v, offsets_q, offsets_k, k_len, temperature, self.causal)
+            res, lse = _PackedAttentionFn.apply(q, k, v, offsets_q, offsets_k, k_len, temperature, self.causal, *hints)
         else:
             if out is not None:
                 E.check_tokens(q=q, out=out)
                 if out.shape != q.shape or not out.is_contiguous():
                     raise ValueError(f"out {tuple(out.shape)}: a contiguous tensor of q's shape {tuple(q.shape)} is required")
-            res, lse = E.packed_attention_forward(q, k, v, offsets_q, offsets_k, k_len, temperature, self.causal, return_lse, out)
+            res, lse = E.packed_attention_forward(q, k, v, offsets_q, offsets_k, k_len, temperature, self.causal, return_lse, out, *hints)
         return (res, lse) if return_lse else res
