@@ -146,15 +146,29 @@ __global__ __launch_bounds__(NW * 64) void packed_attn_rows_kernel(const AttnGeo
     }
 }
 
-// out = sum over the splits of exp2(m - max m) (their sums), over the same sum of their l: one wave per row
+// out = sum over the splits of exp2(m - max m) (their sums), over the same sum of their l: one wave per row, the sums of 16 splits under way
+// at a time
 template <typename T>
 __global__ __launch_bounds__(256) void packed_attn_join_kernel(const AttnGeom g, const float* __restrict__ work, int splits, T* __restrict__ out,
                                                                long long o_ts, long long o_hs, float* __restrict__ lse) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const long long at = (long long)blockIdx.x * 4 + wave;
     if (at >= (long long)g.Nq * g.Hq) return;
+    const size_t rows = (size_t)g.Nq * g.Hq;
+    const float* ml = work + (size_t)splits * rows * g.D;
+    const float* row = work + at * g.D;
+    const float m = lane < splits ? ml[((size_t)lane * rows + at) * 2] : -INFINITY;
+    float l = lane < splits ? ml[((size_t)lane * rows + at) * 2 + 1] : 0.f;
+    float x[16][2];
+    auto fetch = [&](int i0) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) x[i][e] = i0 + i < splits && lane + 64 * e < g.D ? row[(size_t)(i0 + i) * rows * g.D + lane + 64 * e] : 0.f;
+    };
+    fetch(0);
+    // is the row one of a sequence's?
     const int tok = (int)(at / g.Hq), head = (int)(at % g.Hq);
-    // is the row one of a sequence's?  (tokens are looked up as tiles of one row would be: slot = token + sequence)
     int lo = 0, n = g.B;
     while (n > 1) {
         const int step = (n + 63) >> 6;
@@ -163,28 +177,30 @@ __global__ __launch_bounds__(256) void packed_attn_join_kernel(const AttnGeom g,
         lo += (cnt - 1) * step;
         n = min(step, n - (cnt - 1) * step);
     }
-    const AttnSeq s = attn_seq(g, lo);
-    if (tok < s.q0 || tok >= s.q0 + s.lq) return;
-    const size_t rows = (size_t)g.Nq * g.Hq;
-    const float* ml = work + (size_t)splits * rows * g.D;
-    const float m = lane < splits ? ml[((size_t)lane * rows + at) * 2] : -INFINITY;
-    float l = lane < splits ? ml[((size_t)lane * rows + at) * 2 + 1] : 0.f;
+    const int q0 = min(max(g.off_q[lo], 0), g.Nq);
+    if (tok < q0 || tok >= min(max(g.off_q[lo + 1], q0), g.Nq)) return;
     float mm = m;
 #pragma unroll
     for (int d = 32; d; d >>= 1) mm = fmaxf(mm, __shfl_xor(mm, d));
-    const float f = mm == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mm);
+    float f = mm == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mm);
+    if (m != m) f = m;                              // NaN sums stay NaN
     l = m == -INFINITY ? 0.f : l * f;
 #pragma unroll
     for (int d = 32; d; d >>= 1) l += __shfl_xor(l, d);
-    const float inv = attn_inv(l);
-    for (int d = lane; d < ((g.D + 63) & ~63); d += 64) {
-        float a = 0.f;
-        for (int i = 0; i < splits; ++i) {
-            const float fi = __shfl(f, i), mi = __shfl(m, i);
-            if (mi != -INFINITY && d < g.D) a = fmaf(work[((size_t)i * rows + at) * g.D + d], fi, a);
+    float a[2] = {0.f, 0.f};
+    for (int i0 = 0; i0 < splits; i0 += 16) {
+        if (i0) fetch(i0);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {              // a split without keys has left its row unwritten: f = 0
+            const float fi = i0 + i < splits ? __shfl(f, i0 + i) : 0.f;
+#pragma unroll
+            for (int e = 0; e < 2; ++e) a[e] += fi == 0.f ? 0.f : x[i][e] * fi;
         }
-        if (d < g.D) out[(size_t)tok * o_ts + (size_t)head * o_hs + d] = (T)(a * inv);
     }
+    const float inv = attn_inv(l);
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+        if (lane + 64 * e < g.D) out[(size_t)tok * o_ts + (size_t)head * o_hs + lane + 64 * e] = (T)(a[e] * inv);
     if (lse && lane == 0) lse[at] = attn_lse(mm, l);
 }
 
@@ -402,8 +418,8 @@ bool attn_short(const AttnGeom& g, int max_q, int max_k) {
 }
 
 // Who shares a task.  Up to 32 rows per sequence (by the caller's word, else on average) are one wave's rows; more are better off in the
-// kernels of packed_attn.hip.  Without ranges (splits = 1) up to 8 tiles per wave; then ranges of 1024 keys, shorter ones while the launch
-// has fewer than two blocks per CU, down to a tile per wave.
+// kernels of packed_attn.hip.  Without ranges (splits = 1) up to 8 tiles per wave; then ranges of 4096 keys, shorter ones while the launch
+// has fewer than eight blocks per CU (caches are filled to different lengths), down to a tile per wave.
 AttnSplit attn_split(const AttnGeom& g, int max_q, int max_k, int act) {
     AttnSplit s = {0, 0, 1};
     const long long rows = (long long)(max_q > 0 ? max_q : (g.Nq + g.B - 1) / g.B) * g.G;
@@ -414,8 +430,8 @@ AttnSplit attn_split(const AttnGeom& g, int max_q, int max_k, int act) {
     s.waves = bytes <= 128 ? 8 : bytes <= 256 ? 4 : 2;
     if (keys <= 32ll * 8 * s.waves) return s;
     const long long tasks = attn_slots((long long)g.Nq * g.G, g.B, 5) * (long long)g.Hk;
-    int chunk = 1024;
-    while (chunk > 32 * s.waves && tasks * ((keys + chunk - 1) / chunk) < 512) chunk >>= 1;
+    int chunk = 4096;
+    while (chunk > 32 * s.waves && tasks * ((keys + chunk - 1) / chunk) < 2048) chunk >>= 1;
     long long n = (keys + chunk - 1) / chunk;
     if (n > 64) n = 64;
     // partial results of a launch are kept under 2^28 floats

@@ -6,10 +6,10 @@
 //
 // Bound: memory.  The rotation reads and writes every element once (its gradient is the same kernel with the opposite angle); the norm's
 // gradient reads x and dy and recomputes r, so the forward keeps nothing for it.
-// Split: a block takes `tok` tokens.  Their (cos, sin) of every pair are computed ONCE, for all heads of queries and keys, into LDS -- the
-// angle in turns in 64 bits (fp32 loses the angle of a far position: 2^-24 * pos * freq radians), reduced, then sincospi in fp32.  A group
-// of `lpr` lanes then takes one token and every `strands`-th head: its pairs' (cos, sin) sit in registers, each head is C pairs per lane
-// loaded as up to 16-byte vectors.  At least four heads per group where there are that many, so the angles' cost is spread.
+// Split: a wave takes `tok` tokens and waits for no other.  Their (cos, sin) of every pair are computed ONCE, for all heads of queries and
+// keys, into LDS -- the angle in turns in 64 bits (fp32 loses the angle of a far position: 2^-24 * pos * freq radians), reduced, then sincospi
+// in fp32.  A group of `lpr` lanes then takes one token and every `strands`-th head: its pairs' (cos, sin) sit in registers, each head is C
+// pairs per lane loaded as up to 16-byte vectors.  At least four heads per group where there are that many, so the angles' cost is spread.
 #include "common.h"
 
 namespace {
@@ -23,12 +23,12 @@ struct RotGeom {
     const double* turns;     // [D / 2] turns per unit of position of every pair (0: the pair passes through)
     int pos_dt, n_axes;
     int sec0, sec1, sec2, sec3;      // elements per axis; the rest of D passes through
-    int neighbours;          // pairs (2i, 2i+1) of the head vector instead of (i, i + n/2) of the axis' section
+    int neighbours;          // pairs (2i, 2i+1) of the head vector instead of (i, i + n/2) of the axis' section: NB in the kernels
     float sgn;               // +1: rotate, -1: rotate back
     int N, D;
     int chunks;              // D / 2 / C: lanes' work items of one head
     int lpr;                 // lanes per head row (power of two)
-    int strands, tok;        // groups that share a token's heads; tokens per block
+    int strands, tok;        // groups of a wave that share a token's heads; tokens per wave
 };
 
 template <typename T> struct Elem;
@@ -55,10 +55,10 @@ template <typename T, int C> __device__ __forceinline__ void store(T* p, const f
     *reinterpret_cast<Pack<T, C>*>(p) = k;
 }
 
-// The C pairs of work item `j`: elements first[i] = o1 + i and second[i] = o2 + i (halves), or o1 + 2i, o1 + 2i + 1 (neighbours)
-__device__ __forceinline__ void place(const RotGeom& g, int j, int C, int& o1, int& o2) {
+// The C pairs of work item `j`: elements o1 + i and o2 + i (halves), or o1 + 2i, o1 + 2i + 1 (neighbours)
+template <int C, bool NB> __device__ __forceinline__ void place(const RotGeom& g, int j, int& o1, int& o2) {
     int p = j * C;
-    if (g.neighbours) { o1 = 2 * p; o2 = 2 * p + C; return; }
+    if (NB) { o1 = 2 * p; o2 = 0; return; }
     int start = 0, h = g.sec0 >> 1;
     if (p >= h) { p -= h; start += 2 * h; h = g.sec1 >> 1;
         if (p >= h) { p -= h; start += 2 * h; h = g.sec2 >> 1;
@@ -68,26 +68,33 @@ __device__ __forceinline__ void place(const RotGeom& g, int j, int C, int& o1, i
     o2 = o1 + h;
 }
 
-// a[i], b[i] = the pair's two components.  The vectors of a lane are [o1, o1 + C) and [o2, o2 + C): with neighbours they are one run
-template <typename T, int C> __device__ __forceinline__ void load_pairs(const T* row, int o1, int o2, bool nb, float* a, float* b) {
-    float x[C], y[C];
-    load<T, C>(row + o1, x);
-    load<T, C>(row + o2, y);
+template <typename T, int C, bool NB> __device__ __forceinline__ void load_pairs(const T* row, int o1, int o2, float* a, float* b) {
+    if (NB && C == 1) {
+        load<T, 1>(row + o1, a);
+        load<T, 1>(row + o1 + 1, b);
+    } else if (NB) {
+        float x[2 * C];
+        load<T, 2 * C>(row + o1, x);
 #pragma unroll
-    for (int i = 0; i < C; ++i) {
-        a[i] = nb ? (2 * i < C ? x[2 * i < C ? 2 * i : 0] : y[2 * i < C ? 0 : 2 * i - C]) : x[i];
-        b[i] = nb ? (2 * i + 1 < C ? x[2 * i + 1 < C ? 2 * i + 1 : 0] : y[2 * i + 1 < C ? 0 : 2 * i + 1 - C]) : y[i];
+        for (int i = 0; i < C; ++i) { a[i] = x[2 * i]; b[i] = x[2 * i + 1]; }
+    } else {
+        load<T, C>(row + o1, a);
+        load<T, C>(row + o2, b);
     }
 }
-template <typename T, int C> __device__ __forceinline__ void store_pairs(T* row, int o1, int o2, bool nb, const float* a, const float* b) {
-    float x[C], y[C];
+template <typename T, int C, bool NB> __device__ __forceinline__ void store_pairs(T* row, int o1, int o2, const float* a, const float* b) {
+    if (NB && C == 1) {
+        store<T, 1>(row + o1, a);
+        store<T, 1>(row + o1 + 1, b);
+    } else if (NB) {
+        float x[2 * C];
 #pragma unroll
-    for (int i = 0; i < C; ++i) {       // element i and C + i of the run, or of the two halves
-        x[i] = nb ? ((i & 1) ? b[i >> 1] : a[i >> 1]) : a[i];
-        y[i] = nb ? (((C + i) & 1) ? b[(C + i) >> 1] : a[(C + i) >> 1]) : b[i];
+        for (int i = 0; i < C; ++i) { x[2 * i] = a[i]; x[2 * i + 1] = b[i]; }
+        store<T, 2 * C>(row + o1, x);
+    } else {
+        store<T, C>(row + o1, a);
+        store<T, C>(row + o2, b);
     }
-    store<T, C>(row + o1, x);
-    store<T, C>(row + o2, y);
 }
 
 __device__ __forceinline__ double position(const RotGeom& g, int token, int axis) {
@@ -100,11 +107,11 @@ __device__ __forceinline__ double position(const RotGeom& g, int token, int axis
     }
 }
 
-// (cos, sin) of every pair of the block's tokens into cs[tok][D / 2]
+// (cos, sin) of every pair of the wave's tokens into its cs[tok][D / 2]
 __device__ __forceinline__ void angles(const RotGeom& g, int token0, float2* cs) {
     const int P = g.D >> 1;
     const int e0 = g.sec0 >> 1, e1 = e0 + (g.sec1 >> 1), e2 = e1 + (g.sec2 >> 1), e3 = e2 + (g.sec3 >> 1);
-    for (int i = threadIdx.x; i < g.tok * P; i += ROT_THREADS) {
+    for (int i = threadIdx.x & 63; i < g.tok * P; i += 64) {
         const int t = i / P, p = i - t * P;
         float2 v = make_float2(1.f, 0.f);
         if (token0 + t < g.N && p < e3) {
@@ -116,22 +123,23 @@ __device__ __forceinline__ void angles(const RotGeom& g, int token0, float2* cs)
         }
         cs[i] = v;
     }
+    __builtin_amdgcn_wave_barrier();      // LDS accesses of a wave are in order: nothing to wait for, only nothing to move across
 }
 
 struct HeadSet { const void* x; void* y; const float* w; long long ts, hs, yts, yhs; int H; };
 
 // One pass over queries (and keys): y = R(angle) x, or y = R(angle)(w * x * r).  K work items per lane: two only where C = 1 and D > 128
-template <typename T, int C, int K, bool NORM>
+template <typename T, int C, int K, bool NB, bool NORM>
 __global__ __launch_bounds__(ROT_THREADS) void rotary_kernel(const RotGeom g, const HeadSet q, const HeadSet k, float eps) {
-    extern __shared__ float2 cs[];
-    const int token0 = blockIdx.x * g.tok;
+    extern __shared__ float2 shared_cs[];
+    const int wave = threadIdx.x >> 6;
+    float2* cs = shared_cs + wave * g.tok * (g.D >> 1);
+    const int token0 = (blockIdx.x * (ROT_THREADS / 64) + wave) * g.tok;
     angles(g, token0, cs);
-    __syncthreads();
-    const int lane = threadIdx.x & (g.lpr - 1), group = threadIdx.x / g.lpr;
+    const int lane = threadIdx.x & (g.lpr - 1), group = (threadIdx.x & 63) / g.lpr;
     const int t = group / g.strands, strand = group - t * g.strands;
     const int token = token0 + t;
     const bool live = t < g.tok && token < g.N;
-    const bool nb = g.neighbours != 0;
     int o1[K], o2[K];
     bool on[K];
     float c[K][C], s[K][C];
@@ -139,7 +147,7 @@ __global__ __launch_bounds__(ROT_THREADS) void rotary_kernel(const RotGeom g, co
     for (int m = 0; m < K; ++m) {
         const int j = lane + m * g.lpr;
         on[m] = live && j < g.chunks;
-        place(g, on[m] ? j : 0, C, o1[m], o2[m]);
+        place<C, NB>(g, on[m] ? j : 0, o1[m], o2[m]);
 #pragma unroll
         for (int i = 0; i < C; ++i) {
             const float2 v = on[m] ? cs[t * (g.D >> 1) + j * C + i] : make_float2(1.f, 0.f);
@@ -147,45 +155,52 @@ __global__ __launch_bounds__(ROT_THREADS) void rotary_kernel(const RotGeom g, co
             s[m][i] = v.y;
         }
     }
-    for (int h = strand; h < q.H + k.H; h += g.strands) {
-        const HeadSet& z = h < q.H ? q : k;
-        const int hh = h < q.H ? h : h - q.H;
-        const T* x = (const T*)z.x + (size_t)token * z.ts + (size_t)hh * z.hs;
-        T* y = (T*)z.y + (size_t)token * z.yts + (size_t)hh * z.yhs;
-        float a[K][C], b[K][C];
 #pragma unroll
-        for (int m = 0; m < K; ++m) {
-            if (on[m]) load_pairs<T, C>(x, o1[m], o2[m], nb, a[m], b[m]);
-            else
-#pragma unroll
-                for (int i = 0; i < C; ++i) a[m][i] = b[m][i] = 0.f;
-        }
+    for (int which = 0; which < (NORM ? 2 : 1); ++which) {
+        const HeadSet& z = which ? k : q;
+        // heads of queries and keys are dealt to the strands as one list
+        int h = strand;
+        if (which) { const int past = q.H % g.strands; h = strand >= past ? strand - past : strand - past + g.strands; }
+        float wa[K][C], wb[K][C];
         if (NORM) {
-            float ss = 0.f;
 #pragma unroll
-            for (int m = 0; m < K; ++m)
-#pragma unroll
-                for (int i = 0; i < C; ++i) ss = fmaf(a[m][i], a[m][i], fmaf(b[m][i], b[m][i], ss));
-            for (int d = g.lpr >> 1; d; d >>= 1) ss += __shfl_xor(ss, d);
-            const float r = rsqrtf(ss / (float)g.D + eps);
+            for (int m = 0; m < K; ++m) load_pairs<float, C, NB>(z.w, o1[m], o2[m], wa[m], wb[m]);
+        }
+        for (; h < z.H; h += g.strands) {
+            const T* x = (const T*)z.x + (size_t)token * z.ts + (size_t)h * z.hs;
+            T* y = (T*)z.y + (size_t)token * z.yts + (size_t)h * z.yhs;
+            float a[K][C], b[K][C];
 #pragma unroll
             for (int m = 0; m < K; ++m) {
-                float wa[C], wb[C];
-                load_pairs<float, C>(z.w, o1[m], o2[m], nb, wa, wb);
+                if (on[m]) load_pairs<T, C, NB>(x, o1[m], o2[m], a[m], b[m]);
+                else
 #pragma unroll
-                for (int i = 0; i < C; ++i) { a[m][i] *= r * wa[i]; b[m][i] *= r * wb[i]; }
+                    for (int i = 0; i < C; ++i) a[m][i] = b[m][i] = 0.f;
             }
-        }
+            if (NORM) {
+                float ss = 0.f;
 #pragma unroll
-        for (int m = 0; m < K; ++m) {
-            if (!on[m]) continue;
-            float u[C], v[C];
+                for (int m = 0; m < K; ++m)
 #pragma unroll
-            for (int i = 0; i < C; ++i) {
-                u[i] = fmaf(a[m][i], c[m][i], -(b[m][i] * s[m][i]));
-                v[i] = fmaf(a[m][i], s[m][i], b[m][i] * c[m][i]);
+                    for (int i = 0; i < C; ++i) ss = fmaf(a[m][i], a[m][i], fmaf(b[m][i], b[m][i], ss));
+                for (int d = g.lpr >> 1; d; d >>= 1) ss += __shfl_xor(ss, d);
+                const float r = rsqrtf(ss / (float)g.D + eps);
+#pragma unroll
+                for (int m = 0; m < K; ++m)
+#pragma unroll
+                    for (int i = 0; i < C; ++i) { a[m][i] *= r * wa[m][i]; b[m][i] *= r * wb[m][i]; }
             }
-            store_pairs<T, C>(y, o1[m], o2[m], nb, u, v);
+#pragma unroll
+            for (int m = 0; m < K; ++m) {
+                if (!on[m]) continue;
+                float u[C], v[C];
+#pragma unroll
+                for (int i = 0; i < C; ++i) {
+                    u[i] = fmaf(a[m][i], c[m][i], -(b[m][i] * s[m][i]));
+                    v[i] = fmaf(a[m][i], s[m][i], b[m][i] * c[m][i]);
+                }
+                store_pairs<T, C, NB>(y, o1[m], o2[m], u, v);
+            }
         }
     }
 }
@@ -194,29 +209,29 @@ struct GradSet { const void* x; const void* dy; void* dx; const float* w; long l
 
 // The norm's gradient.  A block walks over token tiles (at most ROT_MAX_SLOTS blocks), dw of queries and keys in registers, and leaves
 // one row of partials: their sum in the next launch is in a fixed order, no atomics
-template <typename T, int C, int K>
+template <typename T, int C, int K, bool NB>
 __global__ __launch_bounds__(ROT_THREADS) void headnorm_bwd_kernel(const RotGeom g, const GradSet q, const GradSet k, float eps,
                                                                    float* __restrict__ part) {
-    extern __shared__ float2 cs[];
+    extern __shared__ float2 shared_cs[];
     __shared__ alignas(16) float red[ROT_THREADS / 64][2][ROT_MAX_D];
-    const int lane = threadIdx.x & (g.lpr - 1), group = threadIdx.x / g.lpr;
+    const int wave = threadIdx.x >> 6;
+    float2* cs = shared_cs + wave * g.tok * (g.D >> 1);
+    const int lane = threadIdx.x & (g.lpr - 1), group = (threadIdx.x & 63) / g.lpr;
     const int t = group / g.strands, strand = group - t * g.strands;
-    const bool nb = g.neighbours != 0;
     int o1[K], o2[K];
     float dwa[2][K][C], dwb[2][K][C];
 #pragma unroll
     for (int m = 0; m < K; ++m) {
         const int j = lane + m * g.lpr;
-        place(g, j < g.chunks ? j : 0, C, o1[m], o2[m]);
+        place<C, NB>(g, j < g.chunks ? j : 0, o1[m], o2[m]);
 #pragma unroll
         for (int i = 0; i < C; ++i) dwa[0][m][i] = dwb[0][m][i] = dwa[1][m][i] = dwb[1][m][i] = 0.f;
     }
     const int tiles = (g.N + g.tok - 1) / g.tok;
-    for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
+    for (int tile = blockIdx.x * (ROT_THREADS / 64) + wave; tile < tiles; tile += gridDim.x * (ROT_THREADS / 64)) {
         const int token0 = tile * g.tok, token = token0 + t;
-        __syncthreads();
+        __builtin_amdgcn_wave_barrier();
         angles(g, token0, cs);
-        __syncthreads();
         const bool live = t < g.tok && token < g.N;
         bool on[K];
         float c[K][C], s[K][C];
@@ -237,6 +252,9 @@ __global__ __launch_bounds__(ROT_THREADS) void headnorm_bwd_kernel(const RotGeom
             // heads of queries and keys are dealt to the strands as one list
             int h = strand;
             if (which) { const int past = q.H % g.strands; h = strand >= past ? strand - past : strand - past + g.strands; }
+            float wa[K][C], wb[K][C];
+#pragma unroll
+            for (int m = 0; m < K; ++m) load_pairs<float, C, NB>(z.w, o1[m], o2[m], wa[m], wb[m]);
             for (; h < z.H; h += g.strands) {
                 const T* x = (const T*)z.x + (size_t)token * z.ts + (size_t)h * z.hs;
                 const T* dy = (const T*)z.dy + (size_t)token * z.gts + (size_t)h * z.ghs;
@@ -245,22 +263,21 @@ __global__ __launch_bounds__(ROT_THREADS) void headnorm_bwd_kernel(const RotGeom
                 float ss = 0.f, dot = 0.f;
 #pragma unroll
                 for (int m = 0; m < K; ++m) {
-                    float ga[C], gb[C], wa[C], wb[C];
+                    float ga[C], gb[C];
                     if (on[m]) {
-                        load_pairs<T, C>(x, o1[m], o2[m], nb, a[m], b[m]);
-                        load_pairs<T, C>(dy, o1[m], o2[m], nb, ga, gb);
+                        load_pairs<T, C, NB>(x, o1[m], o2[m], a[m], b[m]);
+                        load_pairs<T, C, NB>(dy, o1[m], o2[m], ga, gb);
                     } else {
 #pragma unroll
                         for (int i = 0; i < C; ++i) a[m][i] = b[m][i] = ga[i] = gb[i] = 0.f;
                     }
-                    load_pairs<float, C>(z.w, o1[m], o2[m], nb, wa, wb);
 #pragma unroll
                     for (int i = 0; i < C; ++i) {
                         const float x0 = a[m][i], x1 = b[m][i];
                         const float u0 = fmaf(ga[i], c[m][i], -(gb[i] * s[m][i])), u1 = fmaf(ga[i], s[m][i], gb[i] * c[m][i]);
                         ss = fmaf(x0, x0, fmaf(x1, x1, ss));
-                        ua[m][i] = u0 * wa[i];
-                        ub[m][i] = u1 * wb[i];
+                        ua[m][i] = u0 * wa[m][i];
+                        ub[m][i] = u1 * wb[m][i];
                         dot = fmaf(ua[m][i], x0, fmaf(ub[m][i], x1, dot));
                         ga[i] = u0 * x0;       // dw terms, still without r
                         gb[i] = u1 * x1;
@@ -283,11 +300,11 @@ __global__ __launch_bounds__(ROT_THREADS) void headnorm_bwd_kernel(const RotGeom
                 for (int m = 0; m < K; ++m) {
                     if (!on[m]) continue;
                     if (K > 1) {
-                        float wa[C], wb[C];
-                        load_pairs<T, C>(dy, o1[m], o2[m], nb, wa, wb);
+                        float ga[C], gb[C];
+                        load_pairs<T, C, NB>(dy, o1[m], o2[m], ga, gb);
 #pragma unroll
                         for (int i = 0; i < C; ++i) {
-                            const float u0 = fmaf(wa[i], c[m][i], -(wb[i] * s[m][i])), u1 = fmaf(wa[i], s[m][i], wb[i] * c[m][i]);
+                            const float u0 = fmaf(ga[i], c[m][i], -(gb[i] * s[m][i])), u1 = fmaf(ga[i], s[m][i], gb[i] * c[m][i]);
                             dwa[which][m][i] = fmaf(u0 * a[m][i], r, dwa[which][m][i]);
                             dwb[which][m][i] = fmaf(u1 * b[m][i], r, dwb[which][m][i]);
                         }
@@ -297,13 +314,12 @@ __global__ __launch_bounds__(ROT_THREADS) void headnorm_bwd_kernel(const RotGeom
                         ua[m][i] = fmaf(r, ua[m][i], -(f * a[m][i]));
                         ub[m][i] = fmaf(r, ub[m][i], -(f * b[m][i]));
                     }
-                    store_pairs<T, C>(dx, o1[m], o2[m], nb, ua[m], ub[m]);
+                    store_pairs<T, C, NB>(dx, o1[m], o2[m], ua[m], ub[m]);
                 }
             }
         }
     }
     // dw of the block: over the groups of a wave by shuffles, over the waves through LDS
-    const int wave = threadIdx.x >> 6;
 #pragma unroll
     for (int which = 0; which < 2; ++which)
 #pragma unroll
@@ -316,7 +332,7 @@ __global__ __launch_bounds__(ROT_THREADS) void headnorm_bwd_kernel(const RotGeom
                 }
             const int j = lane + m * g.lpr;
             if ((threadIdx.x & 63) < g.lpr && j < g.chunks)
-                store_pairs<float, C>(&red[wave][which][0], o1[m], o2[m], nb, dwa[which][m], dwb[which][m]);
+                store_pairs<float, C, NB>(&red[wave][which][0], o1[m], o2[m], dwa[which][m], dwb[which][m]);
         }
     __syncthreads();
     for (int i = threadIdx.x; i < 2 * g.D; i += ROT_THREADS) {
@@ -327,45 +343,48 @@ __global__ __launch_bounds__(ROT_THREADS) void headnorm_bwd_kernel(const RotGeom
     }
 }
 
-// dw[i] = sum over the partials' rows, in 64 bits and a fixed order: 16 columns x 16 row strands per block
-__global__ __launch_bounds__(256) void headnorm_dw_kernel(const float* __restrict__ part, int rows, int n, float* __restrict__ dwq,
-                                                          float* __restrict__ dwk) {
-    __shared__ double acc[16][17];
-    const int c = blockIdx.x * 16 + (threadIdx.x & 15), s = threadIdx.x >> 4;
+// dw[i] = sum over the partials' rows, in 64 bits and a fixed order: 16 columns x 64 row strands per block
+__global__ __launch_bounds__(1024) void headnorm_dw_kernel(const float* __restrict__ part, int rows, int n, float* __restrict__ dwq,
+                                                           float* __restrict__ dwk) {
+    __shared__ double acc[64][17];
+    const int x = threadIdx.x & 15, c = blockIdx.x * 16 + x, s = threadIdx.x >> 4;
     double v = 0.0;
     if (c < 2 * n)
-        for (int r = s; r < rows; r += 16) v += (double)part[(size_t)r * 2 * n + c];
-    acc[s][threadIdx.x & 15] = v;
+#pragma unroll 8
+        for (int r = s; r < rows; r += 64) v += (double)part[(size_t)r * 2 * n + c];
+    acc[s][x] = v;
     __syncthreads();
-    if (s == 0 && c < 2 * n) {
-        for (int i = 1; i < 16; ++i) v += acc[i][threadIdx.x & 15];
-        (c < n ? dwq[c] : dwk[c - n]) = (float)v;
+    for (int h = 32; h; h >>= 1) {
+        if (s < h) acc[s][x] += acc[s + h][x];
+        __syncthreads();
     }
+    if (s == 0 && c < 2 * n) (c < n ? dwq[c] : dwk[c - n]) = (float)acc[0][x];
 }
 
-// Pairs per lane: the widest of 8, 4, 2, 1 that no axis' half section cuts and that every row starts aligned for
+// Pairs per lane: as many as one 16-byte vector holds of one component (halves) or of whole pairs (neighbours), fewer where an axis' half
+// section would be cut or a row does not start aligned for it
 int pick_c(const RotGeom& g, const long long* strides, int n_strides, const void* const* ptrs, int n_ptrs, int size, const float* wq = nullptr,
            const float* wk = nullptr) {
     const int halves[5] = {g.sec0 / 2, g.sec1 / 2, g.sec2 / 2, g.sec3 / 2, (g.D - g.sec0 - g.sec1 - g.sec2 - g.sec3) / 2};
-    for (int c = 8; c > 1; c >>= 1) {
-        const int align = c * size < 16 ? c * size : 16;
+    for (int c = (g.neighbours ? 8 : 16) / size; c > 1; c >>= 1) {
+        const int align = c * size * (g.neighbours ? 2 : 1);
         bool ok = (g.D / 2) % c == 0;
         if (!g.neighbours)
             for (int h : halves) ok = ok && h % c == 0;
         for (int i = 0; i < n_strides; ++i) ok = ok && (strides[i] * size) % align == 0;
         for (int i = 0; i < n_ptrs; ++i) ok = ok && ((uintptr_t)ptrs[i] % align) == 0;
-        ok = ok && (((uintptr_t)wq | (uintptr_t)wk) % (c * 4 < 16 ? c * 4 : 16)) == 0;
+        ok = ok && (((uintptr_t)wq | (uintptr_t)wk) % (align * 4 / size < 16 ? align * 4 / size : 16)) == 0;
         if (ok) return c;
     }
-    return 1;
+    return 1;          // one element at a time
 }
 
-// lanes per row, groups, tokens per block for C pairs per lane and `heads` heads
+// lanes per row, groups, tokens per wave for C pairs per lane and `heads` heads
 int shape(RotGeom& g, int c, int heads) {
     g.chunks = g.D / 2 / c;
     g.lpr = 1;
     while (g.lpr < g.chunks && g.lpr < 64) g.lpr <<= 1;
-    const int groups = ROT_THREADS / g.lpr;
+    const int groups = 64 / g.lpr;
     g.strands = 1;
     while (g.strands < groups && g.strands * 8 <= heads) g.strands <<= 1;
     g.tok = groups / g.strands;
@@ -391,35 +410,30 @@ int geom(RotGeom& g, const void* pos, int pos_dt, int n_axes, int s0, int s1, in
     return UNCR_OK;
 }
 
-template <typename T, int C, bool NORM>
-void launch_fwd(const RotGeom& g, const HeadSet& q, const HeadSet& k, float eps, int items, hipStream_t stream) {
-    const dim3 grid((g.N + g.tok - 1) / g.tok);
-    const size_t lds = (size_t)g.tok * (g.D / 2) * sizeof(float2);
-    if (C == 1 && items > 1) hipLaunchKernelGGL((rotary_kernel<T, C, C == 1 ? 2 : 1, NORM>), grid, dim3(ROT_THREADS), lds, stream, g, q, k, eps);
-    else hipLaunchKernelGGL((rotary_kernel<T, C, 1, NORM>), grid, dim3(ROT_THREADS), lds, stream, g, q, k, eps);
-}
+struct Fwd { RotGeom g; HeadSet q, k; float eps; int items; hipStream_t stream; };
+struct Bwd { RotGeom g; GradSet q, k; float eps; int items, blocks; float* part; hipStream_t stream; };
 
-template <typename T, bool NORM>
-void launch_fwd_c(const RotGeom& g, const HeadSet& q, const HeadSet& k, float eps, int c, int items, hipStream_t stream) {
-    if (c == 8) launch_fwd<T, 8, NORM>(g, q, k, eps, items, stream);
-    else if (c == 4) launch_fwd<T, 4, NORM>(g, q, k, eps, items, stream);
-    else if (c == 2) launch_fwd<T, 2, NORM>(g, q, k, eps, items, stream);
-    else launch_fwd<T, 1, NORM>(g, q, k, eps, items, stream);
-}
+size_t lds_bytes(const RotGeom& g) { return (size_t)(ROT_THREADS / 64) * g.tok * (g.D / 2) * sizeof(float2); }
 
-template <typename T, int C>
-void launch_bwd(const RotGeom& g, const GradSet& q, const GradSet& k, float eps, float* part, int blocks, int items, hipStream_t stream) {
-    const size_t lds = (size_t)g.tok * (g.D / 2) * sizeof(float2);
-    if (C == 1 && items > 1) hipLaunchKernelGGL((headnorm_bwd_kernel<T, C, C == 1 ? 2 : 1>), dim3(blocks), dim3(ROT_THREADS), lds, stream, g, q, k, eps, part);
-    else hipLaunchKernelGGL((headnorm_bwd_kernel<T, C, 1>), dim3(blocks), dim3(ROT_THREADS), lds, stream, g, q, k, eps, part);
+template <typename T, bool NB, bool NORM, int C, int K> void run(const Fwd& f) {
+    const int per = f.g.tok * (ROT_THREADS / 64);
+    hipLaunchKernelGGL((rotary_kernel<T, C, K, NB, NORM>), dim3((f.g.N + per - 1) / per), dim3(ROT_THREADS), lds_bytes(f.g), f.stream, f.g, f.q, f.k, f.eps);
 }
-
-template <typename T>
-void launch_bwd_c(const RotGeom& g, const GradSet& q, const GradSet& k, float eps, float* part, int blocks, int c, int items, hipStream_t stream) {
-    if (c == 8) launch_bwd<T, 8>(g, q, k, eps, part, blocks, items, stream);
-    else if (c == 4) launch_bwd<T, 4>(g, q, k, eps, part, blocks, items, stream);
-    else if (c == 2) launch_bwd<T, 2>(g, q, k, eps, part, blocks, items, stream);
-    else launch_bwd<T, 1>(g, q, k, eps, part, blocks, items, stream);
+template <typename T, bool NB, bool NORM, int C, int K> void run(const Bwd& b) {
+    hipLaunchKernelGGL((headnorm_bwd_kernel<T, C, K, NB>), dim3(b.blocks), dim3(ROT_THREADS), lds_bytes(b.g), b.stream, b.g, b.q, b.k, b.eps, b.part);
+}
+// the widest vector is 16 bytes: 16 / size pairs of halves, 8 / size pairs of neighbours
+template <typename T, bool NB, bool NORM, typename Job> void launch_c(const Job& j, int c) {
+    constexpr int TOP = (NB ? 8 : 16) / sizeof(T);
+    if (c == 8) run<T, NB, NORM, TOP >= 8 ? 8 : 1, 1>(j);
+    else if (c == 4) run<T, NB, NORM, TOP >= 4 ? 4 : 1, 1>(j);
+    else if (c == 2) run<T, NB, NORM, TOP >= 2 ? 2 : 1, 1>(j);
+    else if (j.items > 1) run<T, NB, NORM, 1, 2>(j);
+    else run<T, NB, NORM, 1, 1>(j);
+}
+template <bool NORM, typename Job> void launch(const Job& j, int c, int act) {
+    if (act) j.g.neighbours ? launch_c<__bf16, true, NORM>(j, c) : launch_c<__bf16, false, NORM>(j, c);
+    else j.g.neighbours ? launch_c<float, true, NORM>(j, c) : launch_c<float, false, NORM>(j, c);
 }
 
 }  // namespace
@@ -438,8 +452,7 @@ extern "C" int uncr_rotary_axes(const void* x, long long x_ts, long long x_hs, v
     const void* const pt[] = {x, y};
     const int c = pick_c(g, st, 4, pt, 2, act ? 2 : 4), items = shape(g, c, H);
     const HeadSet q = {x, y, nullptr, x_ts, x_hs, y_ts, y_hs, H}, none = {nullptr, nullptr, nullptr, 0, 0, 0, 0, 0};
-    if (act) launch_fwd_c<__bf16, false>(g, q, none, 0.f, c, items, stream);
-    else launch_fwd_c<float, false>(g, q, none, 0.f, c, items, stream);
+    launch<false>(Fwd{g, q, none, 0.f, items, stream}, c, act);
     UNCR_LAUNCH_CHECK();
     return UNCR_OK;
 }
@@ -459,8 +472,7 @@ extern "C" int uncr_headnorm_rotary_fwd(const void* q, long long q_ts, long long
     const void* const pt[] = {q, k, qo, ko};
     const int c = pick_c(g, st, 5, pt, 4, act ? 2 : 4, wq, wk), items = shape(g, c, Hq + Hk);
     const HeadSet zq = {q, qo, wq, q_ts, q_hs, (long long)Hq * D, D, Hq}, zk = {k, ko, wk, k_ts, k_hs, (long long)Hk * D, D, Hk};
-    if (act) launch_fwd_c<__bf16, true>(g, zq, zk, eps, c, items, stream);
-    else launch_fwd_c<float, true>(g, zq, zk, eps, c, items, stream);
+    launch<true>(Fwd{g, zq, zk, eps, items, stream}, c, act);
     UNCR_LAUNCH_CHECK();
     return UNCR_OK;
 }
@@ -483,14 +495,13 @@ extern "C" int uncr_headnorm_rotary_bwd(const void* q, long long q_ts, long long
         const long long st[] = {q_ts, q_hs, k_ts, k_hs, gq_ts, gq_hs, gk_ts, gk_hs, (long long)D};
         const void* const pt[] = {q, k, gq, gk, dq, dk};
         const int c = pick_c(g, st, 9, pt, 6, act ? 2 : 4, wq, wk), items = shape(g, c, Hq + Hk);
-        const int tiles = (N + g.tok - 1) / g.tok;
+        const int per = g.tok * (ROT_THREADS / 64), tiles = (N + per - 1) / per;
         blocks = tiles < ROT_MAX_SLOTS ? tiles : ROT_MAX_SLOTS;
         const GradSet zq = {q, gq, dq, wq, q_ts, q_hs, gq_ts, gq_hs, Hq}, zk = {k, gk, dk, wk, k_ts, k_hs, gk_ts, gk_hs, Hk};
-        if (act) launch_bwd_c<__bf16>(g, zq, zk, eps, part, blocks, c, items, stream);
-        else launch_bwd_c<float>(g, zq, zk, eps, part, blocks, c, items, stream);
+        launch<true>(Bwd{g, zq, zk, eps, items, blocks, part, stream}, c, act);
         UNCR_LAUNCH_CHECK();
     }
-    hipLaunchKernelGGL(headnorm_dw_kernel, dim3((2 * D + 15) / 16), dim3(256), 0, stream, part, blocks, D, dwq, dwk);
+    hipLaunchKernelGGL(headnorm_dw_kernel, dim3((2 * D + 15) / 16), dim3(1024), 0, stream, part, blocks, D, dwq, dwk);
     UNCR_LAUNCH_CHECK();
     return UNCR_OK;
 }

@@ -158,19 +158,22 @@ def set_profiler(p):
     _PROF = p
 
 
+_CALLS = {}       # entry point -> (function, prototype, which arguments are pointers)
+
+
+def _entry(name: str):
+    L = dev_lib() if name.startswith("uncr_debug_") else lib()
+    proto = L.protos[name]
+    _CALLS[name] = L.fn[name], proto, tuple("*" in typ for typ, _ in proto)
+    return _CALLS[name]
+
+
 def call(name: str, *args):
     """Call an entry point; tensors are converted to pointers; raises RuntimeError on a non-zero code."""
-    L = dev_lib() if name.startswith("uncr_debug_") else lib()
-    f = L.fn[name]
-    proto = L.protos[name]
+    f, proto, pointers = _CALLS.get(name) or _entry(name)
     if len(args) != len(proto):
         raise TypeError(f"{name}: expected {len(proto)} args, got {len(args)}")
-    conv = []
-    for a, (typ, _) in zip(args, proto):
-        if "*" in typ or typ == "hipStream_t":
-            conv.append(_ptr(a) if typ != "hipStream_t" else a)
-        else:
-            conv.append(a)
+    conv = [_ptr(a) if p and a is not None and type(a) is not int else a for a, p in zip(args, pointers)]
     if _PROF is not None and (name in _PROF.names or _PROF.scope is not None):
         import torch
         e0, e1 = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
@@ -192,4 +195,4 @@ def call(name: str, *args):
 
 def query(name: str, *args) -> int:
     """Call a pure size-query entry point (returns its int result, no error convention)."""
-    return lib().fn[name](*args)
+    return (_CALLS.get(name) or _entry(name))[0](*args)

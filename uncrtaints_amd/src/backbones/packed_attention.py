@@ -60,9 +60,10 @@ class HeadNormRotary(nn.Module):
         E.check_tokens(q=q, k=k)
         E.check_device(q=q, q_weight=self.q_weight, k_weight=self.k_weight)
         plan = self.rotary.plan(positions, q.shape[:-2], q.device) if self.rotary is not None else E.RotaryPlan()
-        qo, ko = _HeadNormRotaryFn.apply(q.reshape(-1, *q.shape[-2:]), k.reshape(-1, *k.shape[-2:]), self.q_weight, self.k_weight,
-                                         self.eps, plan)
-        return qo.view(q.shape), ko.view(k.shape)
+        rows = (q, k) if q.dim() == 3 else (q.reshape(-1, *q.shape[-2:]), k.reshape(-1, *k.shape[-2:]))
+        args = (*rows, self.q_weight, self.k_weight, self.eps, plan)
+        qo, ko = _HeadNormRotaryFn.apply(*args) if torch.is_grad_enabled() else E.headnorm_rotary_forward(*args)
+        return (qo, ko) if q.dim() == 3 else (qo.view(q.shape), ko.view(k.shape))
 
 
 class _PackedAttentionFn(torch.autograd.Function):

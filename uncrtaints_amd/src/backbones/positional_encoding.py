@@ -90,20 +90,23 @@ class RotaryAxes(nn.Module):
         from ... import engine as E
         if positions.dtype not in E._POS_DT:
             raise RuntimeError(f"positions: unsupported dtype {positions.dtype} (int32, int64, float32 or float64)")
-        if tuple(positions.shape) != tuple(lead) + (len(self.sections),):
-            raise ValueError(f"positions {tuple(positions.shape)}: expected {tuple(lead) + (len(self.sections),)}")
+        if positions.shape != (*lead, len(self.sections)):
+            raise ValueError(f"positions {tuple(positions.shape)}: expected {(*lead, len(self.sections))}")
         if positions.requires_grad:
             raise ValueError("positions carry no gradient: detach them")
         E.check_device(positions=positions, rotary=self.turns_bits)
         if positions.device != device:
             raise RuntimeError(f"positions are on {positions.device}, the tokens on {device}")
-        return E.RotaryPlan(positions.contiguous().view(-1, len(self.sections)), self.sections, self.turns_bits,
+        return E.RotaryPlan(positions.contiguous(), self.sections, self.turns_bits,
                             self.pairs == "neighbours")
 
     def forward(self, x, positions):
         from ... import engine as E
-        if x.dim() < 2 or x.shape[-1] != self.d or x.shape[-2] == 0:
-            raise ValueError(f"expected tokens [..., heads, {self.d}], got {tuple(x.shape)}")
+        shape = x.shape
+        if len(shape) < 2 or shape[-1] != self.d or shape[-2] == 0:
+            raise ValueError(f"expected tokens [..., heads, {self.d}], got {tuple(shape)}")
         E.check_tokens(x=x)
-        plan = self.plan(positions, x.shape[:-2], x.device)
-        return _RotaryFn.apply(x.reshape(-1, *x.shape[-2:]), plan).view(x.shape)
+        plan = self.plan(positions, shape[:-2], x.device)
+        rows = x if len(shape) == 3 else x.reshape(-1, *shape[-2:])
+        y = _RotaryFn.apply(rows, plan) if x.requires_grad and torch.is_grad_enabled() else E.rotary_axes(rows, plan)
+        return y if len(shape) == 3 else y.view(shape)
