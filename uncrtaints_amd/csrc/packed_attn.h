@@ -201,13 +201,6 @@ template <typename T, int DP> __device__ __forceinline__ f32x16 attn_product(con
 template <typename T> struct AttnProb;
 template <> struct AttnProb<__bf16> {
     bf16x8 v[2];
-    __device__ __forceinline__ float get(int i) const { return (float)v[i / 8][i % 8]; }
-    __device__ __forceinline__ void save(f32x4* at, int lane) const {
-        for (int u = 0; u < 2; ++u) at[u * 64 + lane] = __builtin_bit_cast(f32x4, v[u]);
-    }
-    __device__ __forceinline__ void load(const f32x4* at, int lane) {
-        for (int u = 0; u < 2; ++u) v[u] = __builtin_bit_cast(bf16x8, at[u * 64 + lane]);
-    }
     __device__ __forceinline__ void set(const f32x16& p) {
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
@@ -220,20 +213,54 @@ template <> struct AttnProb<__bf16> {
 };
 template <> struct AttnProb<float> {
     f32x16 v;
-    __device__ __forceinline__ float get(int i) const { return v[i]; }
-    __device__ __forceinline__ void save(f32x4* at, int lane) const {
+    __device__ __forceinline__ void set(const f32x16& p) { v = p; }
+};
+
+// The C registers of a 32-row product on their way through LDS from one wave to another, lane by lane, conflict-free.  With bf16 storage the
+// upper three bytes of each cross (17 significant bits): all four do not fit beside the tiles, and as bf16 P would take the rounding that
+// dS gets anyway a second time (dK's error against 64 bits 0.0030 instead of 0.0024).
+template <typename T> struct AttnPass;
+template <> struct AttnPass<__bf16> {
+    static constexpr int PARTS = 3;
+    static __device__ __forceinline__ void save(f32x4* at, int lane, const f32x16& p) {
+        unsigned d[12];
 #pragma unroll
-        for (int u = 0; u < 4; ++u) at[u * 64 + lane] = (f32x4){v[4 * u], v[4 * u + 1], v[4 * u + 2], v[4 * u + 3]};
+        for (int e = 0; e < 4; ++e) {
+            unsigned w[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) w[i] = __float_as_uint(p[4 * e + i]);
+            d[3 * e] = __builtin_amdgcn_perm(w[1], w[0], 0x05030201u);
+            d[3 * e + 1] = __builtin_amdgcn_perm(w[2], w[1], 0x06050302u);
+            d[3 * e + 2] = __builtin_amdgcn_perm(w[3], w[2], 0x07060503u);
+        }
+#pragma unroll
+        for (int u = 0; u < 3; ++u)
+            at[u * 64 + lane] = (f32x4){__uint_as_float(d[4 * u]), __uint_as_float(d[4 * u + 1]), __uint_as_float(d[4 * u + 2]), __uint_as_float(d[4 * u + 3])};
     }
+    f32x4 v[3];
     __device__ __forceinline__ void load(const f32x4* at, int lane) {
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-            const f32x4 x = at[u * 64 + lane];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) v[4 * u + i] = x[i];
-        }
+        for (int u = 0; u < 3; ++u) v[u] = at[u * 64 + lane];
     }
-    __device__ __forceinline__ void set(const f32x16& p) { v = p; }
+    __device__ __forceinline__ float get(int i) const {
+        const int e = i / 4 * 3;
+        auto d = [&](int k) { return __float_as_uint(v[(e + k) / 4][(e + k) % 4]); };
+        return __uint_as_float(i % 4 == 0 ? __builtin_amdgcn_perm(d(0), d(0), 0x0201000cu) : i % 4 == 1 ? __builtin_amdgcn_perm(d(1), d(0), 0x0504030cu)
+                               : i % 4 == 2 ? __builtin_amdgcn_perm(d(2), d(1), 0x0403020cu) : __builtin_amdgcn_perm(d(2), d(2), 0x0302010cu));
+    }
+};
+template <> struct AttnPass<float> {
+    static constexpr int PARTS = 4;
+    static __device__ __forceinline__ void save(f32x4* at, int lane, const f32x16& p) {
+#pragma unroll
+        for (int u = 0; u < 4; ++u) at[u * 64 + lane] = (f32x4){p[4 * u], p[4 * u + 1], p[4 * u + 2], p[4 * u + 3]};
+    }
+    f32x4 v[4];
+    __device__ __forceinline__ void load(const f32x4* at, int lane) {
+#pragma unroll
+        for (int u = 0; u < 4; ++u) v[u] = at[u * 64 + lane];
+    }
+    __device__ __forceinline__ float get(int i) const { return v[i / 4][i % 4]; }
 };
 
 // X^T (32 of DP x 32 rows) from the rows row0 .. row0 + 31 of a tile, in the row order of AttnProb, and acc += X^T * P

@@ -119,7 +119,7 @@ __global__ __launch_bounds__(NW * 64) void packed_attn_dq_kernel(const AttnGeom 
 //   first:  S = Q K^T, P = exp2(S c - lse), P to LDS, dV^T += dOut^T P          second, one tile behind:  dP = dOut V^T, dS, dK^T += Q^T dS
 // Both make half of the products and hold half of the accumulators (one wave with both needs 470 registers and leaves one wave per SIMD with
 // nothing to run beside it); the exponentials of one wave run beside the products of the other.  P crosses in the accumulator layout, lane
-// by lane, in the storage type: bf16 rounds it once for both products it takes part in.  Q and dOut tiles rotate through three buffers: the one being filled and those of the two roles.
+// by lane.  Q and dOut tiles rotate through three buffers: the one being filled and those of the two roles.
 template <typename T, int DP, bool VEC>
 __global__ __launch_bounds__(512) void packed_attn_dkv_kernel(const AttnGeom g, const AttnTensor q, const AttnTensor k, const AttnTensor v,
                                                               const AttnTensor go, const float* __restrict__ rowstat,
@@ -128,7 +128,7 @@ __global__ __launch_bounds__(512) void packed_attn_dkv_kernel(const AttnGeom g, 
     constexpr int NT = 512, BN = 128, SHIFT = 7, TQ = sizeof(T) == 2 ? 64 : 32;
     constexpr bool EARLY = L::RB <= 256;       // registers for the transposed operand beside the first product (not for fp32 rows of 512 bytes)
     __shared__ alignas(16) char lds_q[3][TQ * L::RB], lds_g[3][TQ * L::RB];
-    __shared__ f32x4 lds_p[2][4][TQ / 32][sizeof(AttnProb<T>) / 16][64];
+    __shared__ f32x4 lds_p[2][4][TQ / 32][AttnPass<T>::PARTS][64];
     __shared__ alignas(16) float lds_s[3][2][64];       // lse in powers of two and delta of a tile's rows
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5, col = lane & 31, pair = wave & 3;
     const bool second = wave >= 4;
@@ -237,7 +237,7 @@ __global__ __launch_bounds__(512) void packed_attn_dkv_kernel(const AttnGeom g, 
                         }
                         AttnProb<T> p;
                         p.set(sc);
-                        p.save(&lds_p[it & 1][pair][t][0][0], lane);
+                        AttnPass<T>::save(&lds_p[it & 1][pair][t][0][0], lane, sc);
 #pragma unroll
                         for (int db = 0; db < L::DB; ++db) {
                             if (!EARLY) y[db].fetch(lds_g[cur], t * 32, db, lane);
@@ -255,7 +255,7 @@ __global__ __launch_bounds__(512) void packed_attn_dkv_kernel(const AttnGeom g, 
                     f32x4 dl[4];
 #pragma unroll
                     for (int e = 0; e < 4; ++e) dl[e] = *reinterpret_cast<const f32x4*>(&lds_s[prev][1][t * 32 + 8 * e + 4 * h]);
-                    AttnProb<T> p;
+                    AttnPass<T> p;
                     p.load(&lds_p[(it - 1) & 1][pair][t][0][0], lane);
                     AttnCols<T, DP> y[L::DB];
 #pragma unroll

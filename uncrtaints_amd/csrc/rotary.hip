@@ -207,7 +207,8 @@ __global__ __launch_bounds__(ROT_THREADS) void rotary_kernel(const RotGeom g, co
 
 struct GradSet { const void* x; const void* dy; void* dx; const float* w; long long ts, hs, gts, ghs; int H; };
 
-// The norm's gradient.  A block walks over token tiles (at most ROT_MAX_SLOTS blocks), dw of queries and keys in registers, and leaves
+// The norm's gradient.  At most four pairs per lane: with eight (164 registers, three waves per SIMD) 40001 tokens x 40 heads x 128 in bf16
+// take 320 us, with four (108, four waves) 247 us (5.0 TB/s).  A block walks over token tiles (at most ROT_MAX_SLOTS blocks), dw of queries and keys in registers, and leaves
 // one row of partials: their sum in the next launch is in a fixed order, no atomics
 template <typename T, int C, int K, bool NB>
 __global__ __launch_bounds__(ROT_THREADS) void headnorm_bwd_kernel(const RotGeom g, const GradSet q, const GradSet k, float eps,
@@ -363,10 +364,11 @@ __global__ __launch_bounds__(1024) void headnorm_dw_kernel(const float* __restri
 
 // Pairs per lane: as many as one 16-byte vector holds of one component (halves) or of whole pairs (neighbours), fewer where an axis' half
 // section would be cut or a row does not start aligned for it
-int pick_c(const RotGeom& g, const long long* strides, int n_strides, const void* const* ptrs, int n_ptrs, int size, const float* wq = nullptr,
+int pick_c(const RotGeom& g, const long long* strides, int n_strides, const void* const* ptrs, int n_ptrs, int size, int max_c, const float* wq = nullptr,
            const float* wk = nullptr) {
     const int halves[5] = {g.sec0 / 2, g.sec1 / 2, g.sec2 / 2, g.sec3 / 2, (g.D - g.sec0 - g.sec1 - g.sec2 - g.sec3) / 2};
-    for (int c = (g.neighbours ? 8 : 16) / size; c > 1; c >>= 1) {
+    const int wide = (g.neighbours ? 8 : 16) / size;
+    for (int c = wide < max_c ? wide : max_c; c > 1; c >>= 1) {
         const int align = c * size * (g.neighbours ? 2 : 1);
         bool ok = (g.D / 2) % c == 0;
         if (!g.neighbours)
@@ -410,8 +412,8 @@ int geom(RotGeom& g, const void* pos, int pos_dt, int n_axes, int s0, int s1, in
     return UNCR_OK;
 }
 
-struct Fwd { RotGeom g; HeadSet q, k; float eps; int items; hipStream_t stream; };
-struct Bwd { RotGeom g; GradSet q, k; float eps; int items, blocks; float* part; hipStream_t stream; };
+struct Fwd { static constexpr int MAX_C = 8; RotGeom g; HeadSet q, k; float eps; int items; hipStream_t stream; };
+struct Bwd { static constexpr int MAX_C = 4; RotGeom g; GradSet q, k; float eps; int items, blocks; float* part; hipStream_t stream; };
 
 size_t lds_bytes(const RotGeom& g) { return (size_t)(ROT_THREADS / 64) * g.tok * (g.D / 2) * sizeof(float2); }
 
@@ -424,7 +426,7 @@ template <typename T, bool NB, bool NORM, int C, int K> void run(const Bwd& b) {
 }
 // the widest vector is 16 bytes: 16 / size pairs of halves, 8 / size pairs of neighbours
 template <typename T, bool NB, bool NORM, typename Job> void launch_c(const Job& j, int c) {
-    constexpr int TOP = (NB ? 8 : 16) / sizeof(T);
+    constexpr int WIDE = (NB ? 8 : 16) / sizeof(T), TOP = WIDE < Job::MAX_C ? WIDE : Job::MAX_C;
     if (c == 8) run<T, NB, NORM, TOP >= 8 ? 8 : 1, 1>(j);
     else if (c == 4) run<T, NB, NORM, TOP >= 4 ? 4 : 1, 1>(j);
     else if (c == 2) run<T, NB, NORM, TOP >= 2 ? 2 : 1, 1>(j);
@@ -450,7 +452,7 @@ extern "C" int uncr_rotary_axes(const void* x, long long x_ts, long long x_hs, v
     if (!x || !y) return UNCR_EINVAL;
     const long long st[] = {x_ts, x_hs, y_ts, y_hs};
     const void* const pt[] = {x, y};
-    const int c = pick_c(g, st, 4, pt, 2, act ? 2 : 4), items = shape(g, c, H);
+    const int c = pick_c(g, st, 4, pt, 2, act ? 2 : 4, Fwd::MAX_C), items = shape(g, c, H);
     const HeadSet q = {x, y, nullptr, x_ts, x_hs, y_ts, y_hs, H}, none = {nullptr, nullptr, nullptr, 0, 0, 0, 0, 0};
     launch<false>(Fwd{g, q, none, 0.f, items, stream}, c, act);
     UNCR_LAUNCH_CHECK();
@@ -470,7 +472,7 @@ extern "C" int uncr_headnorm_rotary_fwd(const void* q, long long q_ts, long long
     if (!q || !k || !wq || !wk || !qo || !ko) return UNCR_EINVAL;
     const long long st[] = {q_ts, q_hs, k_ts, k_hs, (long long)D};
     const void* const pt[] = {q, k, qo, ko};
-    const int c = pick_c(g, st, 5, pt, 4, act ? 2 : 4, wq, wk), items = shape(g, c, Hq + Hk);
+    const int c = pick_c(g, st, 5, pt, 4, act ? 2 : 4, Fwd::MAX_C, wq, wk), items = shape(g, c, Hq + Hk);
     const HeadSet zq = {q, qo, wq, q_ts, q_hs, (long long)Hq * D, D, Hq}, zk = {k, ko, wk, k_ts, k_hs, (long long)Hk * D, D, Hk};
     launch<true>(Fwd{g, zq, zk, eps, items, stream}, c, act);
     UNCR_LAUNCH_CHECK();
@@ -494,7 +496,7 @@ extern "C" int uncr_headnorm_rotary_bwd(const void* q, long long q_ts, long long
         if (!q || !k || !wq || !wk || !gq || !gk || !dq || !dk) return UNCR_EINVAL;
         const long long st[] = {q_ts, q_hs, k_ts, k_hs, gq_ts, gq_hs, gk_ts, gk_hs, (long long)D};
         const void* const pt[] = {q, k, gq, gk, dq, dk};
-        const int c = pick_c(g, st, 9, pt, 6, act ? 2 : 4, wq, wk), items = shape(g, c, Hq + Hk);
+        const int c = pick_c(g, st, 9, pt, 6, act ? 2 : 4, Bwd::MAX_C, wq, wk), items = shape(g, c, Hq + Hk);
         const int per = g.tok * (ROT_THREADS / 64), tiles = (N + per - 1) / per;
         blocks = tiles < ROT_MAX_SLOTS ? tiles : ROT_MAX_SLOTS;
         const GradSet zq = {q, gq, dq, wq, q_ts, q_hs, gq_ts, gq_hs, Hq}, zk = {k, gk, dk, wk, k_ts, k_hs, gk_ts, gk_hs, Hk};
