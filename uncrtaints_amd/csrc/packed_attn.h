@@ -118,6 +118,10 @@ template <bool KEYS> __device__ __forceinline__ bool attn_find_sorted(const Attn
     tile = KEYS ? (top[b] - lo) / unit : tiles[b] - 1 - (top[b] - lo) / unit;
     return true;
 }
+// Fewer than four blocks of `rows` rows per CU: CUs with one block more than others set the time.  Blocks of half as many rows then, whose
+// waves pair up and share the keys of each tile (two sequences of 4096 and 1587 tokens, 8 heads of 32, fp32: forward
+// 254 -> 225 us, dQ 358 -> 313 us)
+static inline bool attn_few_blocks(const AttnGeom& g, int rows) { return (((long long)g.Nq * g.G / rows) + g.B) * g.Hk < 1024; }
 // Sorting costs a block about 2 us: for causal sequences of at least four tiles on average
 static inline bool attn_sorts(const AttnGeom& g, long long rows, int per_tile) {
     return g.causal && g.B <= ATTN_SORT_MAX_B && rows / per_tile >= 4ll * g.B && (long long)g.Nk * g.G < (1ll << 29) && (long long)g.G * per_tile < (1 << 20);
@@ -134,6 +138,9 @@ template <typename T, int DP> struct AttnTile {
     static constexpr int NCH = DP / EPC;                  // chunks per row
     static constexpr int RB = NCH * 16;                   // bytes per row
     static constexpr int KS = NCH / 2;                    // operand steps over DP: a step is one chunk of each lane half
+    // waves per SIMD the kernels are compiled for: no more registers than 512 / WAVES, so that the accumulators stay where vector
+    // instructions reach them (the compiler moves them to and fro otherwise)
+    static constexpr int WAVES = RB <= 128 ? 3 : RB <= 256 ? 2 : 1;
     static constexpr int DB = DP < 32 ? 1 : DP / 32;      // 32-wide blocks of DP (DP = 16: half a block, its other half repeats the first)
 
     static __device__ __forceinline__ int swizzle(int row) {

@@ -7,12 +7,12 @@
 
 namespace {
 
-template <typename T, int DP, int NW, int TK, bool VEC>
-__global__ __launch_bounds__(NW * 64) void packed_attn_fwd_kernel(const AttnGeom g, const AttnTensor q, const AttnTensor k, const AttnTensor v,
+template <typename T, int DP, int NW, int TK, int KSPLIT, bool VEC>
+__global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(AttnTile<T, DP>::WAVES))) void packed_attn_fwd_kernel(const AttnGeom g, const AttnTensor q, const AttnTensor k, const AttnTensor v,
                                                                   T* __restrict__ out, long long o_ts, long long o_hs,
                                                                   float* __restrict__ lse, int slots) {
     typedef AttnTile<T, DP> L;
-    constexpr int NT = NW * 64, BM = NW * 32, SHIFT = NW == 8 ? 8 : NW == 4 ? 7 : NW == 2 ? 6 : 5;
+    constexpr int NT = NW * 64, GROUPS = NW / KSPLIT, BM = GROUPS * 32, SHIFT = BM == 256 ? 8 : BM == 128 ? 7 : 6;
     __shared__ alignas(16) char lds_k[2][TK * L::RB], lds_v[2][TK * L::RB];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5, col = lane & 31;
     if (g.fill) attn_fill_outside<T>(g.off_q, g.B, g.Nq, out, o_ts, o_hs, g.Hq, g.D, lse, blockIdx.x, gridDim.x);
@@ -24,7 +24,7 @@ __global__ __launch_bounds__(NW * 64) void packed_attn_fwd_kernel(const AttnGeom
     const AttnSeq s = attn_seq(g, b);
     const int rows = s.lq * g.G;
     if (tile * BM >= rows) return;
-    const int row0 = tile * BM + wave * 32;
+    const int row0 = tile * BM + wave % GROUPS * 32, share = wave / GROUPS;      // KSPLIT waves have the same rows and every KSPLIT-th 32 keys
     const int row = min(row0 + col, rows - 1), tok = row / g.G, head = hk * g.G + row - tok * g.G;
     // keys [0, limit) are visible to this lane's row
     const int shift = s.lk - s.lq;
@@ -41,6 +41,7 @@ __global__ __launch_bounds__(NW * 64) void packed_attn_fwd_kernel(const AttnGeom
 
     const T* kb = (const T*)k.p + (size_t)s.k0 * k.ts + (size_t)hk * k.hs;
     const T* vb = (const T*)v.p + (size_t)s.k0 * v.ts + (size_t)hk * v.hs;
+    constexpr int SUB = TK / 32 / KSPLIT;
     const int tiles = (block_hi + TK - 1) / TK;
     AttnStage<T, DP, TK, NT, VEC> ks, vs;
     if (tiles) {
@@ -60,24 +61,24 @@ __global__ __launch_bounds__(NW * 64) void packed_attn_fwd_kernel(const AttnGeom
         if (j0 < wave_hi) {
             const char* tk = lds_k[it & 1];
             const char* tv = lds_v[it & 1];
-            f32x16 sc[TK / 32];
+            f32x16 sc[SUB];
 #pragma unroll
-            for (int t = 0; t < TK / 32; ++t) {
+            for (int t = 0; t < SUB; ++t) {
                 AttnRows<T, DP> kf;
-                kf.fetch(tk, t * 32 + col, h);
+                kf.fetch(tk, (t * KSPLIT + share) * 32 + col, h);
                 attn_fence();
                 sc[t] = attn_product(kf, qf);
             }
             if (j0 + TK > wave_lo) {
 #pragma unroll
-                for (int t = 0; t < TK / 32; ++t)
+                for (int t = 0; t < SUB; ++t)
 #pragma unroll
                     for (int i = 0; i < 16; ++i)
-                        if (j0 + t * 32 + 8 * (i / 4) + 4 * h + i % 4 >= limit) sc[t][i] = -INFINITY;
+                        if (j0 + (t * KSPLIT + share) * 32 + 8 * (i / 4) + 4 * h + i % 4 >= limit) sc[t][i] = -INFINITY;
             }
             float mx = sc[0][0];
 #pragma unroll
-            for (int t = 0; t < TK / 32; ++t)
+            for (int t = 0; t < SUB; ++t)
 #pragma unroll
                 for (int i = 0; i < 16; ++i) mx = fmaxf(mx, sc[t][i]);
             mx = fmaxf(mx, attn_other_half(mx)) * g.c;
@@ -92,7 +93,7 @@ __global__ __launch_bounds__(NW * 64) void packed_attn_fwd_kernel(const AttnGeom
             }
             const float ref = m == -INFINITY ? 0.f : m;
 #pragma unroll
-            for (int t = 0; t < TK / 32; ++t) {
+            for (int t = 0; t < SUB; ++t) {
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
                     sc[t][i] = __builtin_amdgcn_exp2f(fmaf(sc[t][i], g.c, -ref));
@@ -103,7 +104,7 @@ __global__ __launch_bounds__(NW * 64) void packed_attn_fwd_kernel(const AttnGeom
 #pragma unroll
                 for (int db = 0; db < L::DB; ++db) {
                     AttnCols<T, DP> vf;
-                    vf.fetch(tv, t * 32, db, lane);
+                    vf.fetch(tv, (t * KSPLIT + share) * 32, db, lane);
                     vf.mma(acc[db], p);
                 }
             }
@@ -116,20 +117,48 @@ __global__ __launch_bounds__(NW * 64) void packed_attn_fwd_kernel(const AttnGeom
         __syncthreads();
     }
     l += attn_other_half(l);
+    if (KSPLIT == 2) {          // the second wave's sums to the first one, through the tiles nobody needs any more
+        float* pass = (float*)&lds_k[0][0] + wave % GROUPS * (L::DB * 16 * 64);
+        __shared__ float pass_m[GROUPS][64], pass_l[GROUPS][64];
+        if (share) {
+#pragma unroll
+            for (int db = 0; db < L::DB; ++db)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) pass[(db * 16 + i) * 64 + lane] = acc[db][i];
+            pass_m[wave % GROUPS][lane] = m;
+            pass_l[wave % GROUPS][lane] = l;
+        }
+        __syncthreads();
+        if (share) return;
+        const float m1 = pass_m[wave % GROUPS][lane], mn = fmaxf(m, m1), ref = mn == -INFINITY ? 0.f : mn;
+        const float f0 = __builtin_amdgcn_exp2f(m - ref), f1 = __builtin_amdgcn_exp2f(m1 - ref);
+        l = l * f0 + pass_l[wave % GROUPS][lane] * f1;
+        m = mn;
+#pragma unroll
+        for (int db = 0; db < L::DB; ++db)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) acc[db][i] = acc[db][i] * f0 + pass[(db * 16 + i) * 64 + lane] * f1;
+    }
     if (row0 + col >= rows) return;
     const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
     attn_store_row<T, L::DB>(out + (size_t)(s.q0 + tok) * o_ts + (size_t)head * o_hs, acc, inv, h, g.D);
     if (lse && h == 0) lse[(size_t)(s.q0 + tok) * g.Hq + head] = l > 0.f || l != l ? (m + __builtin_amdgcn_logf(l)) * 0.69314718055994531f : -INFINITY;
 }
 
-template <typename T, int DP, int NW, int TK>
-void launch(AttnGeom g, const AttnTensor& q, const AttnTensor& k, const AttnTensor& v, void* out, long long o_ts, long long o_hs, float* lse,
-            bool vec, hipStream_t stream) {
-    constexpr int SHIFT = NW == 8 ? 8 : 7;
+template <typename T, int DP, int NW, int TK, int KSPLIT>
+void launch_k(AttnGeom g, const AttnTensor& q, const AttnTensor& k, const AttnTensor& v, void* out, long long o_ts, long long o_hs, float* lse, bool vec,
+              hipStream_t stream) {
+    constexpr int BM = NW / KSPLIT * 32, SHIFT = BM == 256 ? 8 : BM == 128 ? 7 : 6;
     const int slots = attn_slots((long long)g.Nq * g.G, g.B, SHIFT);
-    g.sorted = attn_sorts(g, (long long)g.Nq * g.G, 1 << SHIFT);
-    if (vec) hipLaunchKernelGGL((packed_attn_fwd_kernel<T, DP, NW, TK, true>), dim3(slots * g.Hk), dim3(NW * 64), 0, stream, g, q, k, v, (T*)out, o_ts, o_hs, lse, slots);
-    else hipLaunchKernelGGL((packed_attn_fwd_kernel<T, DP, NW, TK, false>), dim3(slots * g.Hk), dim3(NW * 64), 0, stream, g, q, k, v, (T*)out, o_ts, o_hs, lse, slots);
+    g.sorted = attn_sorts(g, (long long)g.Nq * g.G, BM);
+    if (vec) hipLaunchKernelGGL((packed_attn_fwd_kernel<T, DP, NW, TK, KSPLIT, true>), dim3(slots * g.Hk), dim3(NW * 64), 0, stream, g, q, k, v, (T*)out, o_ts, o_hs, lse, slots);
+    else hipLaunchKernelGGL((packed_attn_fwd_kernel<T, DP, NW, TK, KSPLIT, false>), dim3(slots * g.Hk), dim3(NW * 64), 0, stream, g, q, k, v, (T*)out, o_ts, o_hs, lse, slots);
+}
+template <typename T, int DP, int NW, int TK>
+void launch(const AttnGeom& g, const AttnTensor& q, const AttnTensor& k, const AttnTensor& v, void* out, long long o_ts, long long o_hs, float* lse,
+            bool vec, hipStream_t stream) {
+    if (TK == 64 && attn_few_blocks(g, NW * 32)) launch_k<T, DP, NW, TK, TK == 64 ? 2 : 1>(g, q, k, v, out, o_ts, o_hs, lse, vec, stream);
+    else launch_k<T, DP, NW, TK, 1>(g, q, k, v, out, o_ts, o_hs, lse, vec, stream);
 }
 
 }  // namespace

@@ -9,12 +9,12 @@
 
 namespace {
 
-template <typename T, int DP, int NW, int TK, bool VEC>
-__global__ __launch_bounds__(NW * 64) void packed_attn_dq_kernel(const AttnGeom g, const AttnTensor q, const AttnTensor k, const AttnTensor v,
+template <typename T, int DP, int NW, int TK, int KSPLIT, bool VEC>
+__global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(AttnTile<T, DP>::WAVES))) void packed_attn_dq_kernel(const AttnGeom g, const AttnTensor q, const AttnTensor k, const AttnTensor v,
                                                                  const AttnTensor o, const AttnTensor go, const float* __restrict__ lse,
                                                                  T* __restrict__ dq, float* __restrict__ rowstat, int slots) {
     typedef AttnTile<T, DP> L;
-    constexpr int NT = NW * 64, BM = NW * 32, SHIFT = NW == 8 ? 8 : 7;
+    constexpr int NT = NW * 64, GROUPS = NW / KSPLIT, BM = GROUPS * 32, SHIFT = BM == 256 ? 8 : BM == 128 ? 7 : 6;
     __shared__ alignas(16) char lds_k[2][TK * L::RB], lds_v[2][TK * L::RB];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5, col = lane & 31;
     attn_fill_outside<T>(g.off_q, g.B, g.Nq, dq, (long long)g.Hq * g.D, g.D, g.Hq, g.D, nullptr, blockIdx.x, gridDim.x);
@@ -25,7 +25,7 @@ __global__ __launch_bounds__(NW * 64) void packed_attn_dq_kernel(const AttnGeom 
     const AttnSeq s = attn_seq(g, b);
     const int rows = s.lq * g.G;
     if (tile * BM >= rows) return;
-    const int row0 = tile * BM + wave * 32;
+    const int row0 = tile * BM + wave % GROUPS * 32, share = wave / GROUPS;      // KSPLIT waves have the same rows and every KSPLIT-th 32 keys
     const int row = min(row0 + col, rows - 1), tok = row / g.G, head = hk * g.G + row - tok * g.G;
     const int shift = s.lk - s.lq;
     auto limit_of = [&](int r) { return g.causal ? min(max(min(r, rows - 1) / g.G + shift + 1, 0), s.lk) : s.lk; };
@@ -49,7 +49,7 @@ __global__ __launch_bounds__(NW * 64) void packed_attn_dq_kernel(const AttnGeom 
     // a row that saw nothing has lse = -inf: +inf makes its probabilities 0
     float ls = lse[at] * 1.4426950408889634f;
     if (ls == -INFINITY) ls = INFINITY;
-    if (h == 0 && row0 + col < rows) {          // for the dK/dV kernel: lse in powers of two, and delta behind it
+    if (h == 0 && share == 0 && row0 + col < rows) {          // for the dK/dV kernel: lse in powers of two, and delta behind it
         rowstat[at] = ls;
         rowstat[(size_t)g.Nq * g.Hq + at] = dl;
     }
@@ -80,7 +80,8 @@ __global__ __launch_bounds__(NW * 64) void packed_attn_dq_kernel(const AttnGeom 
             const char* tv = lds_v[it & 1];
             const bool edge = j0 + TK > wave_lo;
 #pragma unroll
-            for (int t = 0; t < TK / 32; ++t) {
+            for (int u = 0; u < TK / 32 / KSPLIT; ++u) {
+                const int t = u * KSPLIT + share;
                 AttnRows<T, DP> x;
                 x.fetch(tk, t * 32 + col, h);
                 attn_fence();
@@ -112,26 +113,41 @@ __global__ __launch_bounds__(NW * 64) void packed_attn_dq_kernel(const AttnGeom 
         attn_arrived();
         __syncthreads();
     }
+    if (KSPLIT == 2) {          // the second wave's sum to the first one, through the tiles nobody needs any more
+        float* pass = (float*)&lds_k[0][0] + wave % GROUPS * (L::DB * 16 * 64);
+        if (share) {
+#pragma unroll
+            for (int db = 0; db < L::DB; ++db)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) pass[(db * 16 + i) * 64 + lane] = acc[db][i];
+        }
+        __syncthreads();
+        if (share) return;
+#pragma unroll
+        for (int db = 0; db < L::DB; ++db)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) acc[db][i] += pass[(db * 16 + i) * 64 + lane];
+    }
     if (row0 + col < rows) attn_store_row<T, L::DB>(dq + at * g.D, acc, g.scale, h, g.D);
 }
 
-// A block owns 128 keys, 32 for each of four pairs of waves.  The first wave of a pair holds its keys' K and the sum dV, the second V and dK:
+// A block owns 32 keys for each of its pairs of waves.  The first wave of a pair holds its keys' K and the sum dV, the second V and dK:
 //   first:  S = Q K^T, P = exp2(S c - lse), P to LDS, dV^T += dOut^T P          second, one tile behind:  dP = dOut V^T, dS, dK^T += Q^T dS
 // Both make half of the products and hold half of the accumulators (one wave with both needs 470 registers and leaves one wave per SIMD with
 // nothing to run beside it); the exponentials of one wave run beside the products of the other.  P crosses in the accumulator layout, lane
 // by lane.  Q and dOut tiles rotate through three buffers: the one being filled and those of the two roles.
-template <typename T, int DP, bool VEC>
-__global__ __launch_bounds__(512) void packed_attn_dkv_kernel(const AttnGeom g, const AttnTensor q, const AttnTensor k, const AttnTensor v,
+template <typename T, int DP, int PAIRS, bool VEC>
+__global__ __launch_bounds__(PAIRS * 128) void packed_attn_dkv_kernel(const AttnGeom g, const AttnTensor q, const AttnTensor k, const AttnTensor v,
                                                               const AttnTensor go, const float* __restrict__ rowstat,
                                                               T* __restrict__ dk, T* __restrict__ dv, int slots) {
     typedef AttnTile<T, DP> L;
-    constexpr int NT = 512, BN = 128, SHIFT = 7, TQ = sizeof(T) == 2 ? 64 : 32;
+    constexpr int NT = PAIRS * 128, BN = PAIRS * 32, SHIFT = PAIRS == 4 ? 7 : 6, TQ = sizeof(T) == 2 ? 64 : 32;
     constexpr bool EARLY = L::RB <= 256;       // registers for the transposed operand beside the first product (not for fp32 rows of 512 bytes)
     __shared__ alignas(16) char lds_q[3][TQ * L::RB], lds_g[3][TQ * L::RB];
-    __shared__ f32x4 lds_p[2][4][TQ / 32][AttnPass<T>::PARTS][64];
-    __shared__ alignas(16) float lds_s[3][2][64];       // lse in powers of two and delta of a tile's rows
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5, col = lane & 31, pair = wave & 3;
-    const bool second = wave >= 4;
+    __shared__ f32x4 lds_p[2][PAIRS][TQ / 32][AttnPass<T>::PARTS][64];
+    __shared__ alignas(16) float lds_s[3][2][TQ];       // lse in powers of two and delta of a tile's rows
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5, col = lane & 31, pair = wave % PAIRS;
+    const bool second = wave >= PAIRS;
     attn_fill_outside<T>(g.off_k, g.B, g.Nk, dk, (long long)g.Hk * g.D, g.D, g.Hk, g.D, nullptr, blockIdx.x, gridDim.x);
     attn_fill_outside<T>(g.off_k, g.B, g.Nk, dv, (long long)g.Hk * g.D, g.D, g.Hk, g.D, nullptr, blockIdx.x, gridDim.x);
     const int hk = blockIdx.x % g.Hk;
@@ -166,9 +182,10 @@ __global__ __launch_bounds__(512) void packed_attn_dkv_kernel(const AttnGeom g, 
         Stage qs, gs;
         AttnCursor<const T> cq[Stage::CNT], cg[Stage::CNT];
         AttnCursor<const float> cl;
-        // lse (first waves) and delta (second waves) of 64 rows go to LDS in fours of waves, 16 rows each
-        const int lrow = pair * 16 + (lane & 15);
-        const bool lme = lane < 16 && lrow < TQ;
+        // lse (first waves) and delta (second waves) of the tile's rows go to LDS in equal shares
+        constexpr int SHARE = TQ / PAIRS;
+        const int lrow = pair * SHARE + lane % SHARE;
+        const bool lme = lane < SHARE;
         // the first tile repeats the last row behind it, and masks it
 #pragma unroll
         for (int i = 0; i < Stage::CNT; ++i) {
@@ -180,8 +197,8 @@ __global__ __launch_bounds__(512) void packed_attn_dkv_kernel(const AttnGeom g, 
             cg[i].set(gb, go.ts, go.hs, r, TQ, g.G);
         }
         {
-            const int r = row_of(0) + min(lrow, TQ - 1), t = min(r, rows - 1) / g.G;
-            if (lme) attn_dma4(&lds_s[0][second][pair * 16], lb + (size_t)t * g.Hq + (min(r, rows - 1) - t * g.G));
+            const int r = row_of(0) + lrow, t = min(r, rows - 1) / g.G;
+            if (lme) attn_dma4(&lds_s[0][second][pair * SHARE], lb + (size_t)t * g.Hq + (min(r, rows - 1) - t * g.G));
             cl.set(lb, g.Hq, 1, r, TQ, g.G);
         }
         auto begin = [&](int buf) {
@@ -193,7 +210,7 @@ __global__ __launch_bounds__(512) void packed_attn_dkv_kernel(const AttnGeom g, 
                 gs.begin(i, lds_g[buf], cg[i].p, g.D);
             }
             cl.move();
-            if (lme) attn_dma4(&lds_s[buf][second][pair * 16], cl.p);
+            if (lme) attn_dma4(&lds_s[buf][second][pair * SHARE], cl.p);
         };
         auto finish = [&](int buf) {
             qs.finish(lds_q[buf]);
@@ -299,17 +316,31 @@ struct Bwd {
     hipStream_t stream;
 };
 
+template <typename T, int DP, int NW, int TK, int KSPLIT, bool VEC> void launch_dq(const Bwd& a) {
+    constexpr int BM = NW / KSPLIT * 32, SHIFT = BM == 256 ? 8 : BM == 128 ? 7 : 6;
+    AttnGeom g = a.g;
+    g.sorted = attn_sorts(g, (long long)g.Nq * g.G, BM);
+    const int slots = attn_slots((long long)g.Nq * g.G, g.B, SHIFT);
+    hipLaunchKernelGGL((packed_attn_dq_kernel<T, DP, NW, TK, KSPLIT, VEC>), dim3(slots * g.Hk), dim3(NW * 64), 0, a.stream, g, a.q, a.k, a.v, a.o, a.go,
+                       a.lse, (T*)a.dq, a.rowstat, slots);
+}
+template <typename T, int DP, int PAIRS, bool VEC> void launch_dkv(const Bwd& a) {
+    AttnGeom g = a.g;
+    g.sorted = attn_sorts(g, g.Nk, PAIRS * 32);
+    const int slots = attn_slots(g.Nk, g.B, PAIRS == 4 ? 7 : 6);
+    hipLaunchKernelGGL((packed_attn_dkv_kernel<T, DP, PAIRS, VEC>), dim3(slots * g.Hk), dim3(PAIRS * 128), 0, a.stream, g, a.q, a.k, a.v, a.go, a.rowstat,
+                       (T*)a.dk, (T*)a.dv, slots);
+}
 template <typename T, int DP, int NW, int TK, bool VEC> void launch_v(const Bwd& a) {
-    AttnGeom gq = a.g, gk = a.g;
-    gq.sorted = attn_sorts(a.g, (long long)a.g.Nq * a.g.G, NW * 32);
-    gk.sorted = attn_sorts(a.g, a.g.Nk, 128);
-    const int sq = attn_slots((long long)a.g.Nq * a.g.G, a.g.B, NW == 8 ? 8 : 7), sk = attn_slots(a.g.Nk, a.g.B, 7);
-    if (a.g.Nq)
-        hipLaunchKernelGGL((packed_attn_dq_kernel<T, DP, NW, TK, VEC>), dim3(sq * a.g.Hk), dim3(NW * 64), 0, a.stream, gq, a.q, a.k, a.v, a.o, a.go,
-                           a.lse, (T*)a.dq, a.rowstat, sq);
-    if (a.g.Nk)
-        hipLaunchKernelGGL((packed_attn_dkv_kernel<T, DP, VEC>), dim3(sk * a.g.Hk), dim3(512), 0, a.stream, gk, a.q, a.k, a.v, a.go,
-                           a.rowstat, (T*)a.dk, (T*)a.dv, sk);
+    if (a.g.Nq) {
+        if (TK == 64 && attn_few_blocks(a.g, NW * 32)) launch_dq<T, DP, NW, TK, TK == 64 ? 2 : 1, VEC>(a);
+        else launch_dq<T, DP, NW, TK, 1, VEC>(a);
+    }
+    if (a.g.Nk) {
+        // two pairs per block: as long as two blocks fit a CU's LDS
+        if (DP * sizeof(T) <= 128 && ((long long)a.g.Nk / 128 + a.g.B) * a.g.Hk < 1024) launch_dkv<T, DP, DP * sizeof(T) <= 128 ? 2 : 4, VEC>(a);
+        else launch_dkv<T, DP, 4, VEC>(a);
+    }
 }
 template <typename T, int DP, int NW, int TK> void launch(const Bwd& a) {
     if (a.vec) launch_v<T, DP, NW, TK, true>(a);
