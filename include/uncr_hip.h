@@ -604,12 +604,13 @@ int uncr_packed_attn_fwd(const void* q, long long q_ts, long long q_hs, const vo
                          const int* off_k, const int* k_len, float temperature, int causal, int fill, int max_q, int max_k, float* work,
                          long long work_floats, int B, int Nq, int Nk, int Hq, int Hk, int D, int act, hipStream_t stream);
 /* gradients dq, dk, dv (contiguous; zeros for rows of no sequence and keys behind k_len) from dout, the forward's inputs, out and lse;
- * rowstat: float [2][Nq][Hq] workspace */
+ * rowstat: float [2][Nq][Hq] workspace; work: float [work_floats] of at least uncr_packed_attn_bwd_work(...) floats */
+int uncr_packed_attn_bwd_work(int max_q, int max_k, int B, int Nq, int Nk, int Hq, int Hk, int D, int act);
 int uncr_packed_attn_bwd(const void* q, long long q_ts, long long q_hs, const void* k, long long k_ts, long long k_hs, const void* v,
                          long long v_ts, long long v_hs, const void* out, long long o_ts, long long o_hs, const void* dout, long long do_ts,
                          long long do_hs, const float* lse, void* dq, void* dk, void* dv, float* rowstat, const int* off_q, const int* off_k,
-                         const int* k_len, float temperature, int causal, int max_q, int max_k, int B, int Nq, int Nk, int Hq, int Hk, int D,
-                         int act, hipStream_t stream);
+                         const int* k_len, float temperature, int causal, int max_q, int max_k, float* work, long long work_floats, int B, int Nq,
+                         int Nk, int Hq, int Hk, int D, int act, hipStream_t stream);
 
 #ifdef __cplusplus
 }

@@ -128,19 +128,29 @@ static inline bool attn_sorts(const AttnGeom& g, long long rows, int per_tile) {
 }
 static inline int attn_slots(long long rows, int B, int shift) { return (int)(rows >> shift) + B; }
 
+// fp32 on the bf16 matrix units: x = x0 + x1 + x2 exactly to 24 bits, each rounded to bf16 from what the ones before leave, and
+//   a b = a0 b0 + a0 b1 + a1 b0 + a1 b1 + a0 b2 + a2 b0      (what is left out is below 2^-24 |a b|, a rounding of fp32)
+// -- six products at 16 times the rate of v_mfma_f32_32x32x2_f32.  A launch before lays the inputs out as rows [3][D rounded up to 8]
+// (attn_planes below); P and dS are taken apart in registers.
+struct AttnThree {};
+
 template <typename T> struct AttnElem;
-template <> struct AttnElem<float> { typedef f32x4 Frag; static constexpr int EPC = 4; };
-template <> struct AttnElem<__bf16> { typedef bf16x8 Frag; static constexpr int EPC = 8; };
+template <> struct AttnElem<float> { typedef f32x4 Frag; typedef float In, Out; static constexpr int EPC = 4; static constexpr bool THREE = false; };
+template <> struct AttnElem<__bf16> { typedef bf16x8 Frag; typedef __bf16 In, Out; static constexpr int EPC = 8; static constexpr bool THREE = false; };
+template <> struct AttnElem<AttnThree> { typedef bf16x8 Frag; typedef __bf16 In; typedef float Out; static constexpr int EPC = 8; static constexpr bool THREE = true; };
 
 template <typename T, int DP> struct AttnTile {
     typedef typename AttnElem<T>::Frag Frag;
+    typedef typename AttnElem<T>::In In;
+    static constexpr bool THREE = AttnElem<T>::THREE;
     static constexpr int EPC = AttnElem<T>::EPC;          // elements per 16-byte chunk
-    static constexpr int NCH = DP / EPC;                  // chunks per row
-    static constexpr int RB = NCH * 16;                   // bytes per row
+    static constexpr int NCH = DP / EPC;                  // chunks per row (and part)
+    static constexpr int CPR = THREE ? 3 * NCH : NCH;     // chunks of a row in LDS
+    static constexpr int RB = CPR * 16;                   // bytes per row
     static constexpr int KS = NCH / 2;                    // operand steps over DP: a step is one chunk of each lane half
     // waves per SIMD the kernels are compiled for: no more registers than 512 / WAVES, so that the accumulators stay where vector
     // instructions reach them (the compiler moves them to and fro otherwise)
-    static constexpr int WAVES = RB <= 128 ? 3 : RB <= 256 ? 2 : 1;
+    static constexpr int WAVES = THREE ? (DP <= 32 ? 3 : 2) : RB <= 128 ? 3 : RB <= 256 ? 2 : 1;
     static constexpr int DB = DP < 32 ? 1 : DP / 32;      // 32-wide blocks of DP (DP = 16: half a block, its other half repeats the first)
 
     static __device__ __forceinline__ int swizzle(int row) {
@@ -149,17 +159,19 @@ template <typename T, int DP> struct AttnTile {
         if (NCH == 4) return (row >> 2) & 3;
         return (row >> 3) & 1;
     }
-    static __device__ __forceinline__ int place(int row, int chunk) { return row * RB + ((chunk ^ swizzle(row)) << 4); }
+    static __device__ __forceinline__ int place(int row, int chunk, int part = 0) { return row * RB + part * NCH * 16 + ((chunk ^ swizzle(row)) << 4); }
 
     // operand A (or B) of step s for row `row` of a tile
-    static __device__ __forceinline__ Frag frag(const char* tile, int row, int s, int h) {
-        return *reinterpret_cast<const Frag*>(tile + place(row, 2 * s + h));
+    static __device__ __forceinline__ Frag frag(const char* tile, int row, int s, int h, int part = 0) {
+        return *reinterpret_cast<const Frag*>(tile + place(row, 2 * s + h, part));
     }
 
     // 16 bytes of a row in global memory, zeros behind D.  VEC: rows start at 16-byte boundaries and D fills whole chunks
-    template <bool VEC> static __device__ __forceinline__ Frag fetch(const T* row, int chunk, int D) {
+    template <bool VEC> static __device__ __forceinline__ Frag fetch(const In* row, int chunk, int D, int part = 0) {
         Frag f = {};
-        if (VEC) {
+        if (THREE) {
+            if (chunk * EPC < D) f = *reinterpret_cast<const Frag*>(row + part * ((D + 7) & ~7) + chunk * EPC);
+        } else if (VEC) {
             if (chunk * EPC < D) f = *reinterpret_cast<const Frag*>(row + chunk * EPC);
         } else {
 #pragma unroll
@@ -168,6 +180,9 @@ template <typename T, int DP> struct AttnTile {
         }
         return f;
     }
+    // what belongs at place c of a tile: chunk and part of row c / CPR
+    static __device__ __forceinline__ int chunk_at(int c) { return (c % CPR % NCH) ^ swizzle(c / CPR); }
+    static __device__ __forceinline__ int part_at(int c) { return c % CPR / NCH; }
 };
 
 // Operands are fetched from LDS in one go and used after it (`attn_fence` keeps the compiler from sinking each read to its use, where
@@ -177,15 +192,29 @@ __device__ __forceinline__ void attn_fence() { __builtin_amdgcn_sched_barrier(0)
 // operand A of a 32-row product: all of a row's chunks this lane half holds
 template <typename T, int DP> struct AttnRows {
     typedef AttnTile<T, DP> L;
-    typename L::Frag f[L::KS];
+    static constexpr int PARTS = L::THREE ? 3 : 1;
+    typename L::Frag f[PARTS][L::KS];
     __device__ __forceinline__ void fetch(const char* tile, int row, int h) {
 #pragma unroll
-        for (int i = 0; i < L::KS; ++i) f[i] = L::frag(tile, row, i, h);
+        for (int p = 0; p < PARTS; ++p)
+#pragma unroll
+            for (int i = 0; i < L::KS; ++i) f[p][i] = L::frag(tile, row, i, h, p);
     }
     // 16 bytes at a time from a row in global memory
-    template <bool VEC> __device__ __forceinline__ void fetch_global(const T* row, int h, int D) {
+    template <bool VEC> __device__ __forceinline__ void fetch_global(const typename L::In* row, int h, int D) {
 #pragma unroll
-        for (int i = 0; i < L::KS; ++i) f[i] = L::template fetch<VEC>(row, 2 * i + h, D);
+        for (int p = 0; p < PARTS; ++p)
+#pragma unroll
+            for (int i = 0; i < L::KS; ++i) f[p][i] = L::template fetch<VEC>(row, 2 * i + h, D, p);
+    }
+    // sum of this half's products with another row
+    __device__ __forceinline__ float dot(const AttnRows& o) const {
+        float d = 0.f;
+#pragma unroll
+        for (int i = 0; i < L::KS; ++i)
+#pragma unroll
+            for (int e = 0; e < L::EPC; ++e) d = fmaf((float)f[0][i][e], (float)o.f[0][i][e], d);
+        return d;
     }
 };
 
@@ -196,11 +225,24 @@ __device__ __forceinline__ void attn_mma(f32x16& acc, const f32x4& a, const f32x
 #pragma unroll
     for (int i = 0; i < 4; ++i) acc = __builtin_amdgcn_mfma_f32_32x32x2f32(a[i], b[i], acc, 0, 0, 0);
 }
+// the six products of two numbers in three parts, small ones first
+__device__ __forceinline__ void attn_mma_three(f32x16& acc, const bf16x8& a0, const bf16x8& a1, const bf16x8& a2, const bf16x8& b0, const bf16x8& b1,
+                                               const bf16x8& b2) {
+    attn_mma(acc, a2, b0);
+    attn_mma(acc, a0, b2);
+    attn_mma(acc, a1, b1);
+    attn_mma(acc, a1, b0);
+    attn_mma(acc, a0, b1);
+    attn_mma(acc, a0, b0);
+}
 // acc (32 rows of A x 32 columns of B) = A * B
 template <typename T, int DP> __device__ __forceinline__ f32x16 attn_product(const AttnRows<T, DP>& a, const AttnRows<T, DP>& b) {
     f32x16 acc = (f32x16)(0.f);
 #pragma unroll
-    for (int i = 0; i < AttnTile<T, DP>::KS; ++i) attn_mma(acc, a.f[i], b.f[i]);
+    for (int i = 0; i < AttnTile<T, DP>::KS; ++i) {
+        if constexpr (AttnTile<T, DP>::THREE) attn_mma_three(acc, a.f[0][i], a.f[1][i], a.f[2][i], b.f[0][i], b.f[1][i], b.f[2][i]);
+        else attn_mma(acc, a.f[0][i], b.f[0][i]);
+    }
     return acc;
 }
 
@@ -221,6 +263,25 @@ template <> struct AttnProb<__bf16> {
 template <> struct AttnProb<float> {
     f32x16 v;
     __device__ __forceinline__ void set(const f32x16& p) { v = p; }
+};
+template <> struct AttnProb<AttnThree> {
+    bf16x8 v[3][2];
+    __device__ __forceinline__ void set(const f32x16& p) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            f32x8 t;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) t[i] = p[8 * u + i];
+#pragma unroll
+            for (int k = 0; k < 3; ++k) {
+                v[k][u] = __builtin_convertvector(t, bf16x8);
+                if (k < 2) {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) t[i] -= (float)v[k][u][i];
+                }
+            }
+        }
+    }
 };
 
 // The C registers of a 32-row product on their way through LDS from one wave to another, lane by lane, conflict-free.  With bf16 storage the
@@ -270,26 +331,40 @@ template <> struct AttnPass<float> {
     __device__ __forceinline__ float get(int i) const { return v[i / 4][i % 4]; }
 };
 
+template <> struct AttnPass<AttnThree> : AttnPass<float> {};
+
 // X^T (32 of DP x 32 rows) from the rows row0 .. row0 + 31 of a tile, in the row order of AttnProb, and acc += X^T * P
 template <typename T, int DP> struct AttnCols;
-template <int DP> struct AttnCols<__bf16, DP> {
-    typedef AttnTile<__bf16, DP> L;
-    bf16x8 f[2];
-    __device__ __forceinline__ void fetch(const char* tile, int row0, int db, int lane) {
-        typedef __attribute__((address_space(3))) s16x4 lds4;
-        const int g = lane >> 4, l = lane & 15;
-        const int chunk = (db * 4 + (g & 1) * 2 + ((l & 3) >> 1)) & (L::NCH - 1), low = (l & 1) * 8;
+// one part of bf16 rows, by transposing reads
+template <typename L> __device__ __forceinline__ void attn_cols(bf16x8 (&f)[2], const char* tile, int row0, int db, int lane, int part) {
+    typedef __attribute__((address_space(3))) s16x4 lds4;
+    const int g = lane >> 4, l = lane & 15;
+    const int chunk = (db * 4 + (g & 1) * 2 + ((l & 3) >> 1)) & (L::NCH - 1), low = (l & 1) * 8;
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            const int row = row0 + 16 * u + 4 * (g >> 1) + (l >> 2);
-            const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(tile + L::place(row, chunk) + low));
-            const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(tile + L::place(row + 8, chunk) + low));
-            f[u] = __builtin_shufflevector(__builtin_bit_cast(bf16x4, a), __builtin_bit_cast(bf16x4, b), 0, 1, 2, 3, 4, 5, 6, 7);
-        }
+    for (int u = 0; u < 2; ++u) {
+        const int row = row0 + 16 * u + 4 * (g >> 1) + (l >> 2);
+        const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(tile + L::place(row, chunk, part) + low));
+        const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(tile + L::place(row + 8, chunk, part) + low));
+        f[u] = __builtin_shufflevector(__builtin_bit_cast(bf16x4, a), __builtin_bit_cast(bf16x4, b), 0, 1, 2, 3, 4, 5, 6, 7);
     }
+}
+template <int DP> struct AttnCols<__bf16, DP> {
+    bf16x8 f[2];
+    __device__ __forceinline__ void fetch(const char* tile, int row0, int db, int lane) { attn_cols<AttnTile<__bf16, DP>>(f, tile, row0, db, lane, 0); }
     __device__ __forceinline__ void mma(f32x16& acc, const AttnProb<__bf16>& p) const {
 #pragma unroll
-        for (int u = 0; u < 2; ++u) acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f[u], p.v[u], acc, 0, 0, 0);
+        for (int u = 0; u < 2; ++u) attn_mma(acc, f[u], p.v[u]);
+    }
+};
+template <int DP> struct AttnCols<AttnThree, DP> {
+    bf16x8 f[3][2];
+    __device__ __forceinline__ void fetch(const char* tile, int row0, int db, int lane) {
+#pragma unroll
+        for (int k = 0; k < 3; ++k) attn_cols<AttnTile<AttnThree, DP>>(f[k], tile, row0, db, lane, k);
+    }
+    __device__ __forceinline__ void mma(f32x16& acc, const AttnProb<AttnThree>& p) const {
+#pragma unroll
+        for (int u = 0; u < 2; ++u) attn_mma_three(acc, f[0][u], f[1][u], f[2][u], p.v[0][u], p.v[1][u], p.v[2][u]);
     }
 };
 template <int DP> struct AttnCols<float, DP> {
@@ -331,32 +406,31 @@ static __device__ const f32x4 attn_zeros = {0.f, 0.f, 0.f, 0.f};      // what ch
 // (NT = 64: a wave's own tile)
 template <typename T, int DP, int ROWS, int NT, bool VEC> struct AttnStage {
     typedef AttnTile<T, DP> L;
-    static constexpr int CNT = (ROWS * L::NCH + NT - 1) / NT;
+    static constexpr int CNT = (ROWS * L::CPR + NT - 1) / NT;
     typename L::Frag f[VEC ? 1 : CNT];
     static __device__ __forceinline__ int me() { return NT == 64 ? threadIdx.x & 63 : threadIdx.x; }
-    static __device__ __forceinline__ bool idle(int c) { return (ROWS * L::NCH) % NT && c >= ROWS * L::NCH; }
-    // the chunk of a row that belongs at place c of the tile
-    static __device__ __forceinline__ int chunk(int c) { return (c % L::NCH) ^ L::swizzle(c / L::NCH); }
-    __device__ __forceinline__ void begin(int i, char* tile, const T* row, int D) {
+    static __device__ __forceinline__ bool idle(int c) { return (ROWS * L::CPR) % NT && c >= ROWS * L::CPR; }
+    __device__ __forceinline__ void begin(int i, char* tile, const typename L::In* row, int D) {
         const int c = me() + i * NT;
         if (idle(c)) return;
         if (VEC) {
-            const T* p = row + chunk(c) * L::EPC;
-            attn_dma16(tile + (c & ~63) * 16, chunk(c) * L::EPC < D ? (const void*)p : (const void*)&attn_zeros);
+            const int e = L::chunk_at(c) * L::EPC;
+            const typename L::In* p = row + e + (L::THREE ? L::part_at(c) * ((D + 7) & ~7) : 0);
+            attn_dma16(tile + (c & ~63) * 16, e < D ? (const void*)p : (const void*)&attn_zeros);
         } else {
-            f[i] = L::template fetch<false>(row, chunk(c), D);
+            f[i] = L::template fetch<false>(row, L::chunk_at(c), D);
         }
     }
     // rows row0 ..: those behind `last` repeat it (their products are masked)
-    __device__ __forceinline__ void begin(char* tile, const T* base, long long ts, int row0, int last, int D) {
+    __device__ __forceinline__ void begin(char* tile, const typename L::In* base, long long ts, int row0, int last, int D) {
 #pragma unroll
-        for (int i = 0; i < CNT; ++i) begin(i, tile, base + (size_t)min(row0 + (me() + i * NT) / L::NCH, last) * ts, D);
+        for (int i = 0; i < CNT; ++i) begin(i, tile, base + (size_t)min(row0 + (me() + i * NT) / L::CPR, last) * ts, D);
     }
     // packed rows: token r / G, head r % G
-    __device__ __forceinline__ void begin_packed(char* tile, const T* base, long long ts, long long hs, int row0, int last, int G, int D) {
+    __device__ __forceinline__ void begin_packed(char* tile, const typename L::In* base, long long ts, long long hs, int row0, int last, int G, int D) {
 #pragma unroll
         for (int i = 0; i < CNT; ++i) {
-            const int r = min(row0 + (me() + i * NT) / L::NCH, last), t = r / G;
+            const int r = min(row0 + (me() + i * NT) / L::CPR, last), t = r / G;
             begin(i, tile, base + (size_t)t * ts + (size_t)(r - t * G) * hs, D);
         }
     }
@@ -491,6 +565,11 @@ __device__ __forceinline__ float attn_inv(float l) { return l > 0.f || l != l ? 
 int attn_geom(AttnGeom& g, const int* off_q, const int* off_k, const int* k_len, float temperature, int causal, int B, int Nq, int Nk, int Hq,
               int Hk, int D, int act);
 bool attn_aligned(const AttnTensor* t, int n, int D, int act);
+// packed_attn_planes.hip: fp32 inputs laid out as rows [3][D rounded up to 8] of bf16 (see AttnThree)
+constexpr int ATTN_MAX_PLANES = 4;
+bool attn_three(const AttnGeom& g, int act, bool vec);
+long long attn_planes_floats(const AttnGeom& g, long long q_like, long long k_like);
+void attn_planes(const AttnGeom& g, const AttnTensor* in, const int* N, const int* H, int n, float* work, AttnTensor* out, hipStream_t stream);
 // packed_attn_rows.hip: kernels whose unit is a wave, for few rows per sequence
 struct AttnSplit { int waves, chunk, splits; };     // waves that share a task, keys per block, blocks per sequence (1: no partial results)
 AttnSplit attn_split(const AttnGeom& g, int max_q, int max_k, int act);

@@ -9,13 +9,15 @@ namespace {
 
 template <typename T, int DP, int NW, int TK, int KSPLIT, bool VEC>
 __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(AttnTile<T, DP>::WAVES))) void packed_attn_fwd_kernel(const AttnGeom g, const AttnTensor q, const AttnTensor k, const AttnTensor v,
-                                                                  T* __restrict__ out, long long o_ts, long long o_hs,
+                                                                  typename AttnElem<T>::Out* __restrict__ out, long long o_ts, long long o_hs,
                                                                   float* __restrict__ lse, int slots) {
     typedef AttnTile<T, DP> L;
+    typedef typename AttnElem<T>::In In;
+    typedef typename AttnElem<T>::Out Out;
     constexpr int NT = NW * 64, GROUPS = NW / KSPLIT, BM = GROUPS * 32, SHIFT = BM == 256 ? 8 : BM == 128 ? 7 : 6;
     __shared__ alignas(16) char lds_k[2][TK * L::RB], lds_v[2][TK * L::RB];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5, col = lane & 31;
-    if (g.fill) attn_fill_outside<T>(g.off_q, g.B, g.Nq, out, o_ts, o_hs, g.Hq, g.D, lse, blockIdx.x, gridDim.x);
+    if (g.fill) attn_fill_outside<Out>(g.off_q, g.B, g.Nq, out, o_ts, o_hs, g.Hq, g.D, lse, blockIdx.x, gridDim.x);
     const int hk = blockIdx.x % g.Hk;
     int b, tile;
     // the last tiles of a causal sequence are the longest: they start first
@@ -33,14 +35,14 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(AttnTil
     const int wave_lo = limit_of(row0), wave_hi = row0 < rows ? limit_of(row0 + 31) : 0, block_hi = limit_of(tile * BM + BM - 1);
 
     AttnRows<T, DP> qf;
-    qf.template fetch_global<VEC>((const T*)q.p + (size_t)(s.q0 + tok) * q.ts + (size_t)head * q.hs, h, g.D);
+    qf.template fetch_global<VEC>((const In*)q.p + (size_t)(s.q0 + tok) * q.ts + (size_t)head * q.hs, h, g.D);
     f32x16 acc[L::DB];
 #pragma unroll
     for (int db = 0; db < L::DB; ++db) acc[db] = (f32x16)(0.f);
     float m = -INFINITY, l = 0.f;
 
-    const T* kb = (const T*)k.p + (size_t)s.k0 * k.ts + (size_t)hk * k.hs;
-    const T* vb = (const T*)v.p + (size_t)s.k0 * v.ts + (size_t)hk * v.hs;
+    const In* kb = (const In*)k.p + (size_t)s.k0 * k.ts + (size_t)hk * k.hs;
+    const In* vb = (const In*)v.p + (size_t)s.k0 * v.ts + (size_t)hk * v.hs;
     constexpr int SUB = TK / 32 / KSPLIT;
     const int tiles = (block_hi + TK - 1) / TK;
     AttnStage<T, DP, TK, NT, VEC> ks, vs;
@@ -141,7 +143,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(AttnTil
     }
     if (row0 + col >= rows) return;
     const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
-    attn_store_row<T, L::DB>(out + (size_t)(s.q0 + tok) * o_ts + (size_t)head * o_hs, acc, inv, h, g.D);
+    attn_store_row<Out, L::DB>(out + (size_t)(s.q0 + tok) * o_ts + (size_t)head * o_hs, acc, inv, h, g.D);
     if (lse && h == 0) lse[(size_t)(s.q0 + tok) * g.Hq + head] = l > 0.f || l != l ? (m + __builtin_amdgcn_logf(l)) * 0.69314718055994531f : -INFINITY;
 }
 
@@ -151,8 +153,10 @@ void launch_k(AttnGeom g, const AttnTensor& q, const AttnTensor& k, const AttnTe
     constexpr int BM = NW / KSPLIT * 32, SHIFT = BM == 256 ? 8 : BM == 128 ? 7 : 6;
     const int slots = attn_slots((long long)g.Nq * g.G, g.B, SHIFT);
     g.sorted = attn_sorts(g, (long long)g.Nq * g.G, BM);
-    if (vec) hipLaunchKernelGGL((packed_attn_fwd_kernel<T, DP, NW, TK, KSPLIT, true>), dim3(slots * g.Hk), dim3(NW * 64), 0, stream, g, q, k, v, (T*)out, o_ts, o_hs, lse, slots);
-    else hipLaunchKernelGGL((packed_attn_fwd_kernel<T, DP, NW, TK, KSPLIT, false>), dim3(slots * g.Hk), dim3(NW * 64), 0, stream, g, q, k, v, (T*)out, o_ts, o_hs, lse, slots);
+    typedef typename AttnElem<T>::Out Out;
+    constexpr bool THREE = AttnElem<T>::THREE;          // always whole vectors
+    if (vec) hipLaunchKernelGGL((packed_attn_fwd_kernel<T, DP, NW, TK, KSPLIT, true>), dim3(slots * g.Hk), dim3(NW * 64), 0, stream, g, q, k, v, (Out*)out, o_ts, o_hs, lse, slots);
+    else hipLaunchKernelGGL((packed_attn_fwd_kernel<T, DP, NW, TK, KSPLIT, THREE>), dim3(slots * g.Hk), dim3(NW * 64), 0, stream, g, q, k, v, (Out*)out, o_ts, o_hs, lse, slots);
 }
 template <typename T, int DP, int NW, int TK>
 void launch(const AttnGeom& g, const AttnTensor& q, const AttnTensor& k, const AttnTensor& v, void* out, long long o_ts, long long o_hs, float* lse,
@@ -191,7 +195,8 @@ extern "C" int uncr_packed_attn_work(int max_q, int max_k, int B, int Nq, int Nk
     static const int none = 0;
     if (attn_geom(g, &none, &none, nullptr, 1.f, 0, B, Nq, Nk, Hq, Hk, D, act) != UNCR_OK) return 0;
     const AttnSplit s = attn_split(g, max_q, max_k, act);
-    return s.waves && s.splits > 1 ? (int)((long long)s.splits * Nq * Hq * (D + 2)) : 0;
+    if (s.waves) return s.splits > 1 ? (int)((long long)s.splits * Nq * Hq * (D + 2)) : 0;
+    return attn_three(g, act, true) ? (int)attn_planes_floats(g, 1, 2) : 0;
 }
 
 extern "C" int uncr_packed_attn_fwd(const void* q, long long q_ts, long long q_hs, const void* k, long long k_ts, long long k_hs, const void* v,
@@ -216,6 +221,13 @@ extern "C" int uncr_packed_attn_fwd(const void* q, long long q_ts, long long q_h
     if (split.waves) {
         if (split.splits > 1 && (!work || work_floats < (long long)split.splits * Nq * Hq * (D + 2))) return UNCR_EINVAL;
         attn_rows_fwd(g, split, tq, tk, tv, out, o_ts, o_hs, lse, work, act, vec, stream);
+    } else if (attn_three(g, act, vec)) {
+        if (!work || work_floats < attn_planes_floats(g, 1, 2)) return UNCR_EINVAL;
+        const int n[3] = {Nq, Nk, Nk}, h[3] = {Hq, Hk, Hk};
+        AttnTensor p[3];
+        attn_planes(g, all, n, h, 3, work, p, stream);
+        if (D <= 32) launch<AttnThree, 32, 4, 64>(g, p[0], p[1], p[2], out, o_ts, o_hs, lse, true, stream);
+        else launch<AttnThree, 64, 4, 32>(g, p[0], p[1], p[2], out, o_ts, o_hs, lse, true, stream);
     } else if (act) {
         if (D <= 32) launch<__bf16, 32, 4, 64>(g, tq, tk, tv, out, o_ts, o_hs, lse, vec, stream);
         else if (D <= 64) launch<__bf16, 64, 4, 64>(g, tq, tk, tv, out, o_ts, o_hs, lse, vec, stream);

@@ -11,13 +11,15 @@ namespace {
 
 template <typename T, int DP, int NW, int TK, int KSPLIT, bool VEC>
 __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(AttnTile<T, DP>::WAVES))) void packed_attn_dq_kernel(const AttnGeom g, const AttnTensor q, const AttnTensor k, const AttnTensor v,
-                                                                 const AttnTensor o, const AttnTensor go, const float* __restrict__ lse,
-                                                                 T* __restrict__ dq, float* __restrict__ rowstat, int slots) {
+                                                                 const AttnTensor o, const AttnTensor go, const AttnTensor go_raw, const float* __restrict__ lse,
+                                                                 typename AttnElem<T>::Out* __restrict__ dq, float* __restrict__ rowstat, int slots) {
     typedef AttnTile<T, DP> L;
+    typedef typename AttnElem<T>::In In;
+    typedef typename AttnElem<T>::Out Out;
     constexpr int NT = NW * 64, GROUPS = NW / KSPLIT, BM = GROUPS * 32, SHIFT = BM == 256 ? 8 : BM == 128 ? 7 : 6;
     __shared__ alignas(16) char lds_k[2][TK * L::RB], lds_v[2][TK * L::RB];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5, col = lane & 31;
-    attn_fill_outside<T>(g.off_q, g.B, g.Nq, dq, (long long)g.Hq * g.D, g.D, g.Hq, g.D, nullptr, blockIdx.x, gridDim.x);
+    attn_fill_outside<Out>(g.off_q, g.B, g.Nq, dq, (long long)g.Hq * g.D, g.D, g.Hq, g.D, nullptr, blockIdx.x, gridDim.x);
     const int hk = blockIdx.x % g.Hk;
     int b, tile;
     if (g.sorted ? !attn_find_sorted<false>(g, BM, blockIdx.x / g.Hk, b, tile)
@@ -33,16 +35,14 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(AttnTil
     const int wave_lo = limit_of(row0), wave_hi = row0 < rows ? limit_of(row0 + 31) : 0, block_hi = limit_of(tile * BM + BM - 1);
 
     AttnRows<T, DP> qf, gf;
-    qf.template fetch_global<VEC>((const T*)q.p + (size_t)(s.q0 + tok) * q.ts + (size_t)head * q.hs, h, g.D);
-    gf.template fetch_global<VEC>((const T*)go.p + (size_t)(s.q0 + tok) * go.ts + (size_t)head * go.hs, h, g.D);
-    float dl = 0.f;
-    {
-        AttnRows<T, DP> of;
-        of.template fetch_global<VEC>((const T*)o.p + (size_t)(s.q0 + tok) * o.ts + (size_t)head * o.hs, h, g.D);
-#pragma unroll
-        for (int i = 0; i < L::KS; ++i)
-#pragma unroll
-            for (int e = 0; e < L::EPC; ++e) dl = fmaf((float)gf.f[i][e], (float)of.f[i][e], dl);
+    qf.template fetch_global<VEC>((const In*)q.p + (size_t)(s.q0 + tok) * q.ts + (size_t)head * q.hs, h, g.D);
+    gf.template fetch_global<VEC>((const In*)go.p + (size_t)(s.q0 + tok) * go.ts + (size_t)head * go.hs, h, g.D);
+    float dl;
+    {           // delta from dOut and Out as they are stored
+        AttnRows<Out, DP> of, gr;
+        of.template fetch_global<VEC>((const Out*)o.p + (size_t)(s.q0 + tok) * o.ts + (size_t)head * o.hs, h, g.D);
+        gr.template fetch_global<VEC>((const Out*)go_raw.p + (size_t)(s.q0 + tok) * go_raw.ts + (size_t)head * go_raw.hs, h, g.D);
+        dl = gr.dot(of);
     }
     dl += attn_other_half(dl);
     const size_t at = (size_t)(s.q0 + tok) * g.Hq + head;
@@ -57,8 +57,8 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(AttnTil
     f32x16 acc[L::DB];
 #pragma unroll
     for (int db = 0; db < L::DB; ++db) acc[db] = (f32x16)(0.f);
-    const T* kb = (const T*)k.p + (size_t)s.k0 * k.ts + (size_t)hk * k.hs;
-    const T* vb = (const T*)v.p + (size_t)s.k0 * v.ts + (size_t)hk * v.hs;
+    const In* kb = (const In*)k.p + (size_t)s.k0 * k.ts + (size_t)hk * k.hs;
+    const In* vb = (const In*)v.p + (size_t)s.k0 * v.ts + (size_t)hk * v.hs;
     const int tiles = (block_hi + TK - 1) / TK;
     AttnStage<T, DP, TK, NT, VEC> ks, vs;
     if (tiles) {
@@ -128,7 +128,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(AttnTil
 #pragma unroll
             for (int i = 0; i < 16; ++i) acc[db][i] += pass[(db * 16 + i) * 64 + lane];
     }
-    if (row0 + col < rows) attn_store_row<T, L::DB>(dq + at * g.D, acc, g.scale, h, g.D);
+    if (row0 + col < rows) attn_store_row<Out, L::DB>(dq + at * g.D, acc, g.scale, h, g.D);
 }
 
 // A block owns 32 keys for each of its pairs of waves.  The first wave of a pair holds its keys' K and the sum dV, the second V and dK:
@@ -139,17 +139,20 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(AttnTil
 template <typename T, int DP, int PAIRS, bool VEC>
 __global__ __launch_bounds__(PAIRS * 128) void packed_attn_dkv_kernel(const AttnGeom g, const AttnTensor q, const AttnTensor k, const AttnTensor v,
                                                               const AttnTensor go, const float* __restrict__ rowstat,
-                                                              T* __restrict__ dk, T* __restrict__ dv, int slots) {
+                                                              typename AttnElem<T>::Out* __restrict__ dk,
+                                                              typename AttnElem<T>::Out* __restrict__ dv, int slots) {
     typedef AttnTile<T, DP> L;
-    constexpr int NT = PAIRS * 128, BN = PAIRS * 32, SHIFT = PAIRS == 4 ? 7 : 6, TQ = sizeof(T) == 2 ? 64 : 32;
+    typedef typename AttnElem<T>::In In;
+    typedef typename AttnElem<T>::Out Out;
+    constexpr int NT = PAIRS * 128, BN = PAIRS * 32, SHIFT = PAIRS == 4 ? 7 : 6, TQ = sizeof(T) == 2 ? 64 : 32;      // AttnThree, fp32: 32
     constexpr bool EARLY = L::RB <= 256;       // registers for the transposed operand beside the first product (not for fp32 rows of 512 bytes)
     __shared__ alignas(16) char lds_q[3][TQ * L::RB], lds_g[3][TQ * L::RB];
     __shared__ f32x4 lds_p[2][PAIRS][TQ / 32][AttnPass<T>::PARTS][64];
     __shared__ alignas(16) float lds_s[3][2][TQ];       // lse in powers of two and delta of a tile's rows
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5, col = lane & 31, pair = wave % PAIRS;
     const bool second = wave >= PAIRS;
-    attn_fill_outside<T>(g.off_k, g.B, g.Nk, dk, (long long)g.Hk * g.D, g.D, g.Hk, g.D, nullptr, blockIdx.x, gridDim.x);
-    attn_fill_outside<T>(g.off_k, g.B, g.Nk, dv, (long long)g.Hk * g.D, g.D, g.Hk, g.D, nullptr, blockIdx.x, gridDim.x);
+    attn_fill_outside<Out>(g.off_k, g.B, g.Nk, dk, (long long)g.Hk * g.D, g.D, g.Hk, g.D, nullptr, blockIdx.x, gridDim.x);
+    attn_fill_outside<Out>(g.off_k, g.B, g.Nk, dv, (long long)g.Hk * g.D, g.D, g.Hk, g.D, nullptr, blockIdx.x, gridDim.x);
     const int hk = blockIdx.x % g.Hk;
     int b, tile;
     // the first keys of a causal sequence are seen by the most rows: they start first
@@ -171,16 +174,16 @@ __global__ __launch_bounds__(PAIRS * 128) void packed_attn_dkv_kernel(const Attn
         AttnRows<T, DP> own;
         {
             const AttnTensor& x = second ? v : k;
-            own.template fetch_global<VEC>((const T*)x.p + (size_t)(s.k0 + min(key, s.lk - 1)) * x.ts + (size_t)hk * x.hs, h, g.D);
+            own.template fetch_global<VEC>((const In*)x.p + (size_t)(s.k0 + min(key, s.lk - 1)) * x.ts + (size_t)hk * x.hs, h, g.D);
         }
-        const T* qb = (const T*)q.p + (size_t)s.q0 * q.ts + (size_t)hk * g.G * q.hs;
-        const T* gb = (const T*)go.p + (size_t)s.q0 * go.ts + (size_t)hk * g.G * go.hs;
+        const In* qb = (const In*)q.p + (size_t)s.q0 * q.ts + (size_t)hk * g.G * q.hs;
+        const In* gb = (const In*)go.p + (size_t)s.q0 * go.ts + (size_t)hk * g.G * go.hs;
         const float* lb = rowstat + (second ? (size_t)g.Nq * g.Hq : 0) + (size_t)s.q0 * g.Hq + hk * g.G;
         // from the last rows to the first: the blocks of a causal sequence then walk over the same rows at the same time, and find them in L2
         auto row_of = [&](int it) { return start + (tiles - 1 - it) * TQ; };
         typedef AttnStage<T, DP, TQ, NT, VEC> Stage;
         Stage qs, gs;
-        AttnCursor<const T> cq[Stage::CNT], cg[Stage::CNT];
+        AttnCursor<const In> cq[Stage::CNT], cg[Stage::CNT];
         AttnCursor<const float> cl;
         // lse (first waves) and delta (second waves) of the tile's rows go to LDS in equal shares
         constexpr int SHARE = TQ / PAIRS;
@@ -189,7 +192,7 @@ __global__ __launch_bounds__(PAIRS * 128) void packed_attn_dkv_kernel(const Attn
         // the first tile repeats the last row behind it, and masks it
 #pragma unroll
         for (int i = 0; i < Stage::CNT; ++i) {
-            const int r = row_of(0) + min((int)(threadIdx.x + i * NT) / L::NCH, TQ - 1);
+            const int r = row_of(0) + min((int)(threadIdx.x + i * NT) / L::CPR, TQ - 1);
             const int t = min(r, rows - 1) / g.G, hd = min(r, rows - 1) - t * g.G;
             qs.begin(i, lds_q[0], qb + (size_t)t * q.ts + (size_t)hd * q.hs, g.D);
             gs.begin(i, lds_g[0], gb + (size_t)t * go.ts + (size_t)hd * go.hs, g.D);
@@ -303,12 +306,12 @@ __global__ __launch_bounds__(PAIRS * 128) void packed_attn_dkv_kernel(const Attn
     if (key >= s.lk)
 #pragma unroll
         for (int db = 0; db < L::DB; ++db) acc[db] = (f32x16)(0.f);
-    attn_store_row<T, L::DB>((second ? dk : dv) + ((size_t)(s.k0 + key) * g.Hk + hk) * g.D, acc, second ? g.scale : 1.f, h, g.D);
+    attn_store_row<Out, L::DB>((second ? dk : dv) + ((size_t)(s.k0 + key) * g.Hk + hk) * g.D, acc, second ? g.scale : 1.f, h, g.D);
 }
 
 struct Bwd {
     AttnGeom g;
-    AttnTensor q, k, v, o, go;
+    AttnTensor q, k, v, o, go, go_raw;          // go_raw: dOut as it came, where go is its parts
     const float* lse;
     void *dq, *dk, *dv;
     float* rowstat;
@@ -322,14 +325,14 @@ template <typename T, int DP, int NW, int TK, int KSPLIT, bool VEC> void launch_
     g.sorted = attn_sorts(g, (long long)g.Nq * g.G, BM);
     const int slots = attn_slots((long long)g.Nq * g.G, g.B, SHIFT);
     hipLaunchKernelGGL((packed_attn_dq_kernel<T, DP, NW, TK, KSPLIT, VEC>), dim3(slots * g.Hk), dim3(NW * 64), 0, a.stream, g, a.q, a.k, a.v, a.o, a.go,
-                       a.lse, (T*)a.dq, a.rowstat, slots);
+                       a.go_raw, a.lse, (typename AttnElem<T>::Out*)a.dq, a.rowstat, slots);
 }
 template <typename T, int DP, int PAIRS, bool VEC> void launch_dkv(const Bwd& a) {
     AttnGeom g = a.g;
     g.sorted = attn_sorts(g, g.Nk, PAIRS * 32);
     const int slots = attn_slots(g.Nk, g.B, PAIRS == 4 ? 7 : 6);
     hipLaunchKernelGGL((packed_attn_dkv_kernel<T, DP, PAIRS, VEC>), dim3(slots * g.Hk), dim3(PAIRS * 128), 0, a.stream, g, a.q, a.k, a.v, a.go, a.rowstat,
-                       (T*)a.dk, (T*)a.dv, slots);
+                       (typename AttnElem<T>::Out*)a.dk, (typename AttnElem<T>::Out*)a.dv, slots);
 }
 template <typename T, int DP, int NW, int TK, bool VEC> void launch_v(const Bwd& a) {
     if (a.g.Nq) {
@@ -338,22 +341,31 @@ template <typename T, int DP, int NW, int TK, bool VEC> void launch_v(const Bwd&
     }
     if (a.g.Nk) {
         // two pairs per block: as long as two blocks fit a CU's LDS
-        if (DP * sizeof(T) <= 128 && ((long long)a.g.Nk / 128 + a.g.B) * a.g.Hk < 1024) launch_dkv<T, DP, DP * sizeof(T) <= 128 ? 2 : 4, VEC>(a);
+        constexpr bool SMALL = AttnTile<T, DP>::RB <= (AttnElem<T>::THREE ? 192 : 128);
+        if (SMALL && ((long long)a.g.Nk / 128 + a.g.B) * a.g.Hk < 1024) launch_dkv<T, DP, SMALL ? 2 : 4, VEC>(a);
         else launch_dkv<T, DP, 4, VEC>(a);
     }
 }
 template <typename T, int DP, int NW, int TK> void launch(const Bwd& a) {
     if (a.vec) launch_v<T, DP, NW, TK, true>(a);
-    else launch_v<T, DP, NW, TK, false>(a);
+    else launch_v<T, DP, NW, TK, AttnElem<T>::THREE>(a);
 }
 
 }  // namespace
+
+extern "C" int uncr_packed_attn_bwd_work(int max_q, int max_k, int B, int Nq, int Nk, int Hq, int Hk, int D, int act) {
+    AttnGeom g;
+    static const int none = 0;
+    if (attn_geom(g, &none, &none, nullptr, 1.f, 0, B, Nq, Nk, Hq, Hk, D, act) != UNCR_OK || attn_short(g, max_q, max_k)) return 0;
+    return attn_three(g, act, true) ? (int)attn_planes_floats(g, 2, 2) : 0;
+}
 
 extern "C" int uncr_packed_attn_bwd(const void* q, long long q_ts, long long q_hs, const void* k, long long k_ts, long long k_hs, const void* v,
                                     long long v_ts, long long v_hs, const void* out, long long o_ts, long long o_hs, const void* dout,
                                     long long do_ts, long long do_hs, const float* lse, void* dq, void* dk, void* dv, float* rowstat,
                                     const int* off_q, const int* off_k, const int* k_len, float temperature, int causal, int max_q,
-                                    int max_k, int B, int Nq, int Nk, int Hq, int Hk, int D, int act, hipStream_t stream) {
+                                    int max_k, float* work, long long work_floats, int B, int Nq, int Nk, int Hq, int Hk, int D, int act,
+                                    hipStream_t stream) {
     Bwd a;
     const int rc = attn_geom(a.g, off_q, off_k, k_len, temperature, causal, B, Nq, Nk, Hq, Hk, D, act);
     if (rc != UNCR_OK) return rc;
@@ -363,13 +375,22 @@ extern "C" int uncr_packed_attn_bwd(const void* q, long long q_ts, long long q_h
         const uintptr_t align = (act ? 2 : 4) * 4;
         if ((uintptr_t)dq % align || (uintptr_t)dk % align || (uintptr_t)dv % align) return UNCR_EINVAL;
     }
-    a.q = {q, q_ts, q_hs}; a.k = {k, k_ts, k_hs}; a.v = {v, v_ts, v_hs}; a.o = {out, o_ts, o_hs}; a.go = {dout, do_ts, do_hs};
+    a.q = {q, q_ts, q_hs}; a.k = {k, k_ts, k_hs}; a.v = {v, v_ts, v_hs}; a.o = {out, o_ts, o_hs}; a.go = a.go_raw = {dout, do_ts, do_hs};
     a.lse = lse; a.dq = dq; a.dk = dk; a.dv = dv; a.rowstat = rowstat; a.stream = stream;
     const AttnTensor all[] = {a.q, a.k, a.v, a.o, a.go};
     a.vec = attn_aligned(all, 5, D, act);
     if (Nq == 0 && Nk == 0) return UNCR_OK;
     if (attn_short(a.g, max_q, max_k)) {
         attn_short_bwd(a.g, a.q, a.k, a.v, a.o, a.go, lse, dq, dk, dv, act, a.vec, stream);
+    } else if (attn_three(a.g, act, a.vec)) {
+        if (!work || work_floats < attn_planes_floats(a.g, 2, 2)) return UNCR_EINVAL;
+        const AttnTensor in[4] = {a.q, a.k, a.v, a.go};
+        const int n[4] = {Nq, Nk, Nk, Nq}, h[4] = {Hq, Hk, Hk, Hq};
+        AttnTensor p[4];
+        attn_planes(a.g, in, n, h, 4, work, p, stream);
+        a.q = p[0]; a.k = p[1]; a.v = p[2]; a.go = p[3];
+        if (D <= 32) launch<AttnThree, 32, 4, 64>(a);
+        else launch<AttnThree, 64, 4, 32>(a);
     } else if (act) {
         if (D <= 32) launch<__bf16, 32, 4, 64>(a);
         else if (D <= 64) launch<__bf16, 64, 4, 64>(a);

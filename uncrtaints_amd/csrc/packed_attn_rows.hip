@@ -15,12 +15,14 @@ __global__ __launch_bounds__(NW * 64) void packed_attn_rows_kernel(const AttnGeo
                                                                    T* __restrict__ out, long long o_ts, long long o_hs, float* __restrict__ lse,
                                                                    float* __restrict__ work, int chunk, int splits, int tasks) {
     typedef AttnTile<T, DP> L;
+    typedef typename AttnElem<T>::In In;
+    typedef typename AttnElem<T>::Out Out;
     typedef AttnStage<T, DP, 32, 64, VEC> Stage;
     constexpr int NBUF = SHARE ? 2 : 1, TILE = 32 * L::RB;
     __shared__ alignas(16) char lds[NW][NBUF][2][TILE];
     __shared__ float lds_m[NW][32], lds_l[NW][32];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5, col = lane & 31;
-    if (g.fill) attn_fill_outside<T>(g.off_q, g.B, g.Nq, out, o_ts, o_hs, g.Hq, g.D, lse, blockIdx.x, gridDim.x);
+    if (g.fill) attn_fill_outside<Out>(g.off_q, g.B, g.Nq, out, o_ts, o_hs, g.Hq, g.D, lse, blockIdx.x, gridDim.x);
     const int task = SHARE ? blockIdx.x : blockIdx.x * NW + wave;
     if (task >= tasks) return;
     const int hk = task % g.Hk, split = SHARE ? task / g.Hk % splits : 0, slot = SHARE ? task / g.Hk / splits : task / g.Hk;
@@ -38,11 +40,11 @@ __global__ __launch_bounds__(NW * 64) void packed_attn_rows_kernel(const AttnGeo
     const int begin = split * range, end = min(hi, begin + range);
 
     AttnRows<T, DP> qf;
-    qf.template fetch_global<VEC>((const T*)q.p + (size_t)(s.q0 + tok) * q.ts + (size_t)head * q.hs, h, g.D);
+    qf.template fetch_global<VEC>((const In*)q.p + (size_t)(s.q0 + tok) * q.ts + (size_t)head * q.hs, h, g.D);
     AttnRun<T, DP> run;
     run.reset();
-    const T* kb = (const T*)k.p + (size_t)s.k0 * k.ts + (size_t)hk * k.hs;
-    const T* vb = (const T*)v.p + (size_t)s.k0 * v.ts + (size_t)hk * v.hs;
+    const In* kb = (const In*)k.p + (size_t)s.k0 * k.ts + (size_t)hk * k.hs;
+    const In* vb = (const In*)v.p + (size_t)s.k0 * v.ts + (size_t)hk * v.hs;
     Stage ks, vs;
     constexpr int STEP = SHARE ? NW * 32 : 32;
     int j0 = begin + (SHARE ? wave * 32 : 0), buf = 0;
@@ -78,7 +80,7 @@ __global__ __launch_bounds__(NW * 64) void packed_attn_rows_kernel(const AttnGeo
     float l = run.l + attn_other_half(run.l), m = run.m;
     if (!SHARE) {
         if (row0 + col >= rows) return;
-        attn_store_row<T, L::DB>(out + (size_t)(s.q0 + tok) * o_ts + (size_t)head * o_hs, run.acc, attn_inv(l), h, g.D);
+        attn_store_row<Out, L::DB>(out + (size_t)(s.q0 + tok) * o_ts + (size_t)head * o_hs, run.acc, attn_inv(l), h, g.D);
         if (lse && h == 0) lse[(size_t)(s.q0 + tok) * g.Hq + head] = attn_lse(m, l);
         return;
     }
@@ -212,24 +214,26 @@ __global__ __launch_bounds__(NW * 64) void packed_attn_short_bwd_kernel(const At
                                                                         const AttnTensor o, const AttnTensor go, const float* __restrict__ lse,
                                                                         T* __restrict__ dq, T* __restrict__ dk, T* __restrict__ dv) {
     typedef AttnTile<T, DP> L;
+    typedef typename AttnElem<T>::In In;
+    typedef typename AttnElem<T>::Out Out;
     typedef AttnStage<T, DP, 32, 64, VEC> Stage;
     constexpr int TILE = 32 * L::RB, PS = 36;
     __shared__ alignas(16) char lds[NW][4][TILE];
     __shared__ alignas(16) float patch[NW][32 * PS];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5, col = lane & 31;
-    attn_fill_outside<T>(g.off_q, g.B, g.Nq, dq, (long long)g.Hq * g.D, g.D, g.Hq, g.D, nullptr, blockIdx.x, gridDim.x);
-    attn_fill_outside<T>(g.off_k, g.B, g.Nk, dk, (long long)g.Hk * g.D, g.D, g.Hk, g.D, nullptr, blockIdx.x, gridDim.x);
-    attn_fill_outside<T>(g.off_k, g.B, g.Nk, dv, (long long)g.Hk * g.D, g.D, g.Hk, g.D, nullptr, blockIdx.x, gridDim.x);
+    attn_fill_outside<Out>(g.off_q, g.B, g.Nq, dq, (long long)g.Hq * g.D, g.D, g.Hq, g.D, nullptr, blockIdx.x, gridDim.x);
+    attn_fill_outside<Out>(g.off_k, g.B, g.Nk, dk, (long long)g.Hk * g.D, g.D, g.Hk, g.D, nullptr, blockIdx.x, gridDim.x);
+    attn_fill_outside<Out>(g.off_k, g.B, g.Nk, dv, (long long)g.Hk * g.D, g.D, g.Hk, g.D, nullptr, blockIdx.x, gridDim.x);
     const int task = blockIdx.x * NW + wave, b = task / g.Hk, hk = task - b * g.Hk;
     if (b >= g.B) return;
     const AttnSeq s = attn_seq(g, b);
     const int rows = s.lq * g.G, shift = s.lk - s.lq;
     char *tk = lds[wave][0], *tv = lds[wave][1], *tq = lds[wave][2], *tg = lds[wave][3];
     float* pt = patch[wave];
-    const T* kb = (const T*)k.p + (size_t)s.k0 * k.ts + (size_t)hk * k.hs;
-    const T* vb = (const T*)v.p + (size_t)s.k0 * v.ts + (size_t)hk * v.hs;
-    const T* qb = (const T*)q.p + (size_t)s.q0 * q.ts + (size_t)hk * g.G * q.hs;
-    const T* gb = (const T*)go.p + (size_t)s.q0 * go.ts + (size_t)hk * g.G * go.hs;
+    const In* kb = (const In*)k.p + (size_t)s.k0 * k.ts + (size_t)hk * k.hs;
+    const In* vb = (const In*)v.p + (size_t)s.k0 * v.ts + (size_t)hk * v.hs;
+    const In* qb = (const In*)q.p + (size_t)s.q0 * q.ts + (size_t)hk * g.G * q.hs;
+    const In* gb = (const In*)go.p + (size_t)s.q0 * go.ts + (size_t)hk * g.G * go.hs;
     Stage s0, s1;
     auto load_keys = [&](int j0) {
         attn_own_lds();
@@ -247,7 +251,7 @@ __global__ __launch_bounds__(NW * 64) void packed_attn_short_bwd_kernel(const At
         const int row = min(r0 + col, rows - 1), t = row / g.G, hd = hk * g.G + row - t * g.G;
         at = (size_t)(s.q0 + t) * g.Hq + hd;
         AttnRows<T, DP> of;
-        of.template fetch_global<VEC>((const T*)o.p + (size_t)(s.q0 + t) * o.ts + (size_t)hd * o.hs, h, g.D);
+        of.template fetch_global<VEC>((const In*)o.p + (size_t)(s.q0 + t) * o.ts + (size_t)hd * o.hs, h, g.D);
         ls = lse[at] * 1.4426950408889634f;
         if (ls == -INFINITY || r0 + col >= rows) ls = INFINITY;      // a row that saw nothing, a row behind the last: no probabilities
         s0.finish(tq);
@@ -256,11 +260,7 @@ __global__ __launch_bounds__(NW * 64) void packed_attn_short_bwd_kernel(const At
         attn_own_lds();
         AttnRows<T, DP> gf;
         gf.fetch(tg, col, h);
-        dl = 0.f;
-#pragma unroll
-        for (int i = 0; i < L::KS; ++i)
-#pragma unroll
-            for (int e = 0; e < L::EPC; ++e) dl = fmaf((float)gf.f[i][e], (float)of.f[i][e], dl);
+        dl = gf.dot(of);
         dl += attn_other_half(dl);
     };
     f32x16 p, ds;
@@ -299,7 +299,7 @@ __global__ __launch_bounds__(NW * 64) void packed_attn_short_bwd_kernel(const At
         }
     };
     auto store_dq = [&](int r0, const f32x16 (&a)[L::DB]) {
-        if (r0 + col < rows) attn_store_row<T, L::DB>(dq + at * g.D, a, g.scale, h, g.D);
+        if (r0 + col < rows) attn_store_row<Out, L::DB>(dq + at * g.D, a, g.scale, h, g.D);
     };
     const bool single = s.lk <= 32;
     for (int j0 = 0; j0 < s.room; j0 += 32) {
@@ -342,8 +342,8 @@ __global__ __launch_bounds__(NW * 64) void packed_attn_short_bwd_kernel(const At
 #pragma unroll
                 for (int db = 0; db < L::DB; ++db) ak[db] = av[db] = (f32x16)(0.f);
             const size_t ka = ((size_t)(s.k0 + j0 + col) * g.Hk + hk) * g.D;
-            attn_store_row<T, L::DB>(dk + ka, ak, g.scale, h, g.D);
-            attn_store_row<T, L::DB>(dv + ka, av, 1.f, h, g.D);
+            attn_store_row<Out, L::DB>(dk + ka, ak, g.scale, h, g.D);
+            attn_store_row<Out, L::DB>(dv + ka, av, 1.f, h, g.D);
         }
     }
     if (single && s.lk > 0) return;

@@ -2278,10 +2278,13 @@ def packed_attention_backward(dout: Tensor, q: Tensor, k: Tensor, v: Tensor, out
         dq = torch.empty((Nq, Hq, D), device=q.device, dtype=q.dtype)
         dk, dv = torch.empty((Nk, Hk, D), device=q.device, dtype=q.dtype), torch.empty((Nk, Hk, D), device=q.device, dtype=q.dtype)
         rowstat = _f32((2, Nq, Hq), q.device)
+        B = off_q.numel() - 1
+        n_work = hb.query("uncr_packed_attn_bwd_work", max_q, max_k, B, Nq, Nk, Hq, Hk, D, _dt(q))
+        work = _f32((n_work,), q.device) if n_work else None
         hb.call("uncr_packed_attn_bwd", q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(),
                 v.stride(0), v.stride(1), out.data_ptr(), out.stride(0), out.stride(1), dout.data_ptr(), dout.stride(0), dout.stride(1),
                 lse, dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), rowstat, off_q, off_k, k_len, float(temperature), int(causal),
-                max_q, max_k, off_q.numel() - 1, Nq, Nk, Hq, Hk, D, _dt(q), _stream())
+                max_q, max_k, work, n_work, B, Nq, Nk, Hq, Hk, D, _dt(q), _stream())
     return dq, dk, dv
 
 
