@@ -218,6 +218,77 @@ def test_long_causal_sequences_of_very_different_lengths(hq, hk, dtype):
 
 @gpu
 @BOTH
+@pytest.mark.parametrize("lq,lk,hq,hk,d,bad", [([200], [200], 4, 2, 64, 150), ([700, 40], [700, 40], 2, 2, 32, 650), ([300], [300], 6, 2, 128, 3),
+                                               ([5, 9], [100, 12], 4, 2, 40, 97), ([3], [3000], 2, 1, 20, 2998), ([20], [20], 2, 2, 16, 7)])
+@pytest.mark.parametrize("value", [math.inf, -math.inf, math.nan])
+def test_later_keys_that_are_not_finite_leave_no_trace_in_earlier_rows(lq, lk, hq, hk, d, bad, value, dtype):
+    """One key and value of the first sequence is not finite: rows in front of it are what they are without it, bit for bit where nothing has to be
+    made again, and within both results' roundings otherwise: h |out| for each store, fp32 sums of n terms, and with bf16 the rounding of P to
+    bf16 in the products (it is not rounded where sums are made again): sum_j h p_j |v_j| <= h max|v| because sum p = 1.  (This last term was
+    missing at first: fp32 passed, bf16 differed by 4.9e-4 where h max|v| = 1.6e-2.)  Rows that see an infinite value are infinite."""
+    from uncrtaints_amd.src.backbones.packed_attention import PackedAttention, pack_offsets
+    q, k, v = (torch.randn(n, h, d, generator=_gen(n + h)).to(dtype).to(DEV) for n, h in ((sum(lq), hq), (sum(lk), hk), (sum(lk), hk)))
+    off_q, off_k = pack_offsets(lq, DEV), pack_offsets(lk, DEV)
+    m = PackedAttention(causal=True)
+    for hints in ({}, dict(max_q=max(lq), max_k=max(lk))):
+        clean = m(q, k, v, off_q, off_k, **hints).double()
+        k2, v2 = k.clone(), v.clone()
+        v2[bad, :, ::3] = value
+        out = m(q, k, v2, off_q, off_k, **hints).double()
+        first = bad - (lk[0] - lq[0])                       # the first row that sees the key
+        n = (max(lk) * U * 4 + (_half_step(dtype) if dtype == torch.bfloat16 else 0.0)) * float(v.double().abs().max())
+        for rows in (slice(0, max(first, 0)), slice(lq[0], sum(lq))):
+            assert torch.isfinite(out[rows]).all()
+            err = (out[rows] - clean[rows]).abs()
+            assert (err <= n + 2 * _half_step(dtype) * clean[rows].abs()).all()
+        seen = out[max(first, 0):lq[0], :, ::3]
+        assert (seen.isnan() if math.isnan(value) else (seen == value) | seen.isnan()).all()
+        k2[bad] = value
+        out = m(q, k2, v2, off_q, off_k, **hints)
+        assert torch.isfinite(out[:max(first, 0)]).all() and torch.isfinite(out[lq[0]:]).all()
+
+
+def _half_step(dtype):
+    return torch.finfo(dtype).eps / 2
+
+
+@gpu
+def test_caches_of_more_than_2_to_the_31_elements():
+    """Rows that lie beyond 2^31 elements (and 2^32 bytes) of a cache; the rest of it is never touched."""
+    from uncrtaints_amd.src.backbones.packed_attention import PackedAttention
+    tokens, kv, d = 2_200_000, 8, 128
+    k, v = (torch.empty(tokens, kv, d, dtype=torch.bfloat16, device=DEV) for _ in range(2))
+    small = [torch.randn(300, kv, d, generator=_gen(i)).to(torch.bfloat16).to(DEV) for i in range(2)]
+    k[-300:], v[-300:] = small
+    off_k = torch.tensor([tokens - 300, tokens - 40, tokens], dtype=torch.int32, device=DEV)
+    near = torch.tensor([0, 260, 300], dtype=torch.int32, device=DEV)
+    m = PackedAttention(causal=True)
+    for lq in ([1, 1], [30, 17], [260, 40]):
+        off_q = torch.tensor([0, lq[0], sum(lq)], dtype=torch.int32, device=DEV)
+        q = torch.randn(sum(lq), 16, d, generator=_gen(9)).to(torch.bfloat16).to(DEV)
+        hints = dict(max_q=max(lq), max_k=260)
+        assert torch.equal(m(q, k, v, off_q, off_k, **hints), m(q, *small, off_q, near, **hints))
+
+
+@gpu
+@BOTH
+def test_no_keys_and_no_queries(dtype):
+    from uncrtaints_amd.src.backbones.packed_attention import PackedAttention
+    m = PackedAttention(causal=True)
+    q, none = torch.randn(6, 4, 16, device=DEV).to(dtype).requires_grad_(), torch.empty(0, 2, 16, device=DEV, dtype=dtype, requires_grad=True)
+    off, zero = torch.tensor([0, 6], dtype=torch.int32, device=DEV), torch.zeros(2, dtype=torch.int32, device=DEV)
+    out, lse = m(q, none, none, off, zero, return_lse=True)
+    dq, dk = torch.autograd.grad(out, (q, none), torch.ones_like(out))
+    assert (out == 0).all() and torch.isinf(lse).all() and (dq == 0).all() and dk.shape == none.shape
+    kv = torch.randn(6, 2, 16, device=DEV).to(dtype).requires_grad_()
+    empty = torch.empty(0, 4, 16, device=DEV, dtype=dtype, requires_grad=True)
+    out = m(empty, kv, kv, zero, off)
+    assert out.shape == empty.shape
+    assert (torch.autograd.grad(out, kv, torch.empty_like(out))[0] == 0).all()
+
+
+@gpu
+@BOTH
 def test_large_scores_and_a_temperature(dtype):
     """Scores of +-several hundred: the running maximum is passed by many powers of two from tile to tile."""
     _run([300], [300], 2, 2, 64, True, dtype, scale=40.0, temperature=2.0)
@@ -454,6 +525,9 @@ def test_packed_attention_refuses_on_the_gpu():
         m(q, q, q, off, out=torch.empty(6, 4, 16, device=DEV)[..., :8])
     with pytest.raises(RuntimeError, match="but q is"):
         m(q, q, q, off, out=torch.empty_like(q, dtype=torch.bfloat16))
+    z = torch.zeros(12, 4, 8, device=DEV)
+    with pytest.raises(ValueError, match="shares"):
+        m(q, z[:6], z[6:], off, out=z[6:])
 
 
 def test_entry_points_refuse_bad_sizes():

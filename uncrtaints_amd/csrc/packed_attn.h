@@ -489,6 +489,52 @@ template <typename T, int DB> __device__ __forceinline__ void attn_store_row(T* 
 
 __device__ __forceinline__ float attn_other_half(float x) { return __shfl_xor(x, 32); }
 
+// Infinities and NaN behind the causal edge.  A probability of 0 times one of them is NaN, and on the edge's tiles a product has rows that see
+// a key beside rows that do not.  Values of those tiles are looked at (attn_odd), and a wave that finds one makes its sums again, key by key,
+// with the keys a row does not see left out: `c`, `m` and `l` stay, the scores were masked before anything was made of them.
+template <typename T, int DP> __device__ __forceinline__ bool attn_odd(const char* tile, int row0, int lane) {
+    typedef AttnTile<T, DP> L;
+    bool odd = false;
+#pragma unroll
+    for (int i = 0; i < L::NCH / 2; ++i) {
+        const typename L::Frag f = L::frag(tile, row0 + (lane & 31), i, lane >> 5);
+#pragma unroll
+        for (int e = 0; e < L::EPC; ++e) odd |= !(fabsf((float)f[e]) <= 3.4028234664e38f);
+    }
+    return odd;
+}
+template <typename T> __device__ __forceinline__ float attn_element(const typename AttnElem<T>::In* row, int d, int D) {
+    float x = (float)row[d];
+    if (AttnElem<T>::THREE) x += (float)row[((D + 7) & ~7) + d] + (float)row[2 * ((D + 7) & ~7) + d];
+    return x;
+}
+// keys first, first + 1, ... + 31, first + step, ... below `end`
+template <typename T, int DP, int DB>
+__device__ __forceinline__ void attn_redo(const typename AttnElem<T>::In* q, const typename AttnElem<T>::In* kb, long long k_ts,
+                                          const typename AttnElem<T>::In* vb, long long v_ts, f32x16 (&acc)[DB], int D, float c, float m, int limit,
+                                          int first, int step, int end, int lane) {
+    const int h = lane >> 5;
+    const float ref = m == -INFINITY ? 0.f : m;
+#pragma unroll
+    for (int db = 0; db < DB; ++db) acc[db] = (f32x16)(0.f);
+    for (int j0 = first; j0 < end; j0 += step)
+        for (int j = j0; j < min(j0 + 32, end); ++j) {
+            const typename AttnElem<T>::In *kr = kb + (size_t)j * k_ts, *vr = vb + (size_t)j * v_ts;
+            float s = 0.f;
+            for (int d = h; d < D; d += 2) s = fmaf(attn_element<T>(q, d, D), attn_element<T>(kr, d, D), s);
+            s += attn_other_half(s);
+            if (j >= limit) continue;
+            const float p = __builtin_amdgcn_exp2f(fmaf(s, c, -ref));
+#pragma unroll
+            for (int db = 0; db < DB; ++db)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const int d = db * 32 + 8 * (i / 4) + 4 * h + i % 4;
+                    if (d < D) acc[db][i] = fmaf(p, attn_element<T>(vr, d, D), acc[db][i]);
+                }
+        }
+}
+
 // Rows of the tensor that belong to no sequence, [0, first) and [behind, N), shared out over the grid: `width` zeros each (and -inf in `lse`)
 template <typename T> __device__ __forceinline__ void attn_fill_outside(const int* off, int B, int N, T* out, long long ts, long long hs, int H,
                                                                         int D, float* lse, int block, int blocks) {
@@ -507,7 +553,9 @@ template <typename T, int DP> struct AttnRun {
     typedef AttnTile<T, DP> L;
     f32x16 acc[L::DB];
     float m, l;
+    bool odd;
     __device__ __forceinline__ void reset() {
+        odd = false;
 #pragma unroll
         for (int db = 0; db < L::DB; ++db) acc[db] = (f32x16)(0.f);
         m = -INFINITY;
@@ -525,7 +573,8 @@ template <typename T, int DP> struct AttnRun {
         }
     }
     // keys j0 .. j0 + 31 of which those below `limit` are this lane's row's
-    __device__ __forceinline__ void tile(const char* tk, const char* tv, const AttnRows<T, DP>& q, float c, int j0, int limit, bool edge, int lane) {
+    __device__ __forceinline__ void tile(const char* tk, const char* tv, const AttnRows<T, DP>& q, float c, int j0, int limit, bool edge, bool causal,
+                                         int lane) {
         const int col = lane & 31, h = lane >> 5;
         AttnRows<T, DP> k;
         k.fetch(tk, col, h);
@@ -535,6 +584,7 @@ template <typename T, int DP> struct AttnRun {
 #pragma unroll
             for (int i = 0; i < 16; ++i)
                 if (j0 + 8 * (i / 4) + 4 * h + i % 4 >= limit) s[i] = -INFINITY;
+            if (causal) odd |= attn_odd<T, DP>(tv, 0, lane);
         }
         float mx = s[0];
 #pragma unroll

@@ -26,7 +26,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(AttnTil
     const AttnSeq s = attn_seq(g, b);
     const int rows = s.lq * g.G;
     if (tile * BM >= rows) return;
-    const int row0 = tile * BM + wave % GROUPS * 32, share = wave / GROUPS;      // KSPLIT waves have the same rows and every KSPLIT-th 32 keys
+    const int row0 = tile * BM + wave % GROUPS * 32, share = KSPLIT == 1 ? 0 : wave / GROUPS;      // KSPLIT waves have the same rows and every KSPLIT-th 32 keys
     const int row = min(row0 + col, rows - 1), tok = row / g.G, head = hk * g.G + row - tok * g.G;
     // keys [0, limit) are visible to this lane's row
     const int shift = s.lk - s.lq;
@@ -40,6 +40,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(AttnTil
 #pragma unroll
     for (int db = 0; db < L::DB; ++db) acc[db] = (f32x16)(0.f);
     float m = -INFINITY, l = 0.f;
+    bool odd = false;
 
     const In* kb = (const In*)k.p + (size_t)s.k0 * k.ts + (size_t)hk * k.hs;
     const In* vb = (const In*)v.p + (size_t)s.k0 * v.ts + (size_t)hk * v.hs;
@@ -77,6 +78,10 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(AttnTil
 #pragma unroll
                     for (int i = 0; i < 16; ++i)
                         if (j0 + (t * KSPLIT + share) * 32 + 8 * (i / 4) + 4 * h + i % 4 >= limit) sc[t][i] = -INFINITY;
+                if (g.causal) {
+#pragma unroll
+                    for (int t = 0; t < SUB; ++t) odd |= attn_odd<T, DP>(tv, (t * KSPLIT + share) * 32, lane);
+                }
             }
             float mx = sc[0][0];
 #pragma unroll
@@ -119,6 +124,9 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(AttnTil
         __syncthreads();
     }
     l += attn_other_half(l);
+    if (__any(odd))
+        attn_redo<T, DP>((const In*)q.p + (size_t)(s.q0 + tok) * q.ts + (size_t)head * q.hs, kb, k.ts, vb, v.ts, acc, g.D, g.c, m, limit, share * 32,
+                         KSPLIT * 32, wave_hi, lane);
     if (KSPLIT == 2) {          // the second wave's sums to the first one, through the tiles nobody needs any more
         float* pass = (float*)&lds_k[0][0] + wave % GROUPS * (L::DB * 16 * 64);
         __shared__ float pass_m[GROUPS][64], pass_l[GROUPS][64];

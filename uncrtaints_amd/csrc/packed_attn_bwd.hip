@@ -27,7 +27,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(AttnTil
     const AttnSeq s = attn_seq(g, b);
     const int rows = s.lq * g.G;
     if (tile * BM >= rows) return;
-    const int row0 = tile * BM + wave % GROUPS * 32, share = wave / GROUPS;      // KSPLIT waves have the same rows and every KSPLIT-th 32 keys
+    const int row0 = tile * BM + wave % GROUPS * 32, share = KSPLIT == 1 ? 0 : wave / GROUPS;      // KSPLIT waves have the same rows and every KSPLIT-th 32 keys
     const int row = min(row0 + col, rows - 1), tok = row / g.G, head = hk * g.G + row - tok * g.G;
     const int shift = s.lk - s.lq;
     auto limit_of = [&](int r) { return g.causal ? min(max(min(r, rows - 1) / g.G + shift + 1, 0), s.lk) : s.lk; };
@@ -137,7 +137,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(AttnTil
 // nothing to run beside it); the exponentials of one wave run beside the products of the other.  P crosses in the accumulator layout, lane
 // by lane.  Q and dOut tiles rotate through three buffers: the one being filled and those of the two roles.
 template <typename T, int DP, int PAIRS, bool VEC>
-__global__ __launch_bounds__(PAIRS * 128) void packed_attn_dkv_kernel(const AttnGeom g, const AttnTensor q, const AttnTensor k, const AttnTensor v,
+__global__ __launch_bounds__(PAIRS * 128) __attribute__((amdgpu_waves_per_eu(2))) void packed_attn_dkv_kernel(const AttnGeom g, const AttnTensor q, const AttnTensor k, const AttnTensor v,
                                                               const AttnTensor go, const float* __restrict__ rowstat,
                                                               typename AttnElem<T>::Out* __restrict__ dk,
                                                               typename AttnElem<T>::Out* __restrict__ dv, int slots) {

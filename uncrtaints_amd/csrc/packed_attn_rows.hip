@@ -65,7 +65,7 @@ __global__ __launch_bounds__(NW * 64) void packed_attn_rows_kernel(const AttnGeo
             attn_arrived();
         }
         attn_own_lds();
-        run.tile(lds[wave][buf][0], lds[wave][buf][1], qf, g.c, j0, limit, j0 + 32 > lo, lane);
+        run.tile(lds[wave][buf][0], lds[wave][buf][1], qf, g.c, j0, limit, j0 + 32 > lo, g.causal != 0, lane);
         if (more) {
             attn_own_lds();
             if (NBUF == 1) {
@@ -78,6 +78,9 @@ __global__ __launch_bounds__(NW * 64) void packed_attn_rows_kernel(const AttnGeo
         if (NBUF == 2) buf ^= 1;
     }
     float l = run.l + attn_other_half(run.l), m = run.m;
+    if (__any(run.odd))
+        attn_redo<T, DP>((const In*)q.p + (size_t)(s.q0 + tok) * q.ts + (size_t)head * q.hs, kb, k.ts, vb, v.ts, run.acc, g.D, g.c, m, limit,
+                         begin + (SHARE ? wave * 32 : 0), STEP, end, lane);
     if (!SHARE) {
         if (row0 + col >= rows) return;
         attn_store_row<Out, L::DB>(out + (size_t)(s.q0 + tok) * o_ts + (size_t)head * o_hs, run.acc, attn_inv(l), h, g.D);

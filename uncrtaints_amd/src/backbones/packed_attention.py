@@ -105,7 +105,8 @@ class PackedAttention(nn.Module):
       offsets_q, offsets_k [B + 1]: int32 on the device, not decreasing; sequence b owns rows offsets[b] .. offsets[b + 1] - 1 (`pack_offsets`).
       Without offsets_k the keys lie like the queries.  They are not read on the host; offsets outside the tensors are clamped on the device.
       k_len [B]: int32, used rows of each key sequence; the rest is room in a cache, never read into a result.
-      A row that sees no key is 0 and takes no part in any gradient.  Rows of no sequence are zeros, in the gradients too.
+      A row that sees no key is 0 and takes no part in any gradient.  Rows of no sequence are zeros, in the gradients too.  Keys and values
+      that a row does not see may hold anything, infinities and NaN included (gradients want all of a sequence's own rows finite).
       max_q, max_k: the longest sequences as far as the program knows them; they choose among the kernels (few rows per sequence over a cache,
       short sequences) and change nothing else: a wrong one costs time.
       out: written in place of a new tensor (only without gradients); rows of no sequence stay as they were.
@@ -158,5 +159,8 @@ class PackedAttention(nn.Module):
                 E.check_tokens(q=q, out=out)
                 if out.shape != q.shape or not out.is_contiguous():
                     raise ValueError(f"out {tuple(out.shape)}: a contiguous tensor of q's shape {tuple(q.shape)} is required")
+                at = out.untyped_storage().data_ptr()
+                if at and any(t.untyped_storage().data_ptr() == at for t in (q, k, v)):
+                    raise ValueError("out shares memory with an input")
             res, lse = E.packed_attention_forward(q, k, v, offsets_q, offsets_k, k_len, temperature, self.causal, return_lse, out, *hints)
         return (res, lse) if return_lse else res
