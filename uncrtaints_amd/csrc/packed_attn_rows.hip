@@ -6,14 +6,18 @@
 //           exponentials are joined by a second launch.
 //   short:  both sides are at most two tiles: each wave has a sequence and head of its own (a block of the kernels in packed_attn.hip
 //           would leave three of its four waves without rows), and the backward makes all three gradients in one pass over one tile.
+// Measured: 24 caches of 331 to 32768 keys, 32/8 heads of 128, bf16: 397 us for 1.88 GB, 4.7 TB/s where a large copy reaches 4.96 (the kernel
+// of packed_attn.hip alone: 1043); one token over 1000 keys, 16/4 heads of 64: 10 us in one launch, bound by the loads that wait for each
+// other (23 us there).  1500 series of up to 30 dates, 16 heads of 16, fp32: forward 49 us, backward 88 (332 and 930 there); half of that is
+// the 272 MB they move, the rest products of 32 x 32 tiles that are a quarter full.
 #include "packed_attn.h"
 
 namespace {
 
 template <typename T, int DP, int NW, bool SHARE, bool VEC>
-__global__ __launch_bounds__(NW * 64) void packed_attn_rows_kernel(const AttnGeom g, const AttnTensor q, const AttnTensor k, const AttnTensor v,
-                                                                   T* __restrict__ out, long long o_ts, long long o_hs, float* __restrict__ lse,
-                                                                   float* __restrict__ work, int chunk, int splits, int tasks) {
+__global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(SHARE ? 1 : DP <= 32 ? 4 : 2))) void packed_attn_rows_kernel(
+    const AttnGeom g, const AttnTensor q, const AttnTensor k, const AttnTensor v, T* __restrict__ out, long long o_ts, long long o_hs,
+    float* __restrict__ lse, float* __restrict__ work, int chunk, int splits, int tasks) {
     typedef AttnTile<T, DP> L;
     typedef typename AttnElem<T>::In In;
     typedef typename AttnElem<T>::Out Out;
@@ -213,9 +217,9 @@ __global__ __launch_bounds__(256) void packed_attn_join_kernel(const AttnGeom g,
 // rows), give dQ as they are, and cross a 32 x 32 patch of LDS to become columns of keys for dK and dV.  More keys than a tile (the caller
 // said otherwise): the same for every tile of keys, and dQ in a second round.
 template <typename T, int DP, int NW, bool VEC>
-__global__ __launch_bounds__(NW * 64) void packed_attn_short_bwd_kernel(const AttnGeom g, const AttnTensor q, const AttnTensor k, const AttnTensor v,
-                                                                        const AttnTensor o, const AttnTensor go, const float* __restrict__ lse,
-                                                                        T* __restrict__ dq, T* __restrict__ dk, T* __restrict__ dv) {
+__global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(DP <= 32 ? 3 : 2))) void packed_attn_short_bwd_kernel(
+    const AttnGeom g, const AttnTensor q, const AttnTensor k, const AttnTensor v, const AttnTensor o, const AttnTensor go,
+    const float* __restrict__ lse, T* __restrict__ dq, T* __restrict__ dk, T* __restrict__ dv) {
     typedef AttnTile<T, DP> L;
     typedef typename AttnElem<T>::In In;
     typedef typename AttnElem<T>::Out Out;
