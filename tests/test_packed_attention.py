@@ -552,3 +552,89 @@ def test_entry_points_refuse_bad_sizes():
                Hk=2, D=8, stream=None)
     for kw in (dict(Hq=5), dict(D=200), dict(lse=None), dict(rowstat=None), dict(dq=None), dict(dk=None), dict(v=None), dict(dk=24 - 4), dict(act=-1)):
         assert bwd(*{**ok2, **kw}.values()) < 0, kw
+
+
+@gpu
+@BOTH
+@pytest.mark.parametrize("lq, lk, hq, hk, d, hints", [
+    ([1, 1, 1], [20000, 0, 4000], 4, 2, 8, True), ([1, 1], [300, 700], 4, 4, 64, True), ([40, 3], [40, 3], 4, 2, 16, True), ([5, 30], [5, 30], 2, 2, 16, True),
+    ([100, 700], [600, 700], 2, 1, 32, False), ([300], [300], 2, 2, 128, False)])
+def test_a_query_that_is_not_a_number_gives_a_row_that_is_none(lq, lk, hq, hk, d, hints, dtype):
+    """In every kernel, the one that joins parts of a cache among them: NaN in the row's result and its lse, the other rows as they should be.
+    A row that sees no key is 0 whatever its query holds."""
+    from uncrtaints_amd.src.backbones.packed_attention import PackedAttention
+    g = _gen(5)
+    q, k, v = (torch.randn(n, h, d, generator=g).to(dtype) for n, h in ((sum(lq), hq), (sum(lk), hk), (sum(lk), hk)))
+    off_q, off_k = _offsets(lq), _offsets(lk)
+    bad = [(int(off_q[b]) + min(n - 1, b), (b + 1) % hq) for b, n in enumerate(lq)]
+    for t, h in bad:
+        q[t, h, d // 2] = math.nan
+    out, lse = PackedAttention()(q.to(DEV), k.to(DEV), v.to(DEV), off_q.to(DEV), off_k.to(DEV), return_lse=True,
+                                 **(dict(max_q=max(lq), max_k=max(lk)) if hints else {}))
+    out, lse = out.cpu(), lse.cpu()
+    for b, n in enumerate(lq):
+        rq, rk = slice(int(off_q[b]), int(off_q[b]) + n), slice(int(off_k[b]), int(off_k[b]) + lk[b])
+        for h in range(hq):
+            c = h // (hq // hk)
+            qs = q[rq, h].double()
+            rows = torch.isfinite(qs).all(1)
+            ref = reference(qs[rows][None], k[rk, c].double(), v[rk, c].double(), torch.zeros(1, int(rows.sum()), d, dtype=torch.float64), False,
+                            math.sqrt(d), dtype)
+            _check("out", out[rq, h][rows], *(t[0] for t in ref["out"]))
+            _check("lse", lse[rq, h][rows], *(t[0] for t in ref["lse"]))
+            if lk[b]:
+                assert out[rq, h][~rows].isnan().all() and lse[rq, h][~rows].isnan().all()
+            else:
+                assert (out[rq, h] == 0).all() and (lse[rq, h] == -math.inf).all()
+
+
+@gpu
+def test_more_single_tokens_than_shared_blocks_hold():
+    """1.1 million series of one date, 8 heads, nothing known of their lengths: one key each, so out is v -- the product with p, the reciprocal of
+    l = p (2.5 units at most, 5 half steps) and the product with it: 7 u."""
+    from uncrtaints_amd.src.backbones.packed_attention import PackedAttention
+    n = 1_100_000
+    g = torch.Generator(device=DEV).manual_seed(6)
+    q, k, v = (torch.randn(n, 8, 4, generator=g, device=DEV) for _ in range(3))
+    out = PackedAttention()(q, k, v, torch.arange(n + 1, dtype=torch.int32, device=DEV))
+    assert bool(((out - v).abs() <= 7 * U * v.abs()).all())
+
+
+@gpu
+def test_out_counts_as_a_change_in_place():
+    from uncrtaints_amd.src.backbones.packed_attention import PackedAttention, pack_offsets
+    m, off = PackedAttention(), pack_offsets([2, 4], DEV)
+    q, w = torch.randn(6, 4, 8, generator=_gen(7)).to(DEV), torch.ones(6, 4, 8, device=DEV, requires_grad=True)
+    with pytest.raises(ValueError, match="requires one"):
+        m(q, q, q, off, out=w)
+    out = torch.zeros(6, 4, 8, device=DEV)
+    loss = (out * w).sum()
+    m(q, q, q, off, out=out)
+    with pytest.raises(RuntimeError, match="inplace"):
+        loss.backward()
+
+
+def test_scales_and_sizes_beyond_the_built_ones_are_refused():
+    """Temperatures whose scale is no number in fp32, and launches of more threads than are counted: refused before anything is enqueued."""
+    from uncrtaints_amd import engine as E
+    from uncrtaints_amd import hip_backend as hb
+    from uncrtaints_amd.src.backbones.packed_attention import PackedAttention
+    for t in (1e-31, 1e-45, 1e31):
+        with pytest.raises(ValueError, match="1e-30"):
+            PackedAttention(temperature=t)
+    with pytest.raises(RuntimeError, match="31 bits"):
+        E.packed_attention_forward(torch.zeros(1, 1, 2).expand(2 ** 31, 1, 2), *(torch.zeros(4, 1, 2),) * 2, *(torch.zeros(2, dtype=torch.int32),) * 2, None, 1.0,
+                                   False, False)
+    args = lambda name: dict.fromkeys([n for _, n in hb.parse_header()[name]], 0)
+    big = 1 << 22
+    ok = {**args("uncr_packed_attn_fwd"), **dict(q=16, k=16, v=16, out=16, off_q=16, off_k=16, lse=None, k_len=None, work=None, temperature=1.0, B=big, Nq=big,
+                                                 Nk=big, Hq=64, Hk=64, D=8, stream=None)}
+    shape = hb.lib().fn["uncr_packed_attn_fwd"](*{**ok, "D": 0}.values())
+    for kw in (dict(), dict(max_q=1, max_k=60), dict(D=128), dict(max_q=64, D=64)):
+        assert hb.lib().fn["uncr_packed_attn_fwd"](*{**ok, **kw}.values()) == shape, kw
+    for t in (1e-31, 1e31):
+        assert hb.lib().fn["uncr_packed_attn_fwd"](*{**ok, "B": 1, "Nq": 0, "temperature": t}.values()) < 0
+    ok = {**args("uncr_packed_attn_bwd"), **dict(q=16, k=16, v=16, out=16, dout=16, lse=16, dq=16, dk=16, dv=16, rowstat=16, off_q=16, off_k=16, k_len=None,
+                                                 work=None, temperature=1.0, B=big, Nq=big, Nk=big, Hq=128, Hk=128, D=8, stream=None)}
+    for kw in (dict(), dict(max_q=1, max_k=60), dict(Nq=0), dict(D=128)):
+        assert hb.lib().fn["uncr_packed_attn_bwd"](*{**ok, **kw}.values()) == shape, kw

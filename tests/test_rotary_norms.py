@@ -305,3 +305,27 @@ def test_rotary_entry_points_refuse_bad_geometry():
     for kw in (dict(D=7), dict(D=258), dict(D=0), dict(N=-1), dict(H=0), dict(s0=3), dict(s0=-2), dict(s1=8), dict(s2=2), dict(n_axes=5),
                dict(n_axes=-1), dict(pos_dt=4), dict(act=2), dict(N=3, pos=None), dict(N=3, turns=None), dict(N=3, x=None), dict(N=3, y=None)):
         assert call(**kw) < 0, kw
+
+
+@gpu
+def test_positions_changed_before_the_backward_are_an_error():
+    from uncrtaints_amd.src.backbones.packed_attention import HeadNormRotary
+    r = _module(64, SHAPES[0][1], "halves").to(DEV)
+    m = HeadNormRotary(64, rotary=r).to(DEV)
+    x, pos = torch.randn(5, 6, 64, generator=_gen(50)).to(DEV).requires_grad_(), _positions(5, 3, torch.int32, 51).to(DEV)
+    ys = r(x, pos), m(x, x, pos)[0]
+    pos += 1
+    for y in ys:
+        with pytest.raises(RuntimeError, match="inplace"):
+            y.sum().backward()
+
+
+def test_more_tokens_than_are_counted_are_refused():
+    from uncrtaints_amd import engine as E
+    from uncrtaints_amd import hip_backend as hb
+    with pytest.raises(RuntimeError, match="31 bits"):
+        E.rotary_axes(torch.zeros(1, 1, 2).expand(2 ** 31, 1, 2), E.RotaryPlan())
+    ok = dict(x=16, x_ts=256, x_hs=256, y=16, y_ts=256, y_hs=256, pos=16, pos_dt=0, n_axes=1, s0=256, s1=0, s2=0, s3=0, turns=16, nb=0, inv=0, N=2 ** 31 - 1,
+              H=1, D=256, act=0, stream=None)
+    fn = hb.lib().fn["uncr_rotary_axes"]
+    assert fn(*ok.values()) == fn(*{**ok, "H": 0}.values()) < 0

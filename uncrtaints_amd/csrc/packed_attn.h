@@ -68,7 +68,7 @@ __device__ __forceinline__ bool attn_find(const int* off, int B, int N, int per,
     }
     b = lo;
     tile = slot - attn_slot(off, lo, N, per, shift);
-    return tile >= 0;
+    return tile >= 0 && tile <= (int)(((long long)N * per) >> shift);      // more only if the offsets decrease: no row number may wrap
 }
 // The same tiles in descending order of their causal work, for a few long sequences: with tiles in the order of the sequences a long one
 // that comes late keeps some blocks busy long after the others have ended (five sequences of 2832 to 5000 tokens, 16/4 heads of 128, dK/dV:
@@ -127,6 +127,8 @@ static inline bool attn_sorts(const AttnGeom& g, long long rows, int per_tile) {
     return g.causal && g.B <= ATTN_SORT_MAX_B && rows / per_tile >= 4ll * g.B && (long long)g.Nk * g.G < (1ll << 29) && (long long)g.G * per_tile < (1 << 20);
 }
 static inline int attn_slots(long long rows, int B, int shift) { return (int)(rows >> shift) + B; }
+// a launch's threads are counted in 32 bits
+static inline bool attn_grid(long long blocks, int threads) { return blocks * threads <= 0xffffffffll; }
 
 // fp32 on the bf16 matrix units: x = x0 + x1 + x2 exactly to 24 bits, each rounded to bf16 from what the ones before leave, and
 //   a b = a0 b0 + a0 b1 + a1 b0 + a1 b1 + a0 b2 + a2 b0      (what is left out is below 2^-24 |a b|, a rounding of fp32)
@@ -624,7 +626,7 @@ void attn_planes(const AttnGeom& g, const AttnTensor* in, const int* N, const in
 struct AttnSplit { int waves, chunk, splits; };     // waves that share a task, keys per block, blocks per sequence (1: no partial results)
 AttnSplit attn_split(const AttnGeom& g, int max_q, int max_k, int act);
 bool attn_short(const AttnGeom& g, int max_q, int max_k);
-void attn_rows_fwd(const AttnGeom& g, const AttnSplit& s, const AttnTensor& q, const AttnTensor& k, const AttnTensor& v, void* out, long long o_ts,
+bool attn_rows_fwd(const AttnGeom& g, const AttnSplit& s, const AttnTensor& q, const AttnTensor& k, const AttnTensor& v, void* out, long long o_ts,
                    long long o_hs, float* lse, float* work, int act, bool vec, hipStream_t stream);
-void attn_short_bwd(const AttnGeom& g, const AttnTensor& q, const AttnTensor& k, const AttnTensor& v, const AttnTensor& o, const AttnTensor& go,
+bool attn_short_bwd(const AttnGeom& g, const AttnTensor& q, const AttnTensor& k, const AttnTensor& v, const AttnTensor& o, const AttnTensor& go,
                     const float* lse, void* dq, void* dk, void* dv, int act, bool vec, hipStream_t stream);

@@ -162,21 +162,23 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(AttnTil
 }
 
 template <typename T, int DP, int NW, int TK, int KSPLIT>
-void launch_k(AttnGeom g, const AttnTensor& q, const AttnTensor& k, const AttnTensor& v, void* out, long long o_ts, long long o_hs, float* lse, bool vec,
+bool launch_k(AttnGeom g, const AttnTensor& q, const AttnTensor& k, const AttnTensor& v, void* out, long long o_ts, long long o_hs, float* lse, bool vec,
               hipStream_t stream) {
     constexpr int BM = NW / KSPLIT * 32, SHIFT = BM == 256 ? 8 : BM == 128 ? 7 : 6;
     const int slots = attn_slots((long long)g.Nq * g.G, g.B, SHIFT);
+    if (!attn_grid((long long)slots * g.Hk, NW * 64)) return false;
     g.sorted = attn_sorts(g, (long long)g.Nq * g.G, BM);
     typedef typename AttnElem<T>::Out Out;
     constexpr bool THREE = AttnElem<T>::THREE;          // always whole vectors
     if (vec) hipLaunchKernelGGL((packed_attn_fwd_kernel<T, DP, NW, TK, KSPLIT, true>), dim3(slots * g.Hk), dim3(NW * 64), 0, stream, g, q, k, v, (Out*)out, o_ts, o_hs, lse, slots);
     else hipLaunchKernelGGL((packed_attn_fwd_kernel<T, DP, NW, TK, KSPLIT, THREE>), dim3(slots * g.Hk), dim3(NW * 64), 0, stream, g, q, k, v, (Out*)out, o_ts, o_hs, lse, slots);
+    return true;
 }
 template <typename T, int DP, int NW, int TK>
-void launch(const AttnGeom& g, const AttnTensor& q, const AttnTensor& k, const AttnTensor& v, void* out, long long o_ts, long long o_hs, float* lse,
+bool launch(const AttnGeom& g, const AttnTensor& q, const AttnTensor& k, const AttnTensor& v, void* out, long long o_ts, long long o_hs, float* lse,
             bool vec, hipStream_t stream) {
-    if (TK == 64 && attn_few_blocks(g, NW * 32)) launch_k<T, DP, NW, TK, TK == 64 ? 2 : 1>(g, q, k, v, out, o_ts, o_hs, lse, vec, stream);
-    else launch_k<T, DP, NW, TK, 1>(g, q, k, v, out, o_ts, o_hs, lse, vec, stream);
+    if (TK == 64 && attn_few_blocks(g, NW * 32)) return launch_k<T, DP, NW, TK, TK == 64 ? 2 : 1>(g, q, k, v, out, o_ts, o_hs, lse, vec, stream);
+    return launch_k<T, DP, NW, TK, 1>(g, q, k, v, out, o_ts, o_hs, lse, vec, stream);
 }
 
 }  // namespace
@@ -185,7 +187,8 @@ int attn_geom(AttnGeom& g, const int* off_q, const int* off_k, const int* k_len,
               int Hk, int D, int act) {
     if (B <= 0 || Nq < 0 || Nk < 0 || Hq <= 0 || Hk <= 0 || Hq % Hk || D <= 0 || D > 128) return UNCR_ESHAPE;
     if ((long long)Nq * (Hq / Hk) > 0x40000000ll || Nk > 0x40000000) return UNCR_ESHAPE;      // rows and keys are counted in 32 bits
-    if ((act != 0 && act != 1) || !off_q || !off_k || !(temperature > 0.f)) return UNCR_EINVAL;
+    // beyond these the scale of the scores or its product with a hidden score, -infinity, is no number
+    if ((act != 0 && act != 1) || !off_q || !off_k || !(temperature >= 1e-30f && temperature <= 1e30f)) return UNCR_EINVAL;
     // blocks of a launch: at least 32 rows each
     if (((((long long)Nq * (Hq / Hk)) >> 5) + B) * Hk > 0x7fffffffll || (((long long)Nk >> 5) + B) * Hk > 0x7fffffffll) return UNCR_ESHAPE;
     g.off_q = off_q; g.off_k = off_k; g.k_len = k_len;
@@ -232,25 +235,27 @@ extern "C" int uncr_packed_attn_fwd(const void* q, long long q_ts, long long q_h
         if ((uintptr_t)out % size || (o_ts * size / 4) % size || (o_hs * size / 4) % size) return UNCR_EINVAL;
     }
     const AttnSplit split = attn_split(g, max_q, max_k, act);
+    bool fits;
     if (split.waves) {
         if (split.splits > 1 && (!work || work_floats < (long long)split.splits * Nq * Hq * (D + 2))) return UNCR_EINVAL;
-        attn_rows_fwd(g, split, tq, tk, tv, out, o_ts, o_hs, lse, work, act, vec, stream);
+        fits = attn_rows_fwd(g, split, tq, tk, tv, out, o_ts, o_hs, lse, work, act, vec, stream);
     } else if (attn_three(g, act, vec)) {
         if (!work || work_floats < attn_planes_floats(g, 1, 2)) return UNCR_EINVAL;
         const int n[3] = {Nq, Nk, Nk}, h[3] = {Hq, Hk, Hk};
         AttnTensor p[3];
         attn_planes(g, all, n, h, 3, work, p, stream);
-        if (D <= 32) launch<AttnThree, 32, 4, 64>(g, p[0], p[1], p[2], out, o_ts, o_hs, lse, true, stream);
-        else launch<AttnThree, 64, 4, 32>(g, p[0], p[1], p[2], out, o_ts, o_hs, lse, true, stream);
+        if (D <= 32) fits = launch<AttnThree, 32, 4, 64>(g, p[0], p[1], p[2], out, o_ts, o_hs, lse, true, stream);
+        else fits = launch<AttnThree, 64, 4, 32>(g, p[0], p[1], p[2], out, o_ts, o_hs, lse, true, stream);
     } else if (act) {
-        if (D <= 32) launch<__bf16, 32, 4, 64>(g, tq, tk, tv, out, o_ts, o_hs, lse, vec, stream);
-        else if (D <= 64) launch<__bf16, 64, 4, 64>(g, tq, tk, tv, out, o_ts, o_hs, lse, vec, stream);
-        else launch<__bf16, 128, 8, 64>(g, tq, tk, tv, out, o_ts, o_hs, lse, vec, stream);
+        if (D <= 32) fits = launch<__bf16, 32, 4, 64>(g, tq, tk, tv, out, o_ts, o_hs, lse, vec, stream);
+        else if (D <= 64) fits = launch<__bf16, 64, 4, 64>(g, tq, tk, tv, out, o_ts, o_hs, lse, vec, stream);
+        else fits = launch<__bf16, 128, 8, 64>(g, tq, tk, tv, out, o_ts, o_hs, lse, vec, stream);
     } else {
-        if (D <= 32) launch<float, 32, 4, 64>(g, tq, tk, tv, out, o_ts, o_hs, lse, vec, stream);
-        else if (D <= 64) launch<float, 64, 4, 64>(g, tq, tk, tv, out, o_ts, o_hs, lse, vec, stream);
-        else launch<float, 128, 4, 32>(g, tq, tk, tv, out, o_ts, o_hs, lse, vec, stream);
+        if (D <= 32) fits = launch<float, 32, 4, 64>(g, tq, tk, tv, out, o_ts, o_hs, lse, vec, stream);
+        else if (D <= 64) fits = launch<float, 64, 4, 64>(g, tq, tk, tv, out, o_ts, o_hs, lse, vec, stream);
+        else fits = launch<float, 128, 4, 32>(g, tq, tk, tv, out, o_ts, o_hs, lse, vec, stream);
     }
+    if (!fits) return UNCR_ESHAPE;
     UNCR_LAUNCH_CHECK();
     return UNCR_OK;
 }

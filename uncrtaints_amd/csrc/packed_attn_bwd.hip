@@ -321,36 +321,39 @@ struct Bwd {
     hipStream_t stream;
 };
 
-template <typename T, int DP, int NW, int TK, int KSPLIT, bool VEC> void launch_dq(const Bwd& a) {
+template <typename T, int DP, int NW, int TK, int KSPLIT, bool VEC> bool launch_dq(const Bwd& a) {
     constexpr int BM = NW / KSPLIT * 32, SHIFT = BM == 256 ? 8 : BM == 128 ? 7 : 6;
     AttnGeom g = a.g;
     g.sorted = attn_sorts(g, (long long)g.Nq * g.G, BM);
     const int slots = attn_slots((long long)g.Nq * g.G, g.B, SHIFT);
+    if (!attn_grid((long long)slots * g.Hk, NW * 64)) return false;
     hipLaunchKernelGGL((packed_attn_dq_kernel<T, DP, NW, TK, KSPLIT, VEC>), dim3(slots * g.Hk), dim3(NW * 64), 0, a.stream, g, a.q, a.k, a.v, a.o, a.go,
                        a.go_raw, a.lse, (typename AttnElem<T>::Out*)a.dq, a.rowstat, slots);
+    return true;
 }
-template <typename T, int DP, int PAIRS, bool VEC> void launch_dkv(const Bwd& a) {
+template <typename T, int DP, int PAIRS, bool VEC> bool launch_dkv(const Bwd& a) {
     AttnGeom g = a.g;
     g.sorted = attn_sorts(g, g.Nk, PAIRS * 32);
     const int slots = attn_slots(g.Nk, g.B, PAIRS == 4 ? 7 : 6);
+    if (!attn_grid((long long)slots * g.Hk, PAIRS * 128)) return false;
     hipLaunchKernelGGL((packed_attn_dkv_kernel<T, DP, PAIRS, VEC>), dim3(slots * g.Hk), dim3(PAIRS * 128), 0, a.stream, g, a.q, a.k, a.v, a.go, a.rowstat,
                        (typename AttnElem<T>::Out*)a.dk, (typename AttnElem<T>::Out*)a.dv, slots);
+    return true;
 }
-template <typename T, int DP, int NW, int TK, bool VEC> void launch_v(const Bwd& a) {
+template <typename T, int DP, int NW, int TK, bool VEC> bool launch_v(const Bwd& a) {
     if (a.g.Nq) {
-        if (TK == 64 && attn_few_blocks(a.g, NW * 32)) launch_dq<T, DP, NW, TK, TK == 64 ? 2 : 1, VEC>(a);
-        else launch_dq<T, DP, NW, TK, 1, VEC>(a);
+        if (!(TK == 64 && attn_few_blocks(a.g, NW * 32) ? launch_dq<T, DP, NW, TK, TK == 64 ? 2 : 1, VEC>(a) : launch_dq<T, DP, NW, TK, 1, VEC>(a))) return false;
     }
     if (a.g.Nk) {
         // two pairs per block: as long as two blocks fit a CU's LDS
         constexpr bool SMALL = AttnTile<T, DP>::RB <= (AttnElem<T>::THREE ? 192 : 128);
-        if (SMALL && ((long long)a.g.Nk / 128 + a.g.B) * a.g.Hk < 1024) launch_dkv<T, DP, SMALL ? 2 : 4, VEC>(a);
-        else launch_dkv<T, DP, 4, VEC>(a);
+        if (SMALL && ((long long)a.g.Nk / 128 + a.g.B) * a.g.Hk < 1024) return launch_dkv<T, DP, SMALL ? 2 : 4, VEC>(a);
+        return launch_dkv<T, DP, 4, VEC>(a);
     }
+    return true;
 }
-template <typename T, int DP, int NW, int TK> void launch(const Bwd& a) {
-    if (a.vec) launch_v<T, DP, NW, TK, true>(a);
-    else launch_v<T, DP, NW, TK, AttnElem<T>::THREE>(a);
+template <typename T, int DP, int NW, int TK> bool launch(const Bwd& a) {
+    return a.vec ? launch_v<T, DP, NW, TK, true>(a) : launch_v<T, DP, NW, TK, AttnElem<T>::THREE>(a);
 }
 
 }  // namespace
@@ -382,8 +385,9 @@ extern "C" int uncr_packed_attn_bwd(const void* q, long long q_ts, long long q_h
     const AttnTensor all[] = {a.q, a.k, a.v, a.o, a.go};
     a.vec = attn_aligned(all, 5, D, act);
     if (Nq == 0 && Nk == 0) return UNCR_OK;
+    bool fits;
     if (attn_short(a.g, max_q, max_k)) {
-        attn_short_bwd(a.g, a.q, a.k, a.v, a.o, a.go, lse, dq, dk, dv, act, a.vec, stream);
+        fits = attn_short_bwd(a.g, a.q, a.k, a.v, a.o, a.go, lse, dq, dk, dv, act, a.vec, stream);
     } else if (attn_three(a.g, act, a.vec)) {
         if (!work || work_floats < attn_planes_floats(a.g, 2, 2)) return UNCR_EINVAL;
         const AttnTensor in[4] = {a.q, a.k, a.v, a.go};
@@ -391,17 +395,18 @@ extern "C" int uncr_packed_attn_bwd(const void* q, long long q_ts, long long q_h
         AttnTensor p[4];
         attn_planes(a.g, in, n, h, 4, work, p, stream);
         a.q = p[0]; a.k = p[1]; a.v = p[2]; a.go = p[3];
-        if (D <= 32) launch<AttnThree, 32, 4, 64>(a);
-        else launch<AttnThree, 64, 4, 32>(a);
+        if (D <= 32) fits = launch<AttnThree, 32, 4, 64>(a);
+        else fits = launch<AttnThree, 64, 4, 32>(a);
     } else if (act) {
-        if (D <= 32) launch<__bf16, 32, 4, 64>(a);
-        else if (D <= 64) launch<__bf16, 64, 4, 64>(a);
-        else launch<__bf16, 128, 8, 64>(a);
+        if (D <= 32) fits = launch<__bf16, 32, 4, 64>(a);
+        else if (D <= 64) fits = launch<__bf16, 64, 4, 64>(a);
+        else fits = launch<__bf16, 128, 8, 64>(a);
     } else {
-        if (D <= 32) launch<float, 32, 4, 64>(a);
-        else if (D <= 64) launch<float, 64, 4, 64>(a);
-        else launch<float, 128, 4, 32>(a);
+        if (D <= 32) fits = launch<float, 32, 4, 64>(a);
+        else if (D <= 64) fits = launch<float, 64, 4, 64>(a);
+        else fits = launch<float, 128, 4, 32>(a);
     }
+    if (!fits) return UNCR_ESHAPE;
     UNCR_LAUNCH_CHECK();
     return UNCR_OK;
 }

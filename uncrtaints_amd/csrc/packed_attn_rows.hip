@@ -192,8 +192,8 @@ __global__ __launch_bounds__(256) void packed_attn_join_kernel(const AttnGeom g,
 #pragma unroll
     for (int d = 32; d; d >>= 1) mm = fmaxf(mm, __shfl_xor(mm, d));
     float f = mm == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mm);
-    if (m != m) f = m;                              // NaN sums stay NaN
-    l = m == -INFINITY ? 0.f : l * f;
+    if (m != m) f = m;                              // NaN sums stay NaN, also those of a row that has no maximum because all its scores are NaN
+    l = m == -INFINITY && l == l ? 0.f : l * f;
 #pragma unroll
     for (int d = 32; d; d >>= 1) l += __shfl_xor(l, d);
     float a[2] = {0.f, 0.f};
@@ -380,24 +380,24 @@ struct Rows {
     hipStream_t stream;
 };
 
-template <typename T, int DP, int NW, bool SHARE, bool VEC> void launch(const Rows& a) {
+template <typename T, int DP, int NW, bool SHARE, bool VEC> bool launch(const Rows& a) {
     const int tasks = attn_slots((long long)a.g.Nq * a.g.G, a.g.B, 5) * a.g.Hk * (SHARE ? a.s.splits : 1);
-    hipLaunchKernelGGL((packed_attn_rows_kernel<T, DP, NW, SHARE, VEC>), dim3(SHARE ? tasks : (tasks + NW - 1) / NW), dim3(NW * 64), 0, a.stream, a.g, a.q,
+    const long long blocks = SHARE ? tasks : ((long long)tasks + NW - 1) / NW;
+    if (!attn_grid(blocks, NW * 64)) return false;
+    hipLaunchKernelGGL((packed_attn_rows_kernel<T, DP, NW, SHARE, VEC>), dim3((unsigned)blocks), dim3(NW * 64), 0, a.stream, a.g, a.q,
                        a.k, a.v, (T*)a.out, a.o_ts, a.o_hs, a.lse, a.work, a.s.chunk, a.s.splits, tasks);
     if (SHARE && a.s.splits > 1)
         hipLaunchKernelGGL((packed_attn_join_kernel<T>), dim3((unsigned)(((long long)a.g.Nq * a.g.Hq + 3) / 4)), dim3(256), 0, a.stream, a.g, a.work,
                            a.s.splits, (T*)a.out, a.o_ts, a.o_hs, a.lse);
+    return true;
 }
-template <typename T, int DP, bool VEC> void launch_n(const Rows& a) {
+template <typename T, int DP, bool VEC> bool launch_n(const Rows& a) {
     constexpr int NW = DP * sizeof(T) <= 128 ? 8 : DP * sizeof(T) <= 256 ? 4 : 2;      // a wave's four tiles are 128 rows: 128 KB of LDS per block
-    if (DP == 128 || a.s.waves > 1) launch<T, DP, NW, true, VEC>(a);
-    else launch<T, DP < 128 ? DP : 64, 4, false, VEC>(a);             // attn_short: heads up to 64
+    if (DP == 128 || a.s.waves > 1) return launch<T, DP, NW, true, VEC>(a);
+    return launch<T, DP < 128 ? DP : 64, 4, false, VEC>(a);           // attn_short: heads up to 64
 }
-template <typename T, bool VEC> void launch_d(const Rows& a) {
-    if (a.g.D <= 16) launch_n<T, 16, VEC>(a);
-    else if (a.g.D <= 32) launch_n<T, 32, VEC>(a);
-    else if (a.g.D <= 64) launch_n<T, 64, VEC>(a);
-    else launch_n<T, 128, VEC>(a);
+template <typename T, bool VEC> bool launch_d(const Rows& a) {
+    return a.g.D <= 16 ? launch_n<T, 16, VEC>(a) : a.g.D <= 32 ? launch_n<T, 32, VEC>(a) : a.g.D <= 64 ? launch_n<T, 64, VEC>(a) : launch_n<T, 128, VEC>(a);
 }
 
 struct Short {
@@ -407,14 +407,15 @@ struct Short {
     void *dq, *dk, *dv;
     hipStream_t stream;
 };
-template <typename T, int DP, bool VEC> void launch_short(const Short& a) {
-    hipLaunchKernelGGL((packed_attn_short_bwd_kernel<T, DP, 4, VEC>), dim3((a.g.B * a.g.Hk + 3) / 4), dim3(256), 0, a.stream, a.g, a.q, a.k, a.v, a.o, a.go,
+template <typename T, int DP, bool VEC> bool launch_short(const Short& a) {
+    const long long blocks = ((long long)a.g.B * a.g.Hk + 3) / 4;
+    if (!attn_grid(blocks, 256)) return false;
+    hipLaunchKernelGGL((packed_attn_short_bwd_kernel<T, DP, 4, VEC>), dim3((unsigned)blocks), dim3(256), 0, a.stream, a.g, a.q, a.k, a.v, a.o, a.go,
                        a.lse, (T*)a.dq, (T*)a.dk, (T*)a.dv);
+    return true;
 }
-template <typename T, bool VEC> void launch_short_d(const Short& a) {
-    if (a.g.D <= 16) launch_short<T, 16, VEC>(a);
-    else if (a.g.D <= 32) launch_short<T, 32, VEC>(a);
-    else launch_short<T, 64, VEC>(a);
+template <typename T, bool VEC> bool launch_short_d(const Short& a) {
+    return a.g.D <= 16 ? launch_short<T, 16, VEC>(a) : a.g.D <= 32 ? launch_short<T, 32, VEC>(a) : launch_short<T, 64, VEC>(a);
 }
 
 }  // namespace
@@ -430,13 +431,14 @@ bool attn_short(const AttnGeom& g, int max_q, int max_k) {
 AttnSplit attn_split(const AttnGeom& g, int max_q, int max_k, int act) {
     AttnSplit s = {0, 0, 1};
     const long long rows = (long long)(max_q > 0 ? max_q : (g.Nq + g.B - 1) / g.B) * g.G;
-    const long long keys = max_k > 0 ? max_k : (g.Nk + g.B - 1) / g.B;
+    const long long keys = max_k > 0 ? (max_k < g.Nk ? max_k : g.Nk) : (g.Nk + g.B - 1) / g.B;
     if (attn_short(g, max_q, max_k)) { s.waves = 1; return s; }
     if (rows > 32) return s;
     const int dp = g.D <= 16 ? 16 : g.D <= 32 ? 32 : g.D <= 64 ? 64 : 128, bytes = dp * (act ? 2 : 4);
     s.waves = bytes <= 128 ? 8 : bytes <= 256 ? 4 : 2;
-    if (keys <= 32ll * 8 * s.waves) return s;
     const long long tasks = attn_slots((long long)g.Nq * g.G, g.B, 5) * (long long)g.Hk;
+    if (dp < 128 && !attn_grid(tasks, s.waves * 64)) s.waves = 1;         // millions of them: a wave each is what a launch can hold
+    if (s.waves == 1 || keys <= 32ll * 8 * s.waves) return s;
     int chunk = 4096;
     while (chunk > 32 * s.waves && tasks * ((keys + chunk - 1) / chunk) < 2048) chunk >>= 1;
     long long n = (keys + chunk - 1) / chunk;
@@ -448,16 +450,16 @@ AttnSplit attn_split(const AttnGeom& g, int max_q, int max_k, int act) {
     return s;
 }
 
-void attn_rows_fwd(const AttnGeom& g, const AttnSplit& s, const AttnTensor& q, const AttnTensor& k, const AttnTensor& v, void* out, long long o_ts,
+bool attn_rows_fwd(const AttnGeom& g, const AttnSplit& s, const AttnTensor& q, const AttnTensor& k, const AttnTensor& v, void* out, long long o_ts,
                    long long o_hs, float* lse, float* work, int act, bool vec, hipStream_t stream) {
     const Rows a = {g, s, q, k, v, out, o_ts, o_hs, lse, work, stream};
-    if (act) vec ? launch_d<__bf16, true>(a) : launch_d<__bf16, false>(a);
-    else vec ? launch_d<float, true>(a) : launch_d<float, false>(a);
+    if (act) return vec ? launch_d<__bf16, true>(a) : launch_d<__bf16, false>(a);
+    return vec ? launch_d<float, true>(a) : launch_d<float, false>(a);
 }
 
-void attn_short_bwd(const AttnGeom& g, const AttnTensor& q, const AttnTensor& k, const AttnTensor& v, const AttnTensor& o, const AttnTensor& go,
+bool attn_short_bwd(const AttnGeom& g, const AttnTensor& q, const AttnTensor& k, const AttnTensor& v, const AttnTensor& o, const AttnTensor& go,
                     const float* lse, void* dq, void* dk, void* dv, int act, bool vec, hipStream_t stream) {
     const Short a = {g, q, k, v, o, go, lse, dq, dk, dv, stream};
-    if (act) vec ? launch_short_d<__bf16, true>(a) : launch_short_d<__bf16, false>(a);
-    else vec ? launch_short_d<float, true>(a) : launch_short_d<float, false>(a);
+    if (act) return vec ? launch_short_d<__bf16, true>(a) : launch_short_d<__bf16, false>(a);
+    return vec ? launch_short_d<float, true>(a) : launch_short_d<float, false>(a);
 }

@@ -417,9 +417,13 @@ struct Bwd { static constexpr int MAX_C = 4; RotGeom g; GradSet q, k; float eps;
 
 size_t lds_bytes(const RotGeom& g) { return (size_t)(ROT_THREADS / 64) * g.tok * (g.D / 2) * sizeof(float2); }
 
+// tokens of a block; the threads of a forward launch are counted in 32 bits
+int per_block(const RotGeom& g) { return g.tok * (ROT_THREADS / 64); }
+bool fits(const RotGeom& g) { return ((long long)g.N + per_block(g) - 1) / per_block(g) * ROT_THREADS <= 0xffffffffll; }
+
 template <typename T, bool NB, bool NORM, int C, int K> void run(const Fwd& f) {
-    const int per = f.g.tok * (ROT_THREADS / 64);
-    hipLaunchKernelGGL((rotary_kernel<T, C, K, NB, NORM>), dim3((f.g.N + per - 1) / per), dim3(ROT_THREADS), lds_bytes(f.g), f.stream, f.g, f.q, f.k, f.eps);
+    const int per = per_block(f.g);
+    hipLaunchKernelGGL((rotary_kernel<T, C, K, NB, NORM>), dim3((unsigned)(((long long)f.g.N + per - 1) / per)), dim3(ROT_THREADS), lds_bytes(f.g), f.stream, f.g, f.q, f.k, f.eps);
 }
 template <typename T, bool NB, bool NORM, int C, int K> void run(const Bwd& b) {
     hipLaunchKernelGGL((headnorm_bwd_kernel<T, C, K, NB>), dim3(b.blocks), dim3(ROT_THREADS), lds_bytes(b.g), b.stream, b.g, b.q, b.k, b.eps, b.part);
@@ -454,6 +458,7 @@ extern "C" int uncr_rotary_axes(const void* x, long long x_ts, long long x_hs, v
     const void* const pt[] = {x, y};
     const int c = pick_c(g, st, 4, pt, 2, act ? 2 : 4, Fwd::MAX_C), items = shape(g, c, H);
     const HeadSet q = {x, y, nullptr, x_ts, x_hs, y_ts, y_hs, H}, none = {nullptr, nullptr, nullptr, 0, 0, 0, 0, 0};
+    if (!fits(g)) return UNCR_ESHAPE;
     launch<false>(Fwd{g, q, none, 0.f, items, stream}, c, act);
     UNCR_LAUNCH_CHECK();
     return UNCR_OK;
@@ -474,6 +479,7 @@ extern "C" int uncr_headnorm_rotary_fwd(const void* q, long long q_ts, long long
     const void* const pt[] = {q, k, qo, ko};
     const int c = pick_c(g, st, 5, pt, 4, act ? 2 : 4, Fwd::MAX_C, wq, wk), items = shape(g, c, Hq + Hk);
     const HeadSet zq = {q, qo, wq, q_ts, q_hs, (long long)Hq * D, D, Hq}, zk = {k, ko, wk, k_ts, k_hs, (long long)Hk * D, D, Hk};
+    if (!fits(g)) return UNCR_ESHAPE;
     launch<true>(Fwd{g, zq, zk, eps, items, stream}, c, act);
     UNCR_LAUNCH_CHECK();
     return UNCR_OK;
@@ -497,8 +503,8 @@ extern "C" int uncr_headnorm_rotary_bwd(const void* q, long long q_ts, long long
         const long long st[] = {q_ts, q_hs, k_ts, k_hs, gq_ts, gq_hs, gk_ts, gk_hs, (long long)D};
         const void* const pt[] = {q, k, gq, gk, dq, dk};
         const int c = pick_c(g, st, 9, pt, 6, act ? 2 : 4, Bwd::MAX_C, wq, wk), items = shape(g, c, Hq + Hk);
-        const int per = g.tok * (ROT_THREADS / 64), tiles = (N + per - 1) / per;
-        blocks = tiles < ROT_MAX_SLOTS ? tiles : ROT_MAX_SLOTS;
+        const long long tiles = ((long long)N + per_block(g) - 1) / per_block(g);
+        blocks = tiles < ROT_MAX_SLOTS ? (int)tiles : ROT_MAX_SLOTS;
         const GradSet zq = {q, gq, dq, wq, q_ts, q_hs, gq_ts, gq_hs, Hq}, zk = {k, gk, dk, wk, k_ts, k_hs, gk_ts, gk_hs, Hk};
         launch<true>(Bwd{g, zq, zk, eps, items, blocks, part, stream}, c, act);
         UNCR_LAUNCH_CHECK();

@@ -2191,6 +2191,8 @@ def check_device(**tensors):
 
 def _token_rows(x: Tensor) -> Tensor:
     """[tokens, heads, d] with d contiguous; token and head strides stay as they are (a slice of a fused projection is read in place)."""
+    if x.shape[0] > 0x7fffffff:
+        raise RuntimeError(f"{x.shape[0]} tokens: they are counted in 31 bits")
     return x if x.stride(-1) == 1 or x.shape[-1] == 1 else x.contiguous()
 
 

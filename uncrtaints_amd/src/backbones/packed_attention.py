@@ -15,14 +15,14 @@ from ... import engine as E
 class _HeadNormRotaryFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, wq, wk, eps, plan):
-        ctx.save_for_backward(q, k, wq, wk)
+        ctx.save_for_backward(q, k, wq, wk, plan.positions)       # positions too: a change in place before the backward is an error
         ctx.eps, ctx.plan = eps, plan
         return E.headnorm_rotary_forward(q, k, wq, wk, eps, plan)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, gq, gk):
-        q, k, wq, wk = ctx.saved_tensors
+        q, k, wq, wk, _ = ctx.saved_tensors
         return (*E.headnorm_rotary_backward(gq, gk, q, k, wq, wk, ctx.eps, ctx.plan), None, None)
 
 
@@ -104,20 +104,22 @@ class PackedAttention(nn.Module):
       all sums are fp32 either way.  Inputs may be strided (slices of one projection, a cache of any layout with d contiguous).
       offsets_q, offsets_k [B + 1]: int32 on the device, not decreasing; sequence b owns rows offsets[b] .. offsets[b + 1] - 1 (`pack_offsets`).
       Without offsets_k the keys lie like the queries.  They are not read on the host; offsets outside the tensors are clamped on the device.
+      Up to 2^30 keys, and 2^30 query rows times heads per key head.
       k_len [B]: int32, used rows of each key sequence; the rest is room in a cache, never read into a result.
       A row that sees no key is 0 and takes no part in any gradient.  Rows of no sequence are zeros, in the gradients too.  Keys and values
-      that a row does not see may hold anything, infinities and NaN included (gradients want all of a sequence's own rows finite).
+      that a row does not see may hold anything, infinities and NaN included (gradients want all of a sequence's own rows finite).  A row that
+      sees one of those is not finite itself; one whose scores are all -infinity counts as a row that sees nothing.
       max_q, max_k: the longest sequences as far as the program knows them; they choose among the kernels (few rows per sequence over a cache,
       short sequences) and change nothing else: a wrong one costs time.
-      out: written in place of a new tensor (only without gradients); rows of no sequence stay as they were.
+      out: written in place of a new tensor (only without gradients, in memory of its own); rows of no sequence stay as they were.
       return_lse: also the logarithm of each row's sum of exponentials [Nq, heads], fp32, without a gradient; -inf where a row sees nothing.
 
     Serving: one query row per sequence (offsets_q = 0, 1, 2, ...) against a cache [B * room, kv_heads, d] with offsets_k = b * room and k_len."""
 
     def __init__(self, causal=False, temperature=None):
         super().__init__()
-        if temperature is not None and not (temperature > 0.0 and math.isfinite(temperature)):
-            raise ValueError(f"temperature {temperature}: must be positive")
+        if temperature is not None and not 1e-30 <= temperature <= 1e30:
+            raise ValueError(f"temperature {temperature}: must be positive, from 1e-30 to 1e30")
         self.causal, self.temperature = bool(causal), temperature
 
     def forward(self, q, k, v, offsets_q, offsets_k=None, k_len=None, max_q=None, max_k=None, out=None, return_lse=False):
@@ -148,7 +150,7 @@ class PackedAttention(nn.Module):
                 raise ValueError(f"{name} {m}: must not be negative")
         E.check_tokens(q=q, k=k, v=v)
         E.check_device(q=q, offsets_q=offsets_q, offsets_k=offsets_k, k_len=k_len)
-        hints = int(max_q or 0), int(max_k or 0)
+        hints = min(int(max_q or 0), q.shape[0]), min(int(max_k or 0), k.shape[0])
         temperature = math.sqrt(d) if self.temperature is None else float(self.temperature)
         if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
             if out is not None:
@@ -159,8 +161,12 @@ class PackedAttention(nn.Module):
                 E.check_tokens(q=q, out=out)
                 if out.shape != q.shape or not out.is_contiguous():
                     raise ValueError(f"out {tuple(out.shape)}: a contiguous tensor of q's shape {tuple(q.shape)} is required")
+                if out.requires_grad:
+                    raise ValueError("out is for calls without gradients: it requires one")
                 at = out.untyped_storage().data_ptr()
                 if at and any(t.untyped_storage().data_ptr() == at for t in (q, k, v)):
                     raise ValueError("out shares memory with an input")
             res, lse = E.packed_attention_forward(q, k, v, offsets_q, offsets_k, k_len, temperature, self.causal, return_lse, out, *hints)
+            if out is not None:
+                torch.autograd.graph.increment_version(out)         # a graph that saved it has to notice
         return (res, lse) if return_lse else res

@@ -42,12 +42,14 @@ class _RotaryFn(torch.autograd.Function):
     def forward(ctx, x, plan):
         from ... import engine as E
         ctx.plan = plan
+        ctx.save_for_backward(plan.positions)       # so that a change in place before the backward is an error
         return E.rotary_axes(x, plan)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
         from ... import engine as E
+        _ = ctx.saved_tensors
         return E.rotary_axes(dy, ctx.plan, inverse=True), None
 
 
@@ -61,7 +63,7 @@ class RotaryAxes(nn.Module):
     pairs: "halves" turns (i, i + n/2) of a section, "neighbours" (2i, 2i + 1).
 
     forward(x [..., heads, d], positions [..., axes]) -> the rotated tensor, contiguous, in x's storage type (fp32 or bf16).  positions:
-    int32, int64, fp32 or fp64, of any size (angles are reduced in 64 bits); they carry no gradient."""
+    int32, int64, fp32 or fp64, of any size (angles are reduced in 64 bits, which hold whole numbers up to 2^53); they carry no gradient."""
 
     def __init__(self, d, sections=None, T=10000.0, pairs="halves"):
         super().__init__()
