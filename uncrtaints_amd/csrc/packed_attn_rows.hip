@@ -15,7 +15,7 @@
 namespace {
 
 template <typename T, int DP, int NW, bool SHARE, bool VEC>
-__global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(SHARE ? 1 : DP <= 32 ? 4 : 2))) void packed_attn_rows_kernel(
+__global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(SHARE ? 1 : DP * sizeof(T) <= 64 ? 4 : DP <= 32 ? 3 : 2))) void packed_attn_rows_kernel(
     const AttnGeom g, const AttnTensor q, const AttnTensor k, const AttnTensor v, T* __restrict__ out, long long o_ts, long long o_hs,
     float* __restrict__ lse, float* __restrict__ work, int chunk, int splits, int tasks) {
     typedef AttnTile<T, DP> L;
@@ -30,128 +30,133 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(SHARE ?
     const int task = SHARE ? blockIdx.x : blockIdx.x * NW + wave;
     if (task >= tasks) return;
     const int hk = task % g.Hk, split = SHARE ? task / g.Hk % splits : 0, slot = SHARE ? task / g.Hk / splits : task / g.Hk;
-    int b, part;
-    if (!attn_find(g.off_q, g.B, g.Nq, g.G, 5, slot, b, part)) return;
+    int b = slot, part = 0;
+    if (SHARE && !attn_find(g.off_q, g.B, g.Nq, g.G, 5, slot, b, part)) return;
     const AttnSeq s = attn_seq(g, b);
-    const int rows = s.lq * g.G, row0 = part * 32;
-    if (row0 >= rows) return;
-    const int row = min(row0 + col, rows - 1), tok = row / g.G, head = hk * g.G + row - tok * g.G;
-    const int shift = s.lk - s.lq;
-    auto limit_of = [&](int r) { return g.causal ? min(max(min(r, rows - 1) / g.G + shift + 1, 0), s.lk) : s.lk; };
-    const int limit = limit_of(row), lo = limit_of(row0), hi = limit_of(row0 + 31);
-    // this block's keys: ranges of `chunk`, longer ones if `splits` of those do not reach the end
-    const int range = SHARE ? max(chunk, ((s.lk + splits - 1) / splits + 31) & ~31) : s.lk;
-    const int begin = split * range, end = min(hi, begin + range);
+    const int rows = s.lq * g.G;
+    // one tile of rows with shared waves, all of its sequence's for a wave of its own
+    for (int row0 = part * 32; row0 < rows; row0 += 32) {
+        const int row = min(row0 + col, rows - 1), tok = row / g.G, head = hk * g.G + row - tok * g.G;
+        const int shift = s.lk - s.lq;
+        auto limit_of = [&](int r) { return g.causal ? min(max(min(r, rows - 1) / g.G + shift + 1, 0), s.lk) : s.lk; };
+        const int limit = limit_of(row), lo = limit_of(row0), hi = limit_of(row0 + 31);
+        // this block's keys: ranges of `chunk`, longer ones if `splits` of those do not reach the end
+        const int range = SHARE ? max(chunk, ((s.lk + splits - 1) / splits + 31) & ~31) : s.lk;
+        const int begin = split * range, end = min(hi, begin + range);
 
-    AttnRows<T, DP> qf;
-    qf.template fetch_global<VEC>((const In*)q.p + (size_t)(s.q0 + tok) * q.ts + (size_t)head * q.hs, h, g.D);
-    AttnRun<T, DP> run;
-    run.reset();
-    const In* kb = (const In*)k.p + (size_t)s.k0 * k.ts + (size_t)hk * k.hs;
-    const In* vb = (const In*)v.p + (size_t)s.k0 * v.ts + (size_t)hk * v.hs;
-    Stage ks, vs;
-    constexpr int STEP = SHARE ? NW * 32 : 32;
-    int j0 = begin + (SHARE ? wave * 32 : 0), buf = 0;
-    if (j0 < end) {
-        ks.begin(lds[wave][0][0], kb, k.ts, j0, s.lk - 1, g.D);
-        vs.begin(lds[wave][0][1], vb, v.ts, j0, s.lk - 1, g.D);
-        ks.finish(lds[wave][0][0]);
-        vs.finish(lds[wave][0][1]);
-    }
-    for (; j0 < end; j0 += STEP) {
-        const bool more = j0 + STEP < end;
-        if (NBUF == 2 && more) {
-            attn_own_lds();
-            ks.begin(lds[wave][buf ^ 1][0], kb, k.ts, j0 + STEP, s.lk - 1, g.D);
-            vs.begin(lds[wave][buf ^ 1][1], vb, v.ts, j0 + STEP, s.lk - 1, g.D);
-            attn_arrived_but<VEC ? 2 * Stage::CNT : 0>();
-        } else {
-            attn_arrived();
+        AttnRows<T, DP> qf;
+        qf.template fetch_global<VEC>((const In*)q.p + (size_t)(s.q0 + tok) * q.ts + (size_t)head * q.hs, h, g.D);
+        AttnRun<T, DP> run;
+        run.reset();
+        const In* kb = (const In*)k.p + (size_t)s.k0 * k.ts + (size_t)hk * k.hs;
+        const In* vb = (const In*)v.p + (size_t)s.k0 * v.ts + (size_t)hk * v.hs;
+        Stage ks, vs;
+        constexpr int STEP = SHARE ? NW * 32 : 32;
+        int j0 = begin + (SHARE ? wave * 32 : 0), buf = 0;
+        if (j0 < end) {
+            ks.begin(lds[wave][0][0], kb, k.ts, j0, s.lk - 1, g.D);
+            vs.begin(lds[wave][0][1], vb, v.ts, j0, s.lk - 1, g.D);
+            ks.finish(lds[wave][0][0]);
+            vs.finish(lds[wave][0][1]);
         }
-        attn_own_lds();
-        run.tile(lds[wave][buf][0], lds[wave][buf][1], qf, g.c, j0, limit, j0 + 32 > lo, g.causal != 0, lane);
-        if (more) {
-            attn_own_lds();
-            if (NBUF == 1) {
-                ks.begin(lds[wave][0][0], kb, k.ts, j0 + STEP, s.lk - 1, g.D);
-                vs.begin(lds[wave][0][1], vb, v.ts, j0 + STEP, s.lk - 1, g.D);
+        for (; j0 < end; j0 += STEP) {
+            const bool more = j0 + STEP < end;
+            if (NBUF == 2 && more) {
+                attn_own_lds();
+                ks.begin(lds[wave][buf ^ 1][0], kb, k.ts, j0 + STEP, s.lk - 1, g.D);
+                vs.begin(lds[wave][buf ^ 1][1], vb, v.ts, j0 + STEP, s.lk - 1, g.D);
+                attn_arrived_but<VEC ? 2 * Stage::CNT : 0>();
+            } else {
+                attn_arrived();
             }
-            ks.finish(lds[wave][NBUF == 2 ? buf ^ 1 : 0][0]);
-            vs.finish(lds[wave][NBUF == 2 ? buf ^ 1 : 0][1]);
-        }
-        if (NBUF == 2) buf ^= 1;
-    }
-    float l = run.l + attn_other_half(run.l), m = run.m;
-    if (__any(run.odd))
-        attn_redo<T, DP>((const In*)q.p + (size_t)(s.q0 + tok) * q.ts + (size_t)head * q.hs, kb, k.ts, vb, v.ts, run.acc, g.D, g.c, m, limit,
-                         begin + (SHARE ? wave * 32 : 0), STEP, end, lane);
-    if (!SHARE) {
-        if (row0 + col >= rows) return;
-        attn_store_row<Out, L::DB>(out + (size_t)(s.q0 + tok) * o_ts + (size_t)head * o_hs, run.acc, attn_inv(l), h, g.D);
-        if (lse && h == 0) lse[(size_t)(s.q0 + tok) * g.Hq + head] = attn_lse(m, l);
-        return;
-    }
-    // the waves' sums, brought to one reference and added in LDS: [wave][row][DP] over the tiles, which no wave needs any more
-    if (h == 0) {
-        lds_m[wave][col] = m;
-        lds_l[wave][col] = l;
-    }
-    __syncthreads();
-    float mm = -INFINITY, ll = 0.f;
-#pragma unroll
-    for (int w = 0; w < NW; ++w) mm = fmaxf(mm, lds_m[w][col]);
-    const float ref = mm == -INFINITY ? 0.f : mm;
-#pragma unroll
-    for (int w = 0; w < NW; ++w) ll += lds_l[w][col] * __builtin_amdgcn_exp2f(lds_m[w][col] - ref);
-    const float f = __builtin_amdgcn_exp2f(m - ref);
-    const int live = min(rows - row0, 32);
-    constexpr int WB = NBUF * 2 * TILE / 4, ROWS = WB / DP < 32 ? WB / DP : 32;       // floats of a wave's tiles; rows of DP they hold
-    float* mine = (float*)&lds[wave][0][0][0];
-    for (int r0 = 0; r0 < live; r0 += ROWS) {
-        if (r0) __syncthreads();
-        if (col >= r0 && col < r0 + ROWS && col < live) {
-#pragma unroll
-            for (int db = 0; db < L::DB; ++db)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int d = db * 32 + 8 * e + 4 * h;
-                    if (d < DP)
-                        *reinterpret_cast<f32x4*>(mine + (col - r0) * DP + d) =
-                            (f32x4){run.acc[db][4 * e] * f, run.acc[db][4 * e + 1] * f, run.acc[db][4 * e + 2] * f, run.acc[db][4 * e + 3] * f};
+            attn_own_lds();
+            run.tile(lds[wave][buf][0], lds[wave][buf][1], qf, g.c, j0, limit, j0 + 32 > lo, g.causal != 0, lane);
+            if (more) {
+                attn_own_lds();
+                if (NBUF == 1) {
+                    ks.begin(lds[wave][0][0], kb, k.ts, j0 + STEP, s.lk - 1, g.D);
+                    vs.begin(lds[wave][0][1], vb, v.ts, j0 + STEP, s.lk - 1, g.D);
                 }
+                ks.finish(lds[wave][NBUF == 2 ? buf ^ 1 : 0][0]);
+                vs.finish(lds[wave][NBUF == 2 ? buf ^ 1 : 0][1]);
+            }
+            if (NBUF == 2) buf ^= 1;
+        }
+        float l = run.l + attn_other_half(run.l), m = run.m;
+        if (__any(run.odd))
+            attn_redo<T, DP>((const In*)q.p + (size_t)(s.q0 + tok) * q.ts + (size_t)head * q.hs, kb, k.ts, vb, v.ts, run.acc, g.D, g.c, m, limit,
+                             begin + (SHARE ? wave * 32 : 0), STEP, end, lane);
+        if (!SHARE) {
+            if (row0 + col < rows) {
+                attn_store_row<Out, L::DB>(out + (size_t)(s.q0 + tok) * o_ts + (size_t)head * o_hs, run.acc, attn_inv(l), h, g.D);
+                if (lse && h == 0) lse[(size_t)(s.q0 + tok) * g.Hq + head] = attn_lse(m, l);
+            }
+            attn_own_lds();
+            continue;
+        }
+        // the waves' sums, brought to one reference and added in LDS: [wave][row][DP] over the tiles, which no wave needs any more
+        if (h == 0) {
+            lds_m[wave][col] = m;
+            lds_l[wave][col] = l;
         }
         __syncthreads();
-        const int n = min(live - r0, ROWS);
-        for (int i = threadIdx.x; i < n * DP; i += NW * 64) {
-            const int r = i / DP, d = i % DP;
-            if (d >= g.D) continue;
-            float a = 0.f, lr = 0.f, mr = -INFINITY;
+        float mm = -INFINITY, ll = 0.f;
 #pragma unroll
-            for (int w = 0; w < NW; ++w) {
-                a += *((const float*)&lds[w][0][0][0] + i);
-                mr = fmaxf(mr, lds_m[w][r0 + r]);
+        for (int w = 0; w < NW; ++w) mm = fmaxf(mm, lds_m[w][col]);
+        const float ref = mm == -INFINITY ? 0.f : mm;
+#pragma unroll
+        for (int w = 0; w < NW; ++w) ll += lds_l[w][col] * __builtin_amdgcn_exp2f(lds_m[w][col] - ref);
+        const float f = __builtin_amdgcn_exp2f(m - ref);
+        const int live = min(rows - row0, 32);
+        constexpr int WB = NBUF * 2 * TILE / 4, ROWS = WB / DP < 32 ? WB / DP : 32;       // floats of a wave's tiles; rows of DP they hold
+        float* mine = (float*)&lds[wave][0][0][0];
+        for (int r0 = 0; r0 < live; r0 += ROWS) {
+            if (r0) __syncthreads();
+            if (col >= r0 && col < r0 + ROWS && col < live) {
+#pragma unroll
+                for (int db = 0; db < L::DB; ++db)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int d = db * 32 + 8 * e + 4 * h;
+                        if (d < DP)
+                            *reinterpret_cast<f32x4*>(mine + (col - r0) * DP + d) =
+                                (f32x4){run.acc[db][4 * e] * f, run.acc[db][4 * e + 1] * f, run.acc[db][4 * e + 2] * f, run.acc[db][4 * e + 3] * f};
+                    }
             }
-            const int rr = row0 + r0 + r, t = rr / g.G;
-            const size_t at = (size_t)(s.q0 + t) * g.Hq + hk * g.G + rr - t * g.G;
+            __syncthreads();
+            const int n = min(live - r0, ROWS);
+            for (int i = threadIdx.x; i < n * DP; i += NW * 64) {
+                const int r = i / DP, d = i % DP;
+                if (d >= g.D) continue;
+                float a = 0.f, lr = 0.f, mr = -INFINITY;
+#pragma unroll
+                for (int w = 0; w < NW; ++w) {
+                    a += *((const float*)&lds[w][0][0][0] + i);
+                    mr = fmaxf(mr, lds_m[w][r0 + r]);
+                }
+                const int rr = row0 + r0 + r, t = rr / g.G;
+                const size_t at = (size_t)(s.q0 + t) * g.Hq + hk * g.G + rr - t * g.G;
+                if (splits > 1) {
+                    if (mr != -INFINITY) work[((size_t)split * g.Nq * g.Hq + at) * g.D + d] = a;
+                } else {
+                    const float rf = mr == -INFINITY ? 0.f : mr;
+#pragma unroll
+                    for (int w = 0; w < NW; ++w) lr += lds_l[w][r0 + r] * __builtin_amdgcn_exp2f(lds_m[w][r0 + r] - rf);
+                    out[(size_t)(s.q0 + t) * o_ts + (size_t)(hk * g.G + rr - t * g.G) * o_hs + d] = (T)(a * attn_inv(lr));
+                }
+            }
+        }
+        if (wave == 0 && h == 0 && col < live) {
+            const size_t at = (size_t)(s.q0 + tok) * g.Hq + head;
             if (splits > 1) {
-                if (mr != -INFINITY) work[((size_t)split * g.Nq * g.Hq + at) * g.D + d] = a;
-            } else {
-                const float rf = mr == -INFINITY ? 0.f : mr;
-#pragma unroll
-                for (int w = 0; w < NW; ++w) lr += lds_l[w][r0 + r] * __builtin_amdgcn_exp2f(lds_m[w][r0 + r] - rf);
-                out[(size_t)(s.q0 + t) * o_ts + (size_t)(hk * g.G + rr - t * g.G) * o_hs + d] = (T)(a * attn_inv(lr));
+                float* ml = work + (size_t)splits * g.Nq * g.Hq * g.D + ((size_t)split * g.Nq * g.Hq + at) * 2;
+                ml[0] = mm;
+                ml[1] = ll;
+            } else if (lse) {
+                lse[at] = attn_lse(mm, ll);
             }
         }
-    }
-    if (wave == 0 && h == 0 && col < live) {
-        const size_t at = (size_t)(s.q0 + tok) * g.Hq + head;
-        if (splits > 1) {
-            float* ml = work + (size_t)splits * g.Nq * g.Hq * g.D + ((size_t)split * g.Nq * g.Hq + at) * 2;
-            ml[0] = mm;
-            ml[1] = ll;
-        } else if (lse) {
-            lse[at] = attn_lse(mm, ll);
-        }
+        return;
     }
 }
 
@@ -417,7 +422,7 @@ struct Rows {
 };
 
 template <typename T, int DP, int NW, bool SHARE, bool VEC> bool launch(const Rows& a) {
-    const int tasks = attn_slots((long long)a.g.Nq * a.g.G, a.g.B, 5) * a.g.Hk * (SHARE ? a.s.splits : 1);
+    const int tasks = SHARE ? attn_slots((long long)a.g.Nq * a.g.G, a.g.B, 5) * a.g.Hk * a.s.splits : a.g.B * a.g.Hk;
     const long long blocks = SHARE ? tasks : ((long long)tasks + NW - 1) / NW;
     if (!attn_grid(blocks, NW * 64)) return false;
     hipLaunchKernelGGL((packed_attn_rows_kernel<T, DP, NW, SHARE, VEC>), dim3((unsigned)blocks), dim3(NW * 64), 0, a.stream, a.g, a.q,
