@@ -25,7 +25,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(SHARE ?
     constexpr int NBUF = SHARE ? 2 : 1, TILE = 32 * L::RB;
     __shared__ alignas(16) char lds[NW][NBUF][2][TILE];
     __shared__ float lds_m[NW][32], lds_l[NW][32];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5, col = lane & 31;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5, col = lane & 31;
     if (g.fill) attn_fill_outside<Out>(g.off_q, g.B, g.Nq, out, o_ts, o_hs, g.Hq, g.D, lse, blockIdx.x, gridDim.x);
     const int task = SHARE ? blockIdx.x : blockIdx.x * NW + wave;
     if (task >= tasks) return;
@@ -237,7 +237,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(DP <= 3
     __shared__ alignas(16) char lds[NW][4][TILE];
     __shared__ alignas(16) float patch[NW][32 * PS];
     __shared__ float lds_d[sizeof(T) == 2 ? NW : 1][64];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5, col = lane & 31;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5, col = lane & 31;
     attn_fill_outside<Out>(g.off_q, g.B, g.Nq, dq, (long long)g.Hq * g.D, g.D, g.Hq, g.D, nullptr, blockIdx.x, gridDim.x);
     attn_fill_outside<Out>(g.off_k, g.B, g.Nk, dk, (long long)g.Hk * g.D, g.D, g.Hk, g.D, nullptr, blockIdx.x, gridDim.x);
     attn_fill_outside<Out>(g.off_k, g.B, g.Nk, dv, (long long)g.Hk * g.D, g.D, g.Hk, g.D, nullptr, blockIdx.x, gridDim.x);
