@@ -469,17 +469,19 @@ template <typename P> struct AttnCursor {
 };
 
 // column `col`'s accumulators acc[DB] (d = 32 db + 8 (i / 4) + 4 h + i % 4) times f into a row of D elements
-template <typename T, int DB> __device__ __forceinline__ void attn_store_row(T* row, const f32x16 (&acc)[DB], float f, int h, int D) {
+template <typename T, int DB, int DP = DB * 32> __device__ __forceinline__ void attn_store_row(T* row, const f32x16 (&acc)[DB], float f, int h, int D) {
     typedef T T4 __attribute__((ext_vector_type(4)));
+    const bool whole = (D & 3) == 0;
 #pragma unroll
     for (int db = 0; db < DB; ++db)
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
+            if (db * 32 + q * 8 >= DP) continue;
             const int d = db * 32 + q * 8 + h * 4;
             T4 v;
 #pragma unroll
             for (int i = 0; i < 4; ++i) v[i] = (T)(acc[db][4 * q + i] * f);
-            if ((D & 3) == 0) {
+            if (whole) {
                 if (d < D) __builtin_memcpy(__builtin_assume_aligned(row + d, sizeof(T) * 4), &v, sizeof(v));
             } else {
 #pragma unroll

@@ -22,7 +22,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(AttnTil
     typedef typename AttnElem<T>::Out Out;
     constexpr int NT = NW * 64, GROUPS = NW / KSPLIT, BM = GROUPS * 32, SHIFT = BM == 256 ? 8 : BM == 128 ? 7 : 6;
     __shared__ alignas(16) char lds_k[2][TK * L::RB], lds_v[2][TK * L::RB];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5, col = lane & 31;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5, col = lane & 31;
     if (g.fill) attn_fill_outside<Out>(g.off_q, g.B, g.Nq, out, o_ts, o_hs, g.Hq, g.D, lse, blockIdx.x, gridDim.x);
     const int hk = blockIdx.x % g.Hk;
     int b, tile;

@@ -88,7 +88,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(SHARE ?
                              begin + (SHARE ? wave * 32 : 0), STEP, end, lane);
         if (!SHARE) {
             if (row0 + col < rows) {
-                attn_store_row<Out, L::DB>(out + (size_t)(s.q0 + tok) * o_ts + (size_t)head * o_hs, run.acc, attn_inv(l), h, g.D);
+                attn_store_row<Out, L::DB, DP>(out + (size_t)(s.q0 + tok) * o_ts + (size_t)head * o_hs, run.acc, attn_inv(l), h, g.D);
                 if (lse && h == 0) lse[(size_t)(s.q0 + tok) * g.Hq + head] = attn_lse(m, l);
             }
             attn_own_lds();
@@ -332,7 +332,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(DP <= 3
         }
     };
     auto store_dq = [&](int r0, const f32x16 (&a)[L::DB]) {
-        if (r0 + col < rows) attn_store_row<Out, L::DB>(dq + at * g.D, a, g.scale, h, g.D);
+        if (r0 + col < rows) attn_store_row<Out, L::DB, DP>(dq + at * g.D, a, g.scale, h, g.D);
     };
     if (round) {
         for (int r0 = 0; r0 < rows; r0 += 32) {
@@ -390,8 +390,8 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(DP <= 3
 #pragma unroll
                 for (int db = 0; db < L::DB; ++db) ak[db] = av[db] = (f32x16)(0.f);
             const size_t ka = ((size_t)(s.k0 + j0 + col) * g.Hk + hk) * g.D;
-            attn_store_row<Out, L::DB>(dk + ka, ak, g.scale, h, g.D);
-            attn_store_row<Out, L::DB>(dv + ka, av, 1.f, h, g.D);
+            attn_store_row<Out, L::DB, DP>(dk + ka, ak, g.scale, h, g.D);
+            attn_store_row<Out, L::DB, DP>(dv + ka, av, 1.f, h, g.D);
         }
     }
     if (single && s.lk > 0) return;
