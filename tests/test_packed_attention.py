@@ -638,3 +638,24 @@ def test_scales_and_sizes_beyond_the_built_ones_are_refused():
                                                  work=None, temperature=1.0, B=big, Nq=big, Nk=big, Hq=128, Hk=128, D=8, stream=None)}
     for kw in (dict(), dict(max_q=1, max_k=60), dict(Nq=0), dict(D=128)):
         assert hb.lib().fn["uncr_packed_attn_bwd"](*{**ok, **kw}.values()) == shape, kw
+
+
+@gpu
+@MASK
+@BOTH
+@pytest.mark.parametrize("hq, hk, d", [(3, 3, 16), (4, 2, 32), (2, 2, 64), (6, 2, 40), (2, 2, 128), (3, 1, 72), (2, 1, 127)])
+def test_many_short_sequences_with_many_rows(hq, hk, d, dtype, causal):
+    """Enough sequences for whole launches of the smaller blocks (up to 64 rows and 48 keys on average), some of them far longer"""
+    g = _gen(70)
+    lq = [int(n) for n in torch.randint(0, 45, (1100 // hk,), generator=g)] + [1, 150, 0, 64, 65]
+    _run(lq, lq, hq, hk, d, causal, dtype, seed=71, hints=False, front=2, behind=3)
+
+
+@gpu
+@MASK
+@BOTH
+def test_many_short_sequences_over_other_keys(dtype, causal):
+    g = _gen(72)
+    lq = [int(n) for n in torch.randint(30, 45, (600,), generator=g)]
+    lk = [int(n) for n in torch.randint(0, 80, (600,), generator=g)]
+    _run(lq, lk, 4, 2, 128, causal, dtype, room=[n + 3 for n in lk], seed=73, hints=False)

@@ -122,6 +122,13 @@ template <bool KEYS> __device__ __forceinline__ bool attn_find_sorted(const Attn
 // waves pair up and share the keys of each tile (two sequences of 4096 and 1587 tokens, 8 heads of 32, fp32: forward
 // 254 -> 225 us, dQ 358 -> 313 us)
 static inline bool attn_few_blocks(const AttnGeom& g, int rows) { return (((long long)g.Nq * g.G / rows) + g.B) * g.Hk < 1024; }
+// Sequences of up to 64 rows on average: blocks of two waves and tiles of 32 keys, four or more per CU, where larger blocks would have most of
+// their waves without rows (1500 causal series of up to 64 tokens, 4 heads of 128, bf16: forward 187 -> 67 us, dQ 243 -> 97; up to 60, 8/4
+// heads of 64: 66 -> 44 and 90 -> 70; fp32, 4 heads of 128: 393 -> 214 and 487 -> 263).  Up to 48 keys: blocks of 64 keys in dK/dV (those of 64,
+// bf16: 184 -> 104 us, fp32: 450 -> 263; 4 heads of 128, bf16, whose tiles of rows are half as long then: 209 -> 121).  Where a launch has few
+// blocks, the half-size blocks above share the keys instead.
+static inline bool attn_low_rows(const AttnGeom& g) { return (long long)g.Nq * g.G <= 64ll * g.B; }
+static inline bool attn_low_keys(const AttnGeom& g) { return g.Nk <= 48ll * g.B; }
 // Sorting costs a block about 2 us: for causal sequences of at least four tiles on average
 static inline bool attn_sorts(const AttnGeom& g, long long rows, int per_tile) {
     return g.causal && g.B <= ATTN_SORT_MAX_B && rows / per_tile >= 4ll * g.B && (long long)g.Nk * g.G < (1ll << 29) && (long long)g.G * per_tile < (1 << 20);

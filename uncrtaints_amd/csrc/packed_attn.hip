@@ -177,7 +177,9 @@ bool launch_k(AttnGeom g, const AttnTensor& q, const AttnTensor& k, const AttnTe
 template <typename T, int DP, int NW, int TK>
 bool launch(const AttnGeom& g, const AttnTensor& q, const AttnTensor& k, const AttnTensor& v, void* out, long long o_ts, long long o_hs, float* lse,
             bool vec, hipStream_t stream) {
+    constexpr int LOW_NW = AttnElem<T>::THREE ? NW : 2, LOW_TK = AttnElem<T>::THREE ? TK : 32;
     if (TK == 64 && attn_few_blocks(g, NW * 32)) return launch_k<T, DP, NW, TK, TK == 64 ? 2 : 1>(g, q, k, v, out, o_ts, o_hs, lse, vec, stream);
+    if (!AttnElem<T>::THREE && attn_low_rows(g)) return launch_k<T, DP, LOW_NW, LOW_TK, 1>(g, q, k, v, out, o_ts, o_hs, lse, vec, stream);
     return launch_k<T, DP, NW, TK, 1>(g, q, k, v, out, o_ts, o_hs, lse, vec, stream);
 }
 

@@ -173,7 +173,7 @@ __global__ __launch_bounds__(PAIRS * 128) __attribute__((amdgpu_waves_per_eu(2))
     typedef AttnTile<T, DP> L;
     typedef typename AttnElem<T>::In In;
     typedef typename AttnElem<T>::Out Out;
-    constexpr int NT = PAIRS * 128, BN = PAIRS * 32, SHIFT = PAIRS == 4 ? 7 : 6, TQ = sizeof(T) == 2 ? 64 : 32;      // AttnThree, fp32: 32
+    constexpr int NT = PAIRS * 128, BN = PAIRS * 32, SHIFT = PAIRS == 4 ? 7 : 6, TQ = sizeof(T) == 2 && (PAIRS == 4 || L::RB <= 128) ? 64 : 32;      // AttnThree, fp32: 32
     constexpr bool EARLY = L::RB <= 256;       // registers for the transposed operand beside the first product (not for fp32 rows of 512 bytes)
     __shared__ alignas(16) char lds_q[3][TQ * L::RB], lds_g[3][TQ * L::RB];
     __shared__ f32x4 lds_p[2][PAIRS][TQ / 32][AttnPass<T>::PARTS][64];
@@ -369,12 +369,17 @@ template <typename T, int DP, int PAIRS, bool VEC> bool launch_dkv(const Bwd& a)
 }
 template <typename T, int DP, int NW, int TK, bool VEC> bool launch_v(const Bwd& a) {
     if (a.g.Nq) {
-        if (!(TK == 64 && attn_few_blocks(a.g, NW * 32) ? launch_dq<T, DP, NW, TK, TK == 64 ? 2 : 1, VEC>(a) : launch_dq<T, DP, NW, TK, 1, VEC>(a))) return false;
+        constexpr int LOW_NW = AttnElem<T>::THREE ? NW : 2, LOW_TK = AttnElem<T>::THREE ? TK : 32;
+        const bool fits = TK == 64 && attn_few_blocks(a.g, NW * 32)         ? launch_dq<T, DP, NW, TK, TK == 64 ? 2 : 1, VEC>(a)
+                          : !AttnElem<T>::THREE && attn_low_rows(a.g) ? launch_dq<T, DP, LOW_NW, LOW_TK, 1, VEC>(a)
+                                                                      : launch_dq<T, DP, NW, TK, 1, VEC>(a);
+        if (!fits) return false;
     }
     if (a.g.Nk) {
-        // two pairs per block: as long as two blocks fit a CU's LDS
-        constexpr bool SMALL = AttnTile<T, DP>::RB <= (AttnElem<T>::THREE ? 192 : 128);
+        // two pairs per block: as long as two blocks fit a CU's LDS (heads of 128: with tiles of 32 rows, for which long sequences would pay)
+        constexpr bool SMALL = AttnTile<T, DP>::RB <= (AttnElem<T>::THREE ? 192 : 128), LOW = !AttnElem<T>::THREE && AttnTile<T, DP>::RB <= 256;
         if (SMALL && ((long long)a.g.Nk / 128 + a.g.B) * a.g.Hk < 1024) return launch_dkv<T, DP, SMALL ? 2 : 4, VEC>(a);
+        if (LOW && attn_low_keys(a.g)) return launch_dkv<T, DP, LOW ? 2 : 4, VEC>(a);
         return launch_dkv<T, DP, 4, VEC>(a);
     }
     return true;

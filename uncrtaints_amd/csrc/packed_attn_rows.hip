@@ -6,10 +6,10 @@
 //           exponentials are joined by a second launch.
 //   short:  both sides are at most two tiles: each wave has a sequence and head of its own (a block of the kernels in packed_attn.hip
 //           would leave three of its four waves without rows), and the backward makes all three gradients in one pass over one tile.
-// Measured: 24 caches of 331 to 32768 keys, 32/8 heads of 128, bf16: 397 us for 1.88 GB, 4.7 TB/s where a large copy reaches 4.96 (the kernel
-// of packed_attn.hip alone: 1043); one token over 1000 keys, 16/4 heads of 64: 10 us in one launch, bound by the loads that wait for each
-// other (23 us there).  1500 series of up to 30 dates, 16 heads of 16, fp32: forward 49 us, backward 88 (332 and 930 there); half of that is
-// the 272 MB they move, the rest products of 32 x 32 tiles that are a quarter full.
+// Measured: 24 caches of 331 to 32768 keys, 32/8 heads of 128, bf16: 396 us for 1.88 GB, 4.7 TB/s where a large copy reaches 4.96 (the kernel
+// of packed_attn.hip alone: 1043); one token over 1000 keys, 16/4 heads of 64: 9.6 us in one launch, bound by the loads that wait for each
+// other (23 us there).  1500 series of up to 30 dates, 16 heads of 16, fp32: forward 43 us, backward 81 (332 and 930 there); the 272 MB they
+// move would take 55, the rest are the vector instructions and products of 32 x 32 tiles that are a quarter full.
 #include "packed_attn.h"
 
 namespace {
