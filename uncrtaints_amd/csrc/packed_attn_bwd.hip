@@ -5,9 +5,10 @@
 // That is 7 products instead of the 5 of a single kernel that would add its share of dQ to memory from every key tile -- but no atomics: the
 // result does not depend on the order blocks run in, and no fp32 copy of dQ is written, read back and rounded.  The group's heads are
 // consecutive rows of one problem, so dK and dV are sums inside a block as well.
-// Bound: the matrix units, and in dK/dV the LDS reads beside them (four operands of 8 KB for every 32 x 32 tile).  Five causal sequences of
-// 2832 to 5000 tokens, 16/4 heads of 128, bf16: dQ 540 us (907 TFLOP/s), dK/dV 800 us (816).  Two sequences of 4096 and 1587 tokens, 8 heads
-// of 32, fp32 in three bf16 parts: dQ 193 us, dK/dV 301 (in fp32 products 289 and 398).
+// Bound: the matrix units, and in dK/dV the LDS reads beside them (four operands of 8 KB for every 32 x 32 tile).  Fastest launches: five causal
+// sequences of 2832 to 5000 tokens, 16/4 heads of 128, bf16: dQ 533 us (919 TFLOP/s), dK/dV 793 us (823); the clock falls with the power, the
+// medians are 5 % above.  Two sequences of 4096 and 1587 tokens, 8 heads of 32, fp32 in three bf16 parts: dQ 190 us, dK/dV 305 (in fp32 products
+// 289 and 398).
 #include "packed_attn.h"
 
 namespace {

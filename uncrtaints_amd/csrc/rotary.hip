@@ -10,6 +10,8 @@
 // keys, into LDS -- the angle in turns in 64 bits (fp32 loses the angle of a far position: 2^-24 * pos * freq radians), reduced, then sincospi
 // in fp32.  A group of `lpr` lanes then takes one token and every `strands`-th head: its pairs' (cos, sin) sit in registers, each head is C
 // pairs per lane loaded as up to 16-byte vectors.  At least four heads per group where there are that many, so the angles' cost is spread.
+// Measured, bf16: 65537 tokens, 40 heads of 128, rotation 262 us (5.1 TB/s; a large copy 4.96); 40001 tokens, 32 + 8 heads of 128, norms and
+// rotation 159 us, gradient 245 us and 5 us for the sums of dw (5.1 and 5.0 TB/s).  One token: 3 us.
 #include "common.h"
 
 namespace {
