@@ -659,3 +659,28 @@ def test_many_short_sequences_over_other_keys(dtype, causal):
     lq = [int(n) for n in torch.randint(30, 45, (600,), generator=g)]
     lk = [int(n) for n in torch.randint(0, 80, (600,), generator=g)]
     _run(lq, lk, 4, 2, 128, causal, dtype, room=[n + 3 for n in lk], seed=73, hints=False)
+
+
+def _compiles(tmp_path, body):
+    """Does a kernel with this body, next to the attention kernels' header, compile? -> (status, messages)"""
+    import os
+    import subprocess
+    from uncrtaints_amd import build
+    src = tmp_path / "probe.hip"
+    src.write_text('#include "packed_attn.h"\n__global__ void probe(float* out) {\n' + body + "\n}\n")
+    r = subprocess.run([os.environ.get("HIPCC", "/opt/rocm/bin/hipcc"), "--offload-arch=gfx950", "-std=c++17", "-fsyntax-only", "-I" + build.CSRC, str(src)],
+                       capture_output=True, text=True, timeout=100)
+    return r.returncode, r.stdout + r.stderr
+
+
+def test_the_sums_of_joining_waves_stay_inside_one_lds_object(tmp_path):
+    """Forward and dQ blocks whose waves share the keys (half as many groups as waves) add their sums through the tiles' LDS: every built
+    instance's sums lie inside the object they are addressed in, and a geometry whose sums do not is no program."""
+    built = [("__bf16", 32, 64, 2), ("__bf16", 64, 64, 2), ("__bf16", 128, 64, 4), ("float", 32, 64, 2), ("float", 64, 64, 2), ("AttnThree", 32, 64, 2)]
+    body = "".join(f"{{ __shared__ AttnBuffers<{t}, {dp}, {tk}> b; float* p = b.template join<{groups}>({groups} - 1);\n"
+                   f"  static_assert(sizeof(b) == sizeof(b.k) + sizeof(b.v)); p[{max(dp, 32) // 32} * 1024 - 1] = 0.f; out[0] = p[0]; }}\n"
+                   for t, dp, tk, groups in built)
+    status, said = _compiles(tmp_path, body)
+    assert status == 0, said
+    status, said = _compiles(tmp_path, "__shared__ AttnBuffers<__bf16, 128, 32> b; out[0] = b.template join<4>(3)[0];")
+    assert status != 0 and "do not hold the sums" in said

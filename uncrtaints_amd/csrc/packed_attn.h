@@ -194,6 +194,18 @@ template <typename T, int DP> struct AttnTile {
     static __device__ __forceinline__ int part_at(int c) { return c % CPR / NCH; }
 };
 
+// The two buffers of key and value tiles of a block, in ONE object: once nobody needs the tiles any more, the waves that shared the keys add
+// their sums through all of it (bf16 heads of 128: 64 KB, which the keys' buffers alone would not hold)
+template <typename T, int DP, int TK> struct AttnBuffers {
+    typedef AttnTile<T, DP> L;
+    char k[2][TK * L::RB], v[2][TK * L::RB];
+    // accumulators of group `i` of GROUPS pairs of waves: [DB * 16][64 lanes]
+    template <int GROUPS> __device__ __forceinline__ float* join(int i) {
+        static_assert(sizeof(float) * GROUPS * L::DB * 16 * 64 <= sizeof(AttnBuffers), "the tiles do not hold the sums of the waves that join");
+        return (float*)this + i * (L::DB * 16 * 64);
+    }
+};
+
 // Operands are fetched from LDS in one go and used after it (`attn_fence` keeps the compiler from sinking each read to its use, where
 // every product waits for the latency of its own operand)
 __device__ __forceinline__ void attn_fence() { __builtin_amdgcn_sched_barrier(0); }

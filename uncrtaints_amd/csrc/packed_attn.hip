@@ -21,7 +21,8 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(AttnTil
     typedef typename AttnElem<T>::In In;
     typedef typename AttnElem<T>::Out Out;
     constexpr int NT = NW * 64, GROUPS = NW / KSPLIT, BM = GROUPS * 32, SHIFT = BM == 256 ? 8 : BM == 128 ? 7 : 6;
-    __shared__ alignas(16) char lds_k[2][TK * L::RB], lds_v[2][TK * L::RB];
+    __shared__ alignas(16) AttnBuffers<T, DP, TK> lds;
+    auto &lds_k = lds.k, &lds_v = lds.v;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5, col = lane & 31;
     if (g.fill) attn_fill_outside<Out>(g.off_q, g.B, g.Nq, out, o_ts, o_hs, g.Hq, g.D, lse, blockIdx.x, gridDim.x);
     const int hk = blockIdx.x % g.Hk;
@@ -133,8 +134,8 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(AttnTil
     if (__any(odd))
         attn_redo<T, DP>((const In*)q.p + (size_t)(s.q0 + tok) * q.ts + (size_t)head * q.hs, kb, k.ts, vb, v.ts, acc, g.D, g.c, m, limit, share * 32,
                          KSPLIT * 32, wave_hi, lane);
-    if (KSPLIT == 2) {          // the second wave's sums to the first one, through the tiles nobody needs any more
-        float* pass = (float*)&lds_k[0][0] + wave % GROUPS * (L::DB * 16 * 64);
+    if constexpr (KSPLIT == 2) {          // the second wave's sums to the first one, through the tiles nobody needs any more
+        float* pass = lds.template join<GROUPS>(wave % GROUPS);
         __shared__ float pass_m[GROUPS][64], pass_l[GROUPS][64];
         if (share) {
 #pragma unroll

@@ -21,7 +21,8 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(AttnTil
     typedef typename AttnElem<T>::In In;
     typedef typename AttnElem<T>::Out Out;
     constexpr int NT = NW * 64, GROUPS = NW / KSPLIT, BM = GROUPS * 32, SHIFT = BM == 256 ? 8 : BM == 128 ? 7 : 6;
-    __shared__ alignas(16) char lds_k[2][TK * L::RB], lds_v[2][TK * L::RB];
+    __shared__ alignas(16) AttnBuffers<T, DP, TK> lds;
+    auto &lds_k = lds.k, &lds_v = lds.v;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5, col = lane & 31;
     attn_fill_outside<Out>(g.off_q, g.B, g.Nq, dq, (long long)g.Hq * g.D, g.D, g.Hq, g.D, nullptr, blockIdx.x, gridDim.x);
     const int hk = blockIdx.x % g.Hk;
@@ -144,8 +145,8 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(AttnTil
         attn_arrived();
         __syncthreads();
     }
-    if (KSPLIT == 2) {          // the second wave's sum to the first one, through the tiles nobody needs any more
-        float* pass = (float*)&lds_k[0][0] + wave % GROUPS * (L::DB * 16 * 64);
+    if constexpr (KSPLIT == 2) {          // the second wave's sum to the first one, through the tiles nobody needs any more
+        float* pass = lds.template join<GROUPS>(wave % GROUPS);
         if (share) {
 #pragma unroll
             for (int db = 0; db < L::DB; ++db)
