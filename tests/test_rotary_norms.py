@@ -329,3 +329,27 @@ def test_more_tokens_than_are_counted_are_refused():
               H=1, D=256, act=0, stream=None)
     fn = hb.lib().fn["uncr_rotary_axes"]
     assert fn(*ok.values()) == fn(*{**ok, "H": 0}.values()) < 0
+
+
+def _norm_gradients(q, k, m, eps):
+    """The norms' gradients (no rotation) against the formula's in 64 bits, within this file's bounds: u is dy itself here."""
+    gq, gk = torch.randn(q.shape, generator=_gen(61)).to(q.dtype), torch.randn(k.shape, generator=_gen(62)).to(k.dtype)
+    qd, kd = q.to(DEV).requires_grad_(), k.to(DEV).requires_grad_()
+    grads = torch.autograd.grad(m(qd, kd), (qd, kd, m.q_weight, m.k_weight), (gq.to(DEV), gk.to(DEV)))
+    for name, x, g, w, dx, dw in (("q", q, gq, m.q_weight, grads[0], grads[2]), ("k", k, gk, m.k_weight, grads[1], grads[3])):
+        x, g, w = x.double(), g.double(), w.detach().cpu().double()
+        r = 1.0 / (x.square().mean(-1, keepdim=True) + eps).sqrt()
+        xh = x * r
+        ref = r * (w * g - xh * (w * g * xh).mean(-1, keepdim=True))
+        _check("d" + name, dx, ref, 64 * U * r * ((w * g).abs() + xh.abs() * (w * g * xh).abs().mean(-1, keepdim=True)) + _half(q.dtype) * ref.abs())
+        _check("dw" + name, dw, (g * xh).sum((0, 1)), (64 + 512) * U * (g * xh).abs().sum((0, 1)))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("n", [1, 3, 53])
+@pytest.mark.parametrize("d,hq,hk", [(128, 8, 2), (16, 1, 1), (64, 3, 2), (6, 2, 1)])
+def test_norm_gradients_without_eps_where_the_last_tokens_fill_no_wave(d, hq, hk, n, dtype):
+    from uncrtaints_amd.src.backbones.packed_attention import HeadNormRotary
+    q, k = (torch.randn(n, h, d, generator=_gen(70 + h)).to(dtype) for h in (hq, hk))
+    _norm_gradients(q, k, HeadNormRotary(d, eps=0.0).to(DEV), 0.0)

@@ -290,6 +290,7 @@ __global__ __launch_bounds__(ROT_THREADS) void headnorm_bwd_kernel(const RotGeom
                         const float r = rsqrtf(ss / (float)g.D + eps);
 #pragma unroll
                         for (int i = 0; i < C; ++i) {
+                            if (!on[m]) continue;         // a group behind the last token: r = 1 / sqrt(eps), infinite without eps
                             dwa[which][m][i] = fmaf(ga[i], r, dwa[which][m][i]);
                             dwb[which][m][i] = fmaf(gb[i], r, dwb[which][m][i]);
                         }
