@@ -353,3 +353,18 @@ def test_norm_gradients_without_eps_where_the_last_tokens_fill_no_wave(d, hq, hk
     from uncrtaints_amd.src.backbones.packed_attention import HeadNormRotary
     q, k = (torch.randn(n, h, d, generator=_gen(70 + h)).to(dtype) for h in (hq, hk))
     _norm_gradients(q, k, HeadNormRotary(d, eps=0.0).to(DEV), 0.0)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("d,hq,hk", [(64, 4, 2), (40, 3, 1), (202, 2, 2), (256, 8, 1)])
+def test_norm_gradients_of_very_large_and_very_small_rows(d, hq, hk, dtype):
+    from uncrtaints_amd.src.backbones.packed_attention import HeadNormRotary
+    scale = torch.tensor([1.0, 1e15, 1e16, 1e17, 1e-6, 1e-10, 1e-13, 1e-17]).view(8, 1, 1)
+    q, k = (scale * torch.randn(8, h, d, generator=_gen(60 + h))  for h in (hq, hk))
+    q, k = q.to(dtype), k.to(dtype)
+    m = HeadNormRotary(d, eps=0.0).to(DEV)
+    _norm_gradients(q, k, m, 0.0)
+    m = HeadNormRotary(d, eps=1e-30).to(DEV)
+    q[2] = 0.0
+    _norm_gradients(q, k, m, 1e-30)

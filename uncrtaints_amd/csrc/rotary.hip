@@ -2,7 +2,7 @@
 //
 //   angle(p) = pos[token][axis(p)] * freq(p);   (a, b) -> (a cos - b sin, a sin + b cos)   for the pair p = (a, b) of a head vector
 //   norm:  y = R(angle) (w * x * r),  r = 1 / sqrt(mean(x^2) + eps)    (mean over the head's D values)
-//   its gradient, u = R(-angle) dy:   dx = r * (w u) - x * r^3 / D * sum(w u x),   dw = sum over tokens and heads of u * x * r
+//   its gradient, u = R(-angle) dy, xhat = x r:   dx = r * (w u - xhat * mean(w u xhat)),   dw = sum over tokens and heads of u * xhat
 //
 // Bound: memory.  The rotation reads and writes every element once (its gradient is the same kernel with the opposite angle); the norm's
 // gradient reads x and dy and recomputes r, so the forward keeps nothing for it.
@@ -299,7 +299,9 @@ __global__ __launch_bounds__(ROT_THREADS) void headnorm_bwd_kernel(const RotGeom
                 if (K > 1)
                     for (int d = g.lpr >> 1; d; d >>= 1) { ss += __shfl_xor(ss, d); dot += __shfl_xor(dot, d); }
                 const float r = rsqrtf(ss / (float)g.D + eps);
-                const float f = r * r * r * dot / (float)g.D;
+                // mean of w u xhat: with xhat = x r and this every factor stays near the result's size, where x r^3 leaves fp32 for rows of rms
+                // 1e13 and more or 1e-13 and less
+                const float proj = dot * r / (float)g.D;
 #pragma unroll
                 for (int m = 0; m < K; ++m) {
                     if (!on[m]) continue;
@@ -315,8 +317,8 @@ __global__ __launch_bounds__(ROT_THREADS) void headnorm_bwd_kernel(const RotGeom
                     }
 #pragma unroll
                     for (int i = 0; i < C; ++i) {
-                        ua[m][i] = fmaf(r, ua[m][i], -(f * a[m][i]));
-                        ub[m][i] = fmaf(r, ub[m][i], -(f * b[m][i]));
+                        ua[m][i] = r * fmaf(-proj, a[m][i] * r, ua[m][i]);
+                        ub[m][i] = r * fmaf(-proj, b[m][i] * r, ub[m][i]);
                     }
                     store_pairs<T, C, NB>(dx, o1[m], o2[m], ua[m], ub[m]);
                 }
