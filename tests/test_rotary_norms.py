@@ -368,3 +368,34 @@ def test_norm_gradients_of_very_large_and_very_small_rows(d, hq, hk, dtype):
     m = HeadNormRotary(d, eps=1e-30).to(DEV)
     q[2] = 0.0
     _norm_gradients(q, k, m, 1e-30)
+
+
+@gpu
+def test_norm_gradients_of_the_most_tokens_that_are_counted():
+    """Close to 2^31 rows of one head of 2 values, all the same row; a lane adds the weights' terms of 2^31 / (64 tokens x 4096 waves) = 8192 of them
+    one after the other in fp32."""
+    from uncrtaints_amd import engine as E
+    n = 2 ** 31 - 1
+    x, g = (torch.tensor(v, dtype=torch.bfloat16, device=DEV).view(1, 1, 2).expand(n, 1, 2) for v in ([3.0, 4.0], [1.0, -2.0]))
+    w = torch.tensor([1.0, 0.5], device=DEV)
+    dq, dk, dwq, dwk = E.headnorm_rotary_backward(g, g, x, x, w, w, 0.0, E.RotaryPlan())
+    x64, g64, w64 = (t.double().cpu() for t in (x[0, 0], g[0, 0], w))
+    r = 1.0 / x64.square().mean().sqrt()
+    xh = x64 * r
+    ref = r * (w64 * g64 - xh * (w64 * g64 * xh).mean())
+    for dx in (dq, dk):
+        _check("dx", dx[0, 0], ref, 64 * U * r * 10 + _half(torch.bfloat16) * ref.abs())
+        rows = dx.view(-1).view(torch.int32)
+        assert bool((rows == rows[0]).all())
+    for dw in (dwq, dwk):
+        assert bool(((dw.double().cpu() / n - g64 * xh).abs() <= (64 + 8192) * U * (g64 * xh).abs()).all())
+
+
+def test_norm_gradients_refuse_tiles_that_are_not_counted():
+    from uncrtaints_amd import hip_backend as hb
+    name = "uncr_headnorm_rotary_bwd"
+    ok = dict.fromkeys([n for _, n in hb.parse_header()[name]], 0)
+    ok.update(q=20, k=20, gq=20, gk=20, dq=20, dk=20, wq=16, wk=16, part=16, dwq=16, dwk=16, pos=None, turns=None, eps=1.0, N=2 ** 31 - 1, Hq=1, Hk=1, D=256,
+              stream=None)          # rows that start at no vector boundary: a wave takes one token at a time
+    fn = hb.lib().fn[name]
+    assert fn(*ok.values()) == fn(*{**ok, "Hq": 0}.values()) < 0

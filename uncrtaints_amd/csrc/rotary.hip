@@ -214,7 +214,7 @@ struct GradSet { const void* x; const void* dy; void* dx; const float* w; long l
 // one row of partials: their sum in the next launch is in a fixed order, no atomics
 template <typename T, int C, int K, bool NB>
 __global__ __launch_bounds__(ROT_THREADS) void headnorm_bwd_kernel(const RotGeom g, const GradSet q, const GradSet k, float eps,
-                                                                   float* __restrict__ part) {
+                                                                   int tiles, float* __restrict__ part) {
     extern __shared__ float2 shared_cs[];
     __shared__ alignas(16) float red[ROT_THREADS / 64][2][ROT_MAX_D];
     const int wave = threadIdx.x >> 6;
@@ -230,7 +230,6 @@ __global__ __launch_bounds__(ROT_THREADS) void headnorm_bwd_kernel(const RotGeom
 #pragma unroll
         for (int i = 0; i < C; ++i) dwa[0][m][i] = dwb[0][m][i] = dwa[1][m][i] = dwb[1][m][i] = 0.f;
     }
-    const int tiles = (g.N + g.tok - 1) / g.tok;
     for (int tile = blockIdx.x * (ROT_THREADS / 64) + wave; tile < tiles; tile += gridDim.x * (ROT_THREADS / 64)) {
         const int token0 = tile * g.tok, token = token0 + t;
         __builtin_amdgcn_wave_barrier();
@@ -418,7 +417,7 @@ int geom(RotGeom& g, const void* pos, int pos_dt, int n_axes, int s0, int s1, in
 }
 
 struct Fwd { static constexpr int MAX_C = 8; RotGeom g; HeadSet q, k; float eps; int items; hipStream_t stream; };
-struct Bwd { static constexpr int MAX_C = 4; RotGeom g; GradSet q, k; float eps; int items, blocks; float* part; hipStream_t stream; };
+struct Bwd { static constexpr int MAX_C = 4; RotGeom g; GradSet q, k; float eps; int items, blocks, tiles; float* part; hipStream_t stream; };
 
 size_t lds_bytes(const RotGeom& g) { return (size_t)(ROT_THREADS / 64) * g.tok * (g.D / 2) * sizeof(float2); }
 
@@ -431,7 +430,7 @@ template <typename T, bool NB, bool NORM, int C, int K> void run(const Fwd& f) {
     hipLaunchKernelGGL((rotary_kernel<T, C, K, NB, NORM>), dim3((unsigned)(((long long)f.g.N + per - 1) / per)), dim3(ROT_THREADS), lds_bytes(f.g), f.stream, f.g, f.q, f.k, f.eps);
 }
 template <typename T, bool NB, bool NORM, int C, int K> void run(const Bwd& b) {
-    hipLaunchKernelGGL((headnorm_bwd_kernel<T, C, K, NB>), dim3(b.blocks), dim3(ROT_THREADS), lds_bytes(b.g), b.stream, b.g, b.q, b.k, b.eps, b.part);
+    hipLaunchKernelGGL((headnorm_bwd_kernel<T, C, K, NB>), dim3(b.blocks), dim3(ROT_THREADS), lds_bytes(b.g), b.stream, b.g, b.q, b.k, b.eps, b.tiles, b.part);
 }
 // the widest vector is 16 bytes: 16 / size pairs of halves, 8 / size pairs of neighbours
 template <typename T, bool NB, bool NORM, typename Job> void launch_c(const Job& j, int c) {
@@ -508,10 +507,12 @@ extern "C" int uncr_headnorm_rotary_bwd(const void* q, long long q_ts, long long
         const long long st[] = {q_ts, q_hs, k_ts, k_hs, gq_ts, gq_hs, gk_ts, gk_hs, (long long)D};
         const void* const pt[] = {q, k, gq, gk, dq, dk};
         const int c = pick_c(g, st, 9, pt, 6, act ? 2 : 4, Bwd::MAX_C, wq, wk), items = shape(g, c, Hq + Hk);
-        const long long tiles = ((long long)N + per_block(g) - 1) / per_block(g);
-        blocks = tiles < ROT_MAX_SLOTS ? (int)tiles : ROT_MAX_SLOTS;
+        // a wave's tiles; their numbers are counted in 32 bits, up to a round of all waves behind the last one
+        const long long tiles = ((long long)N + g.tok - 1) / g.tok, wanted = ((long long)N + per_block(g) - 1) / per_block(g);
+        blocks = wanted < ROT_MAX_SLOTS ? (int)wanted : ROT_MAX_SLOTS;
+        if (tiles + (long long)blocks * (ROT_THREADS / 64) > 0x7fffffffll) return UNCR_ESHAPE;
         const GradSet zq = {q, gq, dq, wq, q_ts, q_hs, gq_ts, gq_hs, Hq}, zk = {k, gk, dk, wk, k_ts, k_hs, gk_ts, gk_hs, Hk};
-        launch<true>(Bwd{g, zq, zk, eps, items, blocks, part, stream}, c, act);
+        launch<true>(Bwd{g, zq, zk, eps, items, blocks, (int)tiles, part, stream}, c, act);
         UNCR_LAUNCH_CHECK();
     }
     hipLaunchKernelGGL(headnorm_dw_kernel, dim3((2 * D + 15) / 16), dim3(1024), 0, stream, part, blocks, D, dwq, dwk);
