@@ -399,3 +399,54 @@ def test_norm_gradients_refuse_tiles_that_are_not_counted():
               stream=None)          # rows that start at no vector boundary: a wave takes one token at a time
     fn = hb.lib().fn[name]
     assert fn(*ok.values()) == fn(*{**ok, "Hq": 0}.values()) < 0
+
+
+def test_forward_mode_tangents_are_refused():
+    """A result without a tangent would pass for one whose derivative is 0.  Refused before anything is launched (no GPU here), through dual tensors
+    and through functional transforms, in the forward and in a backward whose incoming gradient is dual."""
+    import torch.autograd.forward_ad as fw
+    from uncrtaints_amd import engine as E
+    from uncrtaints_amd.src.backbones.packed_attention import HeadNormRotary, PackedAttention, pack_offsets
+    from uncrtaints_amd.src.backbones.positional_encoding import RotaryAxes
+    x, pos, off, w = torch.ones(3, 2, 8), torch.zeros(3, 2), pack_offsets([3], "cpu"), torch.ones(8)
+    r = RotaryAxes(8, sections=(4, 4))
+    norm, plain, attend = HeadNormRotary(8, rotary=r), HeadNormRotary(8), PackedAttention()
+    calls = [lambda t: r(t, pos), lambda t: norm(t, x, pos), lambda t: norm(x, t, pos), lambda t: plain(x, t), lambda t: attend(t, x, x, off),
+             lambda t: attend(x, t, x, off), lambda t: attend(x, x, t, off), lambda t: E.rotary_axes(t, E.RotaryPlan(), inverse=True),
+             lambda t: E.headnorm_rotary_backward(t, x, x, x, w, w, 1e-6, E.RotaryPlan()),
+             lambda t: E.headnorm_rotary_backward(x, t, x, x, w, w, 1e-6, E.RotaryPlan()),
+             lambda t: E.packed_attention_backward(t, x, x, x, x, w, off, off, None, 1.0, False)]
+    for call in calls:
+        for grad in (True, False):
+            with torch.set_grad_enabled(grad), fw.dual_level(), pytest.raises(NotImplementedError, match="tangent"):
+                call(fw.make_dual(x, x))
+            with torch.set_grad_enabled(grad), pytest.raises(NotImplementedError, match="tangent"):
+                torch.func.jvp(call, (x,), (x,))
+    with fw.dual_level():
+        with pytest.raises(NotImplementedError, match="positions"):
+            r.plan(fw.make_dual(pos, pos), (3,), pos.device)
+        del norm.k_weight
+        norm.k_weight = fw.make_dual(w, w)
+        with pytest.raises(NotImplementedError, match="k_weight"):
+            norm(x, x, pos)
+        with pytest.raises(RuntimeError, match="cuda device"):          # a level without tangents refuses nothing
+            r(x, pos)
+
+
+@gpu
+def test_forward_mode_tangents_are_refused_on_the_gpu():
+    import torch.autograd.forward_ad as fw
+    from uncrtaints_amd.src.backbones.packed_attention import HeadNormRotary, PackedAttention, pack_offsets
+    x, off = torch.ones(3, 2, 8, device=DEV), pack_offsets([3], DEV)
+    leaf = x.clone().requires_grad_()
+    r = _module(8, ((8, 100.0),), "halves").to(DEV)
+    pos = torch.ones(3, 1, device=DEV)
+    attend, norm = PackedAttention(), HeadNormRotary(8, rotary=r).to(DEV)
+    with fw.dual_level():
+        dual = fw.make_dual(x, x)
+        for call in (lambda t: r(t, pos), lambda t: norm(t, x, pos), lambda t: attend(x, x, t, off)):
+            with pytest.raises(NotImplementedError, match="tangent"):
+                call(dual)
+        for y in (r(leaf, pos), norm(leaf, x, pos)[0], attend(leaf, x, x, off)):
+            with pytest.raises(NotImplementedError, match="tangent"):
+                torch.autograd.grad(y, leaf, dual)

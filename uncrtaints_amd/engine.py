@@ -20,6 +20,7 @@ from dataclasses import dataclass
 from typing import Dict, Optional, Tuple
 
 import torch
+from torch.autograd import forward_ad
 
 from . import hip_backend as hb
 
@@ -2163,6 +2164,15 @@ def _on(dev):
     return _HERE if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
 
 
+def refuse_tangents(**tensors):
+    """The kernels have no forward-mode derivative: a tensor with a tangent is refused, its result would come back without one."""
+    if forward_ad._current_level < 0:          # no forward-mode differentiation under way, as unpack_dual decides it
+        return
+    for name, t in tensors.items():
+        if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+            raise NotImplementedError(f"{name} carries a forward-mode tangent: no forward-mode derivative is built")
+
+
 def check_tokens(**tensors):
     """Token rows [tokens, heads, d]: storage type, common type and device.  Raises before anything is launched."""
     first = None
@@ -2177,6 +2187,7 @@ def check_tokens(**tensors):
 
 
 def check_device(**tensors):
+    refuse_tangents(**tensors)
     dev = None
     for name, t in tensors.items():
         if t is None:
@@ -2214,6 +2225,7 @@ class RotaryPlan:
 
 def rotary_axes(x: Tensor, plan: RotaryPlan, inverse: bool = False) -> Tensor:
     """x [N, H, D] rotated (back, with `inverse`) by the plan's positions -> contiguous [N, H, D]"""
+    refuse_tangents(x=x)
     x = _token_rows(x)
     N, H, D = x.shape
     with _on(x.device):
@@ -2237,6 +2249,7 @@ def headnorm_rotary_forward(q: Tensor, k: Tensor, wq: Tensor, wk: Tensor, eps: f
 
 def headnorm_rotary_backward(gq: Tensor, gk: Tensor, q: Tensor, k: Tensor, wq: Tensor, wk: Tensor, eps: float, plan: RotaryPlan):
     """-> dq [N, Hq, D], dk [N, Hk, D] in the storage type, dwq [D], dwk [D] in fp32"""
+    refuse_tangents(gq=gq, gk=gk)
     q, k, gq, gk = _token_rows(q), _token_rows(k), _token_rows(gq), _token_rows(gk)
     N, Hq, D = q.shape
     Hk = k.shape[1]
@@ -2273,6 +2286,7 @@ def packed_attention_forward(q: Tensor, k: Tensor, v: Tensor, off_q: Tensor, off
 def packed_attention_backward(dout: Tensor, q: Tensor, k: Tensor, v: Tensor, out: Tensor, lse: Tensor, off_q: Tensor, off_k: Tensor,
                               k_len: Optional[Tensor], temperature: float, causal: bool, max_q: int = 0, max_k: int = 0):
     """-> dq [Nq, Hq, D], dk, dv [Nk, Hk, D] in the storage type"""
+    refuse_tangents(dout=dout)
     q, k, v, dout = _token_rows(q), _token_rows(k), _token_rows(v), _token_rows(dout)
     Nq, Hq, D = q.shape
     Nk, Hk, _ = k.shape
