@@ -450,3 +450,15 @@ def test_forward_mode_tangents_are_refused_on_the_gpu():
         norm.k_weight = fw.make_dual(torch.ones(8, device=DEV), torch.ones(8, device=DEV))
         with pytest.raises(NotImplementedError, match="k_weight"):
             norm(x, x, pos)
+
+
+def test_norm_weights_of_another_size_are_refused():
+    """A replaced parameter: the kernels read d values of each."""
+    from uncrtaints_amd.src.backbones.packed_attention import HeadNormRotary
+    x = torch.zeros(3, 2, 8)
+    for name in ("q_weight", "k_weight"):
+        for w in (torch.ones(7), torch.ones(1), torch.ones(()), torch.ones(9), torch.ones(2, 8), torch.ones(0)):
+            m = HeadNormRotary(8)
+            setattr(m, name, torch.nn.Parameter(w))
+            with pytest.raises(ValueError, match=name):
+                m(x, x)

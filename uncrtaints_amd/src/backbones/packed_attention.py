@@ -55,6 +55,9 @@ class HeadNormRotary(nn.Module):
             raise ValueError(f"q has tokens {tuple(q.shape[:-2])}, k {tuple(k.shape[:-2])}")
         if self.q_weight.dtype != torch.float32 or self.k_weight.dtype != torch.float32:
             raise RuntimeError("the norms' weights stay float32 (activations may be bfloat16)")
+        for name, w in (("q_weight", self.q_weight), ("k_weight", self.k_weight)):
+            if w.shape != (self.d,):
+                raise ValueError(f"{name}: expected [{self.d}], got {tuple(w.shape)}")
         if (positions is None) != (self.rotary is None):
             raise ValueError("positions are required with a rotary, and only with one")
         E.check_tokens(q=q, k=k)
