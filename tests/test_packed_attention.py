@@ -684,3 +684,43 @@ def test_the_sums_of_joining_waves_stay_inside_one_lds_object(tmp_path):
     assert status == 0, said
     status, said = _compiles(tmp_path, "__shared__ AttnBuffers<__bf16, 128, 32> b; out[0] = b.template join<4>(3)[0];")
     assert status != 0 and "do not hold the sums" in said
+
+
+def test_extent_of_a_tensor():
+    from uncrtaints_amd import engine as E
+    z = torch.zeros(4, 6, 8)
+    at = z.data_ptr()
+    assert E.extent(z) == (at, at + 4 * 192) and E.extent(z[1:3]) == (at + 4 * 48, at + 4 * 144) and E.extent(z[:0]) == (z[:0].data_ptr(),) * 2
+    assert E.extent(z[:, 1:3]) == (at + 4 * 8, at + 4 * (144 + 24)) and E.extent(z[..., ::2]) == (at, at + 4 * 191)
+    assert E.extent(z[:1].expand(9, 6, 8)) == (at, at + 4 * 48) and E.extent(z.transpose(0, 2)) == E.extent(z)
+
+
+@gpu
+def test_out_beside_the_inputs_in_one_buffer():
+    """A workspace that a program cuts up itself: rows that do not overlap are served, any that do are refused, the offsets' among them."""
+    from uncrtaints_amd.src.backbones.packed_attention import PackedAttention, pack_offsets
+    m = PackedAttention()
+    z = torch.randn(4 * 6 + 1, 4, 8, generator=_gen(8)).to(DEV)
+    q, k, v, out = (z[6 * i:6 * i + 6] for i in range(4))
+    off = pack_offsets([2, 4], DEV)
+    want = m(q, k, v, off)
+    kept = z.clone()
+    got = m(q, k, v, off, out=out)
+    assert got.data_ptr() == out.data_ptr() and torch.equal(out, want)
+    kept[18:24] = want
+    assert torch.equal(z, kept)
+    z[24].view(-1)[:3] = off.view(torch.float32)
+    inside = z[24].view(-1)[:3].view(torch.int32)
+    assert torch.equal(m(q, k, v, inside, out=out), want)
+    for bad in (z[17:23], z[1:7], z[11:17]):
+        with pytest.raises(ValueError, match="shares"):
+            m(q, k, v, off, out=bad)
+    with pytest.raises(ValueError, match="shares"):
+        m(q, k, v, inside, out=z[19:25])
+    with pytest.raises(ValueError, match="shares"):
+        m(q, k, v, off, offsets_k=off, k_len=inside[1:], out=z[19:25])
+    with pytest.raises(ValueError, match="shares"):          # rows of a strided input around it
+        m(z[::4][:6], k, v, off, out=out)
+    assert torch.equal(z[:18], kept[:18])
+    empty = torch.zeros(0, 4, 8, device=DEV)
+    assert m(empty, k, v, torch.zeros(2, dtype=torch.int32, device=DEV), torch.tensor([0, 6], dtype=torch.int32, device=DEV), out=empty).shape == (0, 4, 8)

@@ -2200,6 +2200,12 @@ def check_device(**tensors):
             raise RuntimeError(f"{name} is on {t.device}, the other tensors on {dev}")
 
 
+def extent(x: Tensor) -> Tuple[int, int]:
+    """Addresses of a tensor's first byte and of the one behind its last (equal for a tensor without values)"""
+    at = x.data_ptr()
+    return at, at + (x.element_size() * (1 + sum((n - 1) * s for n, s in zip(x.shape, x.stride()))) if x.numel() else 0)
+
+
 def _token_rows(x: Tensor) -> Tensor:
     """[tokens, heads, d] with d contiguous; token and head strides stay as they are (a slice of a fused projection is read in place)."""
     if x.shape[0] > 0x7fffffff:

@@ -114,7 +114,8 @@ class PackedAttention(nn.Module):
       sees one of those is not finite itself; one whose scores are all -infinity counts as a row that sees nothing.
       max_q, max_k: the longest sequences as far as the program knows them; they choose among the kernels (few rows per sequence over a cache,
       short sequences) and change nothing else: a wrong one costs time.
-      out: written in place of a new tensor (only without gradients, in memory of its own); rows of no sequence stay as they were.
+      out: contiguous, written in place of a new tensor (only without gradients); rows of no sequence stay as they were.  No input may reach into
+      its memory, from an input's first value to its last one.  Where d is a multiple of 4 it starts at a multiple of 4 values.
       return_lse: also the logarithm of each row's sum of exponentials [Nq, heads], fp32, without a gradient; -inf where a row sees nothing.
 
     Serving: one query row per sequence (offsets_q = 0, 1, 2, ...) against a cache [B * room, kv_heads, d] with offsets_k = b * room and k_len."""
@@ -166,9 +167,10 @@ class PackedAttention(nn.Module):
                     raise ValueError(f"out {tuple(out.shape)}: a contiguous tensor of q's shape {tuple(q.shape)} is required")
                 if out.requires_grad:
                     raise ValueError("out is for calls without gradients: it requires one")
-                at = out.untyped_storage().data_ptr()
-                if at and any(t.untyped_storage().data_ptr() == at for t in (q, k, v)):
-                    raise ValueError("out shares memory with an input")
+                first, behind = E.extent(out)
+                for t in (q, k, v, offsets_q, offsets_k, k_len):
+                    if t is not None and E.extent(t)[0] < behind and first < E.extent(t)[1]:
+                        raise ValueError("out shares memory with an input")
             res, lse = E.packed_attention_forward(q, k, v, offsets_q, offsets_k, k_len, temperature, self.causal, return_lse, out, *hints)
             if out is not None:
                 torch.autograd.graph.increment_version(out)         # a graph that saved it has to notice
