@@ -24,19 +24,29 @@ FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-fno-slp-vector
 
 
 def source_sha() -> str:
-    """sha256 (first 16 hex digits) over the kernel sources: measurements that depend on the kernels' code (the PMC traffic
-    file under profiles/) record it, and bench.py only attaches them while it still matches."""
+    """sha256 (first 16 hex digits) over the kernel sources and the flags they are compiled with: measurements that depend on the kernels'
+    code (the PMC traffic file under profiles/) record it, and bench.py only attaches them while it still matches."""
     import hashlib
     h = hashlib.sha256()
     for f in sorted(os.listdir(CSRC)):
         if f.endswith((".hip", ".h")) and f != "dev_probes.hip":
             h.update(f.encode())
             h.update(open(os.path.join(CSRC, f), "rb").read())
+    h.update(repr((FLAGS, SOURCES)).encode())
     return h.hexdigest()[:16]
 
 
 def _newer(src, dst):
     return (not os.path.exists(dst)) or os.path.getmtime(src) > os.path.getmtime(dst)
+
+
+def _made_by(out):
+    """The flags that made a built file, as recorded beside it (None: not known)"""
+    try:
+        with open(out + ".flags") as f:
+            return f.read()
+    except FileNotFoundError:
+        return None
 
 
 def build_lib(force: bool = False, verbose: bool = False) -> str:
@@ -45,28 +55,38 @@ def build_lib(force: bool = False, verbose: bool = False) -> str:
     objdir = os.path.join(LIBDIR, "obj")
     os.makedirs(objdir, exist_ok=True)
     hdrs = [os.path.join(CSRC, h) for h in os.listdir(CSRC) if h.endswith(".h")]
-    jobs = []
-    for s, extra, o in SOURCES:
-        src, obj = os.path.join(CSRC, s + ".hip"), os.path.join(objdir, o + ".o")
-        if force or _newer(src, obj) or any(_newer(h, obj) for h in hdrs):
-            jobs.append([hipcc, *FLAGS, *extra, "-c", src, "-o", obj])
 
-    def run(cmd):
+    def stale(out, sources, flags):
+        """A file is made again if a source is newer or if other flags made it: objects of two sets of flags are not linked together"""
+        return force or any(_newer(s, out) for s in sources) or _made_by(out) != " ".join(flags)
+
+    def run(job):
+        out, flags, inputs = job
+        cmd = [hipcc, *flags, *inputs, "-o", out]
         if verbose:
             print(" ".join(cmd), flush=True)
+        if os.path.exists(out + ".flags"):
+            os.remove(out + ".flags")
         r = subprocess.run(cmd, capture_output=True, text=True)
         if r.returncode != 0:
             raise RuntimeError("hipcc failed:\n" + " ".join(cmd) + "\n" + r.stdout + r.stderr)
+        with open(out + ".flags", "w") as f:
+            f.write(" ".join(flags))
 
+    jobs = []
+    for s, extra, o in SOURCES:
+        src, obj, flags = os.path.join(CSRC, s + ".hip"), os.path.join(objdir, o + ".o"), [*FLAGS, *extra, "-c"]
+        if stale(obj, [src, *hdrs], flags):
+            jobs.append((obj, flags, [src]))
     if jobs:
         with ThreadPoolExecutor(max_workers=min(13, len(jobs))) as ex:
             list(ex.map(run, jobs))
-    objs = [os.path.join(objdir, o + ".o") for _, _, o in SOURCES]
-    if force or jobs or not os.path.exists(LIB):
-        run([hipcc, "--offload-arch=gfx950", "-shared", "-fPIC", "-o", LIB, *objs])
-    dsrc = os.path.join(CSRC, "dev_probes.hip")
-    if force or _newer(dsrc, DEV_LIB) or any(_newer(h, DEV_LIB) for h in hdrs):
-        run([hipcc, *FLAGS, "-shared", "-o", DEV_LIB, dsrc])
+    objs, link = [os.path.join(objdir, o + ".o") for _, _, o in SOURCES], ["--offload-arch=gfx950", "-shared", "-fPIC"]
+    if jobs or stale(LIB, objs, link):
+        run((LIB, link, objs))
+    dsrc, flags = os.path.join(CSRC, "dev_probes.hip"), [*FLAGS, "-shared"]
+    if stale(DEV_LIB, [dsrc, *hdrs], flags):
+        run((DEV_LIB, flags, [dsrc]))
     return LIB
 
 
