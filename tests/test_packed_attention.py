@@ -724,3 +724,58 @@ def test_out_beside_the_inputs_in_one_buffer():
     assert torch.equal(z[:18], kept[:18])
     empty = torch.zeros(0, 4, 8, device=DEV)
     assert m(empty, k, v, torch.zeros(2, dtype=torch.int32, device=DEV), torch.tensor([0, 6], dtype=torch.int32, device=DEV), out=empty).shape == (0, 4, 8)
+
+
+# The instances that only launches of 1024 blocks and more take (whole blocks of rows, four pairs of waves in dK/dV, with and without tiles in
+# descending order of work), over long sequences: many key heads that repeat three, so that the reference has only those to make.
+WIDE = [   # lengths, key heads, queries per key head, d, types, aligned rows
+    ([1700, 900, 1800], 64, 1, 128, (torch.bfloat16, torch.float32), True),
+    ([1700, 900, 1800], 64, 1, 64, (torch.bfloat16, torch.float32), True),
+    ([1700, 900, 1800], 64, 1, 32, (torch.bfloat16, torch.float32), True),
+    ([1300, 0, 1500], 64, 1, 20, (torch.bfloat16, torch.float32), True),
+    ([1700, 1, 1800], 64, 1, 72, (torch.bfloat16,), True),
+    ([1100, 1300], 16, 8, 128, (torch.bfloat16,), True),
+    ([1100, 1300], 64, 1, 32, (torch.float32, torch.bfloat16), False),
+    ([1100, 1300], 64, 1, 64, (torch.float32, torch.bfloat16), False),
+    ([1400, 1500], 64, 2, 127, (torch.bfloat16, torch.float32), False),
+    ([400, 300, 500, 480], 64, 2, 64, (torch.float32,), True),
+]
+
+
+@gpu
+@MASK
+@pytest.mark.parametrize("lens,hk,G,d,dtype,aligned", [(*w[:4], t, w[5]) for w in WIDE for t in w[4]])
+def test_launches_of_many_blocks_over_long_sequences(lens, hk, G, d, dtype, aligned, causal):
+    from uncrtaints_amd.src.backbones.packed_attention import PackedAttention
+    n, g, base = sum(lens), _gen(80 + d), 3
+    q, k, v, do = (torch.randn(n, h, d, generator=g).to(dtype) for h in (base * G, base, base, base * G))
+
+    def repeat(t, per):          # [n, base * per, d] -> [n, hk * per, d], key head c repeating c % base
+        idx = torch.cat([torch.arange(per) + c % base * per for c in range(hk)])
+        t = t.to(DEV)[:, idx.to(DEV)]
+        if aligned:
+            return t
+        z = torch.empty(n, t.shape[1] * d + 3, dtype=dtype, device=DEV)
+        z[:, 1:1 + t.shape[1] * d] = t.flatten(1)
+        return z[:, 1:1 + t.shape[1] * d].unflatten(1, (t.shape[1], d))
+
+    leaves = [repeat(t, per).detach().requires_grad_() for t, per in ((q, G), (k, 1), (v, 1))]
+    off = _offsets(lens)
+    out, lse = PackedAttention(causal=causal)(*leaves, off.to(DEV), return_lse=True)
+    got = dict(zip(("out", "lse", "dq", "dk", "dv"), (out.detach(), lse, *torch.autograd.grad(out, leaves, repeat(do, G)))))
+    for name, t in got.items():          # the heads that repeat the first three are equal to them, bit for bit
+        per = G if name in ("out", "lse", "dq") else 1
+        for c in range(base, hk):
+            assert torch.equal(t[:, c * per:(c + 1) * per], t[:, c % base * per:(c % base + 1) * per]), (name, c)
+        got[name] = t[:, :base * per].cpu()
+    for b, length in enumerate(lens):
+        rows = slice(int(off[b]), int(off[b]) + length)
+        for c in range(base):
+            hs = slice(c * G, (c + 1) * G)
+            ref = reference(q[rows, hs].double().transpose(0, 1), k[rows, c].double(), v[rows, c].double(), do[rows, hs].double().transpose(0, 1), causal,
+                            math.sqrt(d), dtype)
+            for name in ("out", "dq"):
+                _check(name, got[name][rows, hs], *(t.transpose(0, 1) for t in ref[name]))
+            _check("lse", got["lse"][rows, hs], *(t.T for t in ref["lse"]))
+            for name in ("dk", "dv"):
+                _check(name, got[name][rows, c], *ref[name])
