@@ -726,26 +726,8 @@ def test_out_beside_the_inputs_in_one_buffer():
     assert m(empty, k, v, torch.zeros(2, dtype=torch.int32, device=DEV), torch.tensor([0, 6], dtype=torch.int32, device=DEV), out=empty).shape == (0, 4, 8)
 
 
-# The instances that only launches of 1024 blocks and more take (whole blocks of rows, four pairs of waves in dK/dV, with and without tiles in
-# descending order of work), over long sequences: many key heads that repeat three, so that the reference has only those to make.
-WIDE = [   # lengths, key heads, queries per key head, d, types, aligned rows
-    ([1700, 900, 1800], 64, 1, 128, (torch.bfloat16, torch.float32), True),
-    ([1700, 900, 1800], 64, 1, 64, (torch.bfloat16, torch.float32), True),
-    ([1700, 900, 1800], 64, 1, 32, (torch.bfloat16, torch.float32), True),
-    ([1300, 0, 1500], 64, 1, 20, (torch.bfloat16, torch.float32), True),
-    ([1700, 1, 1800], 64, 1, 72, (torch.bfloat16,), True),
-    ([1100, 1300], 16, 8, 128, (torch.bfloat16,), True),
-    ([1100, 1300], 64, 1, 32, (torch.float32, torch.bfloat16), False),
-    ([1100, 1300], 64, 1, 64, (torch.float32, torch.bfloat16), False),
-    ([1400, 1500], 64, 2, 127, (torch.bfloat16, torch.float32), False),
-    ([400, 300, 500, 480], 64, 2, 64, (torch.float32,), True),
-]
-
-
-@gpu
-@MASK
-@pytest.mark.parametrize("lens,hk,G,d,dtype,aligned", [(*w[:4], t, w[5]) for w in WIDE for t in w[4]])
-def test_launches_of_many_blocks_over_long_sequences(lens, hk, G, d, dtype, aligned, causal):
+def _wide(lens, hk, G, d, dtype, aligned, causal):
+    """Forward and backward with `hk` key heads that repeat three"""
     from uncrtaints_amd.src.backbones.packed_attention import PackedAttention
     n, g, base = sum(lens), _gen(80 + d), 3
     q, k, v, do = (torch.randn(n, h, d, generator=g).to(dtype) for h in (base * G, base, base, base * G))
@@ -779,3 +761,50 @@ def test_launches_of_many_blocks_over_long_sequences(lens, hk, G, d, dtype, alig
             _check("lse", got["lse"][rows, hs], *(t.T for t in ref["lse"]))
             for name in ("dk", "dv"):
                 _check(name, got[name][rows, c], *ref[name])
+
+
+# The instances that only launches of 1024 blocks and more take (whole blocks of rows, four pairs of waves in dK/dV, with and without tiles in
+# descending order of work), over long sequences: many key heads that repeat three, so that the reference has only those to make.
+WIDE = [   # lengths, key heads, queries per key head, d, types, aligned rows
+    ([1700, 900, 1800], 64, 1, 128, (torch.bfloat16, torch.float32), True),
+    ([1700, 900, 1800], 64, 1, 64, (torch.bfloat16, torch.float32), True),
+    ([1700, 900, 1800], 64, 1, 32, (torch.bfloat16, torch.float32), True),
+    ([1300, 0, 1500], 64, 1, 20, (torch.bfloat16, torch.float32), True),
+    ([1700, 1, 1800], 64, 1, 72, (torch.bfloat16,), True),
+    ([1100, 1300], 16, 8, 128, (torch.bfloat16,), True),
+    ([1100, 1300], 64, 1, 32, (torch.float32, torch.bfloat16), False),
+    ([1100, 1300], 64, 1, 64, (torch.float32, torch.bfloat16), False),
+    ([1400, 1500], 64, 2, 127, (torch.bfloat16, torch.float32), False),
+    ([400, 300, 500, 480], 64, 2, 64, (torch.float32,), True),
+    ([400, 300, 500, 480], 64, 2, 32, (torch.float32,), True),
+]
+
+
+@gpu
+@MASK
+@pytest.mark.parametrize("lens,hk,G,d,dtype,aligned", [(*w[:4], t, w[5]) for w in WIDE for t in w[4]])
+def test_launches_of_many_blocks_over_long_sequences(lens, hk, G, d, dtype, aligned, causal):
+    _wide(lens, hk, G, d, dtype, aligned, causal)
+
+
+@gpu
+@MASK
+@BOTH
+@pytest.mark.parametrize("aligned", [True, False])
+@pytest.mark.parametrize("G,d", [(1, 32), (1, 64), (1, 128), (3, 64), (2, 36), (1, 100)])
+def test_many_sequences_of_up_to_64_rows(G, d, aligned, dtype, causal):
+    """33 to 64 rows on average, enough sequences for 1024 blocks: blocks of two waves, forward and backward"""
+    lens = [int(n) for n in torch.randint(33 // G, 60 // G, (64,), generator=_gen(90 + G))] + [0, 130, 1]
+    _wide(lens, 24, G, d, dtype, aligned, causal)
+
+
+@gpu
+@BOTH
+@pytest.mark.parametrize("d", [16, 32, 64, 128])
+def test_wave_kernels_over_rows_that_start_at_no_vector_boundary(d, dtype):
+    _run([1] * 3, [700, 0, 130], 4, 2, d, True, dtype, room=[704, 3, 130], train=False, layout="odd_start")
+    _run([1, 2], [5000, 300], 8, 2, d, True, dtype, train=False, layout="odd_start", hints=False)
+    _run([20, 3, 40, 0, 31], [20, 3, 40, 0, 31], 3, 3, d, True, dtype, layout="odd_start")
+    _run([9, 3], [60, 33], 4, 2, d, False, dtype, layout="odd_start")
+    _run([70, 3, 131], [70, 3, 131], 4, 2, d, True, dtype, layout="odd_start")
+    _run([1] * 3, [700, 0, 130], 4, 2, d, True, dtype, room=[704, 3, 130], train=False)

@@ -462,3 +462,14 @@ def test_norm_weights_of_another_size_are_refused():
             setattr(m, name, torch.nn.Parameter(w))
             with pytest.raises(ValueError, match=name):
                 m(x, x)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("d,sections,pairs", [(202, ((66, 10000.0), (70, 100.0), (66, 100.0)), "neighbours"), (250, ((100, 10000.0), (90, 20.0)), "neighbours"),
+                                              (44, ((12, 100.0), (20, 50.0)), "halves"), (44, ((12, 100.0), (20, 50.0)), "neighbours")])
+def test_pairs_that_fill_no_vector(d, sections, pairs, dtype):
+    """More neighbours than a wave has lanes, one at a time; two pairs per lane"""
+    test_rotary_axes(d, sections, pairs, dtype, 37, 5)
+    for kind in ("plain", "odd_start"):
+        test_head_norm_rotary(kind, d, sections, pairs, dtype, 53, 6, 2)
