@@ -138,7 +138,7 @@ static inline int attn_slots(long long rows, int B, int shift) { return (int)(ro
 static inline bool attn_grid(long long blocks, int threads) { return blocks * threads <= 0xffffffffll; }
 
 // fp32 on the bf16 matrix units: x = x0 + x1 + x2 exactly to 24 bits, each rounded to bf16 from what the ones before leave, and
-//   a b = a0 b0 + a0 b1 + a1 b0 + a1 b1 + a0 b2 + a2 b0      (what is left out is below 2^-24 |a b|, a rounding of fp32)
+//   a b = a0 b0 + a0 b1 + a1 b0 + a1 b1 + a0 b2 + a2 b0      (left out: a1 b2 + a2 b1 of at most 2 * 2^-24 |a b|, two half steps of fp32)
 // -- six products at 16 times the rate of v_mfma_f32_32x32x2_f32.  A launch before lays the inputs out as rows [3][D rounded up to 8]
 // (attn_planes below); P and dS are taken apart in registers.
 struct AttnThree {};
@@ -306,8 +306,9 @@ template <> struct AttnProb<AttnThree> {
 };
 
 // The C registers of a 32-row product on their way through LDS from one wave to another, lane by lane, conflict-free.  With bf16 storage the
-// upper three bytes of each cross (17 significant bits): all four do not fit beside the tiles, and as bf16 P would take the rounding that
-// dS gets anyway a second time (dK's error against 64 bits 0.0030 instead of 0.0024).
+// upper three bytes of each cross, 16 significant bits: all four do not fit beside the tiles, and as bf16 P would take the rounding that
+// dS gets anyway a second time (dK's error against 64 bits 0.0030 instead of 0.0024).  The lowest byte is cut off, not rounded: P is up to
+// 2^-15 of itself too small, 1/128 of the half step that dS is rounded by right after.
 template <typename T> struct AttnPass;
 template <> struct AttnPass<__bf16> {
     static constexpr int PARTS = 3;

@@ -42,7 +42,10 @@ __global__ __launch_bounds__(256) void attn_planes_kernel(const Planes a, int D)
 
 }  // namespace
 
-// Long fp32 sequences: from 512 keys on average the products are worth the launch before them
+// Long fp32 sequences.  The launch before the products costs 10 bytes per element of all tensors, used or not; what it buys grows with the rows
+// that meet a key.  Forward, three parts beside fp32 products: 32 sequences of 600 keys, 16/4 heads of 64: 128 rows of each 95 against 125 us, 512 rows
+// 230 against 283; 8 of 8192 keys: 512 rows 748 against 1177.  The rule looks at the keys alone, and a few rows over a cache lose by it: 40 rows of
+// each, 8 heads of 64, over 8 caches of 8192 keys 628 against 372 us, over 512 used rows of such caches 162 against 30.
 bool attn_three(const AttnGeom& g, int act, bool vec) {
     return act == 0 && vec && g.D <= 64 && g.D % 4 == 0 && g.Nq > 0 && g.Nk / g.B >= 512 && attn_planes_floats(g, 2, 2) < (1ll << 30);
 }

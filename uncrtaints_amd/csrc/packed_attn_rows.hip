@@ -466,8 +466,12 @@ bool attn_short(const AttnGeom& g, int max_q, int max_k) {
     return max_q > 0 && max_k > 0 && (long long)max_q * g.G <= 64 && max_k <= 64 && g.D <= 64;
 }
 
-// Who shares a task.  Up to 32 rows per sequence (by the caller's word, else on average) are one wave's rows; more are better off in the
-// kernels of packed_attn.hip.  Without ranges (splits = 1) up to 8 tiles per wave; then ranges of 4096 keys, shorter ones while the launch
+// Who shares a task.  Up to 32 rows per sequence (by the caller's word, else on average) are one wave's rows; more go to the kernels of
+// packed_attn.hip, which read a key tile once for 128 or 256 rows and have no ranges.  Both sides, 16/4 heads of 128, bf16, packed_attn.hip against these
+// tiles of 32 rows with ranges: 64 caches of 2048 keys, 9 tokens each 111 against 153 us, 64 tokens 193 against 332; 24 of 32768, 64 tokens 949
+// against 1737.  Few blocks over long caches lose by the rule: 9 tokens over one cache of 32768 keys 692 against 50 us, over 24 of them 918 against
+// 503; one token, 64 heads on one key head of 64, one cache of 32768: 434 against 27.
+// Without ranges (splits = 1) up to 8 tiles per wave; then ranges of 4096 keys, shorter ones while the launch
 // has fewer than eight blocks per CU (caches are filled to different lengths), down to a tile per wave.
 AttnSplit attn_split(const AttnGeom& g, int max_q, int max_k, int act) {
     AttnSplit s = {0, 0, 1};

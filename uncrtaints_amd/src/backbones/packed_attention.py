@@ -31,7 +31,8 @@ class HeadNormRotary(nn.Module):
     y = rotate(weight * x / sqrt(mean(x^2) + eps)), the mean over the d values of one head.
 
     d: head size (even, at most 256); q_weight, k_weight: fp32 parameters [d], shared by the heads.  rotary: a
-    positional_encoding.RotaryAxes of the same head size, or None for the norms alone.
+    positional_encoding.RotaryAxes of the same head size, or None for the norms alone.  The sum of a head's squares is an fp32 number: values
+    from 1e-18 to 1e18, or smaller ones that eps outweighs.  eps may be 0; heads of zeros are NaN then.
 
     forward(q [..., heads, d], k [..., kv_heads, d], positions [..., axes]) -> (q, k), contiguous, in the inputs' storage type."""
 
@@ -104,14 +105,19 @@ class PackedAttention(nn.Module):
 
     forward(q [Nq, heads, d], k [Nk, kv_heads, d], v [Nk, kv_heads, d], offsets_q, offsets_k=None, k_len=None, ...) -> out [Nq, heads, d]
       heads is a multiple of kv_heads: query head i reads key head i // (heads // kv_heads).  d is at most 128.  fp32 or bf16; the softmax and
-      all sums are fp32 either way.  Inputs may be strided (slices of one projection, a cache of any layout with d contiguous).
+      all sums are fp32 either way.  With bf16 the probabilities, and in the backward pass dS, are rounded to bf16 before they are multiplied by
+      values, keys, queries or incoming gradients: gradients are off by about 1.4 times what the rounding of the result alone would leave (heads of
+      4 values: twice).  Scores q k / temperature are fp32 numbers, rounded by 2^-24 of their size, and so is the logarithm that gradients
+      take their probabilities from: scores of 2^20 leave gradients with one digit, and from 2^30 on a row may not be finite.
+      Inputs may be strided (slices of one projection, a cache of any layout with d contiguous).
       offsets_q, offsets_k [B + 1]: int32 on the device, not decreasing; sequence b owns rows offsets[b] .. offsets[b + 1] - 1 (`pack_offsets`).
       Without offsets_k the keys lie like the queries.  They are not read on the host; offsets outside the tensors are clamped on the device.
       Up to 2^30 keys, and 2^30 query rows times heads per key head.
       k_len [B]: int32, used rows of each key sequence; the rest is room in a cache, never read into a result.
       A row that sees no key is 0 and takes no part in any gradient.  Rows of no sequence are zeros, in the gradients too.  Keys and values
-      that a row does not see may hold anything, infinities and NaN included (gradients want all of a sequence's own rows finite).  A row that
-      sees one of those is not finite itself; one whose scores are all -infinity counts as a row that sees nothing.
+      that a row does not see may hold anything, infinities and NaN included (gradients want all of a sequence's own rows finite).  What a row
+      that sees an infinity holds is not defined: most often it is not finite; where its only trace is a score of -infinity it may be what the
+      other keys make it, or 0 like a row that sees nothing.  A row that sees NaN in a key is NaN, in a value NaN at its place.
       max_q, max_k: the longest sequences as far as the program knows them; they choose among the kernels (few rows per sequence over a cache,
       short sequences) and change nothing else: a wrong one costs time.
       out: contiguous, written in place of a new tensor (only without gradients); rows of no sequence stay as they were.  No input may reach into
