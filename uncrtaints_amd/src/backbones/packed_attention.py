@@ -106,7 +106,7 @@ class PackedAttention(nn.Module):
     forward(q [Nq, heads, d], k [Nk, kv_heads, d], v [Nk, kv_heads, d], offsets_q, offsets_k=None, k_len=None, ...) -> out [Nq, heads, d]
       heads is a multiple of kv_heads: query head i reads key head i // (heads // kv_heads).  d is at most 128.  fp32 or bf16; the softmax and
       all sums are fp32 either way.  With bf16 the probabilities, and in the backward pass dS, are rounded to bf16 before they are multiplied by
-      values, keys, queries or incoming gradients: gradients are off by about 1.4 times what the rounding of the result alone would leave (heads of
+      values, keys, queries or incoming gradients: gradients are off by about 1.5 times what the rounding of the result alone would leave (heads of
       4 values: twice).  Scores q k / temperature are fp32 numbers, rounded by 2^-24 of their size, and so is the logarithm that gradients
       take their probabilities from: scores of 2^20 leave gradients with one digit, and from 2^30 on a row may not be finite.
       Inputs may be strided (slices of one projection, a cache of any layout with d contiguous).
