@@ -808,3 +808,81 @@ def test_wave_kernels_over_rows_that_start_at_no_vector_boundary(d, dtype):
     _run([9, 3], [60, 33], 4, 2, d, False, dtype, layout="odd_start")
     _run([70, 3, 131], [70, 3, 131], 4, 2, d, True, dtype, layout="odd_start")
     _run([1] * 3, [700, 0, 130], 4, 2, d, True, dtype, room=[704, 3, 130], train=False)
+
+
+@gpu
+@BOTH
+def test_two_captured_graphs_with_workspaces_replayed_at_once(dtype):
+    """Ranges of a cache (partial results) and, in fp32, long sequences in three parts: each graph has a workspace of its own, so replays on two streams
+    at once, and eager calls between them, leave each other alone."""
+    from uncrtaints_amd.src.backbones.packed_attention import PackedAttention, pack_offsets
+    m = PackedAttention(causal=True)
+    one, lens = pack_offsets([1] * 3, DEV), pack_offsets([6000, 700, 30], DEV)
+    k, v = (torch.randn(6730, 2, 64, generator=_gen(i)).to(dtype).to(DEV) for i in (1, 2))
+    qs = [torch.randn(3, 8, 64, generator=_gen(10 + i)).to(dtype).to(DEV) for i in range(2)]
+    long = [torch.randn(6730, 4, 64, generator=_gen(20 + i)).to(dtype).to(DEV) for i in range(2)]
+    calls = [lambda i=i: (m(qs[i], k, v, one, lens, max_q=1, max_k=6000), m(long[i], k, v, lens)) for i in range(2)]
+    want = [c() for c in calls]
+    torch.cuda.synchronize()
+    graphs, held = [torch.cuda.CUDAGraph() for _ in range(2)], []
+    for g, c in zip(graphs, calls):
+        with torch.cuda.graph(g):
+            held.append(c())
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for turn in range(4):
+        for h in held:
+            for t in h:
+                t.fill_(7.0)
+        torch.cuda.synchronize()
+        for _ in range(3):
+            for g, s in zip(graphs, streams):
+                with torch.cuda.stream(s):
+                    g.replay()
+            eager = calls[turn % 2]()
+        torch.cuda.synchronize()
+        for i in range(2):
+            assert all(torch.equal(a, b) for a, b in zip(held[i], want[i])), (turn, i)
+        assert all(torch.equal(a, b) for a, b in zip(eager, want[turn % 2]))
+
+
+@gpu
+@BOTH
+@pytest.mark.parametrize("lens,hints", [([30, 9, 64], True), ([30, 9, 64], False), ([700, 600], False)])
+def test_broadcast_inputs_and_gradients(lens, hints, dtype):
+    """Heads that share one row in memory, one query for all tokens, and an incoming gradient that is one number: as where each has memory of its own."""
+    from uncrtaints_amd.src.backbones.packed_attention import PackedAttention, pack_offsets
+    n, off, m = sum(lens), pack_offsets(lens, DEV), PackedAttention(causal=True)
+    hints = dict(max_q=max(lens), max_k=max(lens)) if hints else {}
+    q1, k1, v1 = (torch.randn(*s, generator=_gen(30 + i)).to(dtype).to(DEV) for i, s in enumerate(((1, 4, 32), (n, 1, 32), (n, 1, 32))))
+    views = [q1.expand(n, 4, 32), k1.expand(n, 2, 32), v1.expand(n, 2, 32)]
+    got, want = [], []
+    for res, own in ((got, False), (want, True)):
+        leaves = [(t.contiguous() if own else t).detach().requires_grad_() for t in views]
+        y = m(*leaves, off, **hints)
+        res += [y.detach(), *torch.autograd.grad(y, leaves, torch.full_like(y, 0.5) if own else torch.full((1, 1, 1), 0.5, dtype=dtype, device=DEV).expand_as(y))]
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    base = [t.clone().requires_grad_() for t in (q1, k1, v1)]
+    y = m(*(t.expand(n, h, 32) for t, h in zip(base, (4, 2, 2))), off, **hints)
+    grads = torch.autograd.grad(y, base, torch.full_like(y, 0.5))
+    for g, w, dim in zip(grads, want[1:], (0, 1, 1)):
+        assert torch.equal(g, w.sum(dim, keepdim=True))
+
+
+@gpu
+@BOTH
+def test_inference_mode(dtype):
+    from uncrtaints_amd.src.backbones.packed_attention import HeadNormRotary, PackedAttention, pack_offsets
+    from uncrtaints_amd.src.backbones.positional_encoding import RotaryAxes
+    x, pos, off = torch.randn(20, 2, 16, generator=_gen(40)).to(dtype).to(DEV), torch.arange(20, device=DEV)[:, None], pack_offsets([11, 9], DEV)
+    norm, m = HeadNormRotary(16, rotary=RotaryAxes(16)).to(DEV), PackedAttention()
+
+    def path(**kw):
+        q, k = norm(x, x, pos)
+        return m(q, k, x, off, **kw).detach()
+
+    want = path()
+    with torch.inference_mode():
+        out = torch.empty_like(x)
+        assert torch.equal(path(), want) and torch.equal(path(out=out), want) and torch.equal(out, want)
+    with torch.no_grad():
+        assert torch.equal(path(out=out), want)
